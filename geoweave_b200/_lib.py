@@ -32,6 +32,7 @@ _load_error: Exception | None = None
 
 # name -> (restype, argtypes); the list mirrors include/geoweave_b200.h one to one
 _I64x3 = POINTER(c_int64)
+_I64x2 = POINTER(c_int64)
 SIGNATURES = {
     "gw_strerror": (c_char_p, [c_int]),
     "gw_last_cuda_error": (c_int, []),
@@ -84,6 +85,16 @@ SIGNATURES = {
     "gw_project_fused": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
                                  c_void_p, c_int, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_float,
                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "gw_packed_attn_fwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int64, c_int64, c_int, c_int, c_int, c_int64]),
+    "gw_packed_attn_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_int,
+                                   _I64x2, _I64x2, _I64x2, c_float, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p,
+                                   c_void_p]),
+    "gw_packed_attn_bwd_workspace_bytes": (c_size_t, [c_int64, c_int]),
+    "gw_packed_attn_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64,
+                                   c_int64, c_int, c_int, c_int, _I64x2, _I64x2, _I64x2, _I64x2, c_float, c_int, c_void_p, c_void_p,
+                                   c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "gw_rotary_axes": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int64, c_int, c_int, c_int, _I64x3, _I64x3, c_void_p, c_int, c_int,
+                               POINTER(c_int), c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
 }
 
 
@@ -154,6 +165,10 @@ def require_cuda(*tensors) -> torch.device:
 
 def i64x3(vals):
     return (c_int64 * 3)(*[int(v) for v in vals])
+
+
+def i64x2(vals):
+    return (c_int64 * 2)(*[int(v) for v in vals])
 
 
 # ---------------------------------------------------------------------------------------------

@@ -1,0 +1,107 @@
+// Attention over packed sequences: the problem description shared by its kernels, and how a block finds its work.
+//
+// Sequences lie back to back along the token axis; cu_q / cu_k (int32 [nseq + 1], on the device) hold their borders.  The
+// host never reads them: a grid is launched for the largest number of tiles that the totals allow,
+// floor(total / tile) + nseq, plus one, and each block finds its sequence by a warp-wide prefix sum over the lengths.
+// Blocks behind the last tile (one at least) share the rows behind the last sequence, which get zeros.
+#pragma once
+
+#include "gw_common.cuh"
+
+namespace gw {
+
+struct PackedParams {
+  const void *q, *k, *v;
+  const int32_t *cu_q, *cu_k;
+  int nseq;
+  int64_t total_q, total_k;
+  int H, Hk, D;
+  int64_t qs[2], ks[2], vs[2];  // element strides {token, head}
+  float scale;
+  int causal;
+  void* o;        // [total_q, H, D] contiguous
+  float* lse;     // [H, total_q] natural logarithm, nullable in the forward pass
+  // backward
+  const void* d_o;
+  int64_t dos[2];
+  float* delta;   // [H, total_q]: rowsum(d_o * o)
+  void *dq, *dk, *dv;  // contiguous
+  int* status;
+};
+
+// One sequence as its tiles see it; every field is in bounds whatever the border arrays hold.
+struct PackedSeq {
+  int q0, lq, k0, lk;  // first row and length on both sides
+  int tile;            // tile number within the sequence
+};
+
+__device__ __forceinline__ int packed_border(const int32_t* cu, int i, int64_t total) {
+  const int c = cu[i];
+  return c < 0 ? 0 : (c > total ? static_cast<int>(total) : c);
+}
+
+// Warp-wide: tile `slot` of the list of all sequences' tiles (tile_rows rows each, along the q or the k side).  True
+// when there is such a tile.  Otherwise *tiles is the number of tiles, *end the row behind the last sequence, and border
+// arrays that do not start at zero, decrease or pass the totals are reported.  All lanes get the same answers.
+__device__ __forceinline__ bool packed_find(const PackedParams& p, bool key_side, int tile_rows, int64_t slot, PackedSeq* out,
+                                            int64_t* tiles, int64_t* end) {
+  const int lane = threadIdx.x & 31;
+  int64_t base = 0;
+  bool bad = false;
+  for (int b0 = 0; b0 < p.nseq; b0 += 32) {
+    const int b = b0 + lane;
+    int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+    if (b < p.nseq) {
+      q0 = packed_border(p.cu_q, b, p.total_q);
+      q1 = packed_border(p.cu_q, b + 1, p.total_q);
+      k0 = packed_border(p.cu_k, b, p.total_k);
+      k1 = packed_border(p.cu_k, b + 1, p.total_k);
+      bad |= q0 != p.cu_q[b] || q1 != p.cu_q[b + 1] || k0 != p.cu_k[b] || k1 != p.cu_k[b + 1] || q1 < q0 || k1 < k0;
+      bad |= b == 0 && (q0 != 0 || k0 != 0);
+      q1 = max(q0, q1);
+      k1 = max(k0, k1);
+    }
+    const int n = key_side ? (k1 - k0 + tile_rows - 1) / tile_rows : (q1 - q0 + tile_rows - 1) / tile_rows;
+    int64_t incl = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += up;
+    }
+    const int64_t total = __shfl_sync(0xffffffffu, incl, 31);
+    if (slot < base + total) {
+      const int src = __ffs(__ballot_sync(0xffffffffu, slot < base + incl)) - 1;
+      out->q0 = __shfl_sync(0xffffffffu, q0, src);
+      out->lq = __shfl_sync(0xffffffffu, q1, src) - out->q0;
+      out->k0 = __shfl_sync(0xffffffffu, k0, src);
+      out->lk = __shfl_sync(0xffffffffu, k1, src) - out->k0;
+      out->tile = static_cast<int>(slot - base - __shfl_sync(0xffffffffu, incl - n, src));
+      return true;
+    }
+    base += total;
+  }
+  *tiles = base;
+  *end = p.nseq > 0 ? packed_border(key_side ? p.cu_k : p.cu_q, p.nseq, key_side ? p.total_k : p.total_q) : 0;
+  if (__any_sync(0xffffffffu, bad) && lane == 0) report_status(p.status, GW_ERR_INVALID_ARG);
+  return false;
+}
+
+// The rows of one head behind the last sequence, shared by the blocks `part` of `parts`.
+template <typename T>
+__device__ __forceinline__ void packed_zero_rows(void* out, float* lse, int64_t from, int64_t to, int heads, int head, int D, int64_t part,
+                                                 int64_t parts) {
+  T* dst = static_cast<T*>(out);
+  const int64_t n = (to - from) * D;
+  for (int64_t i = part * blockDim.x + threadIdx.x; i < n; i += parts * blockDim.x)
+    dst[((from + i / D) * heads + head) * D + i % D] = from_float<T>(0.f);
+  if (lse != nullptr)
+    for (int64_t i = from + part * blockDim.x + threadIdx.x; i < to; i += parts * blockDim.x)
+      lse[static_cast<int64_t>(head) * to + i] = -INFINITY;
+}
+
+inline int64_t packed_tile_bound(int64_t total, int tile_rows, int nseq) { return total / tile_rows + nseq + 1; }
+
+int packed_plain_fwd(const PackedParams& p, int dtype, cudaStream_t st);
+int packed_plain_bwd(const PackedParams& p, int dtype, cudaStream_t st);
+
+}  // namespace gw

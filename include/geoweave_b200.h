@@ -299,6 +299,57 @@ int gw_project_fused(const void* x, const void* weight, const void* bias, int dt
                      float idx_k_norm_eps, void* q, void* k, void* v, void* q_idx, void* k_idx, void* w, int* status_dev,
                      gw_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Attention over packed sequences, softmax over every allowed key: the frame blocks (each view attends to itself) and the
+ * dense global layers around the sparse ones.
+ *
+ *   S = scale * q k^T,  P = softmax(S) over the allowed keys,  out = P v,  lse = log sum exp S  (natural logarithm)
+ *
+ * q [total_q, H, D], k, v [total_k, Hk, D] of `dtype` (GW_F32, GW_BF16, GW_F16), element strides {token, head} of each,
+ * contiguous D; query head h reads key head h / (H / Hk).  Sequence b holds the rows cu_q[b] .. cu_q[b+1] of q and
+ * cu_k[b] .. cu_k[b+1] of k and v (int32 [nseq + 1] on the device, starting at 0, not decreasing, within the totals; anything
+ * else sets the status word, and no access leaves the tensors).  causal: query i of lq sees the keys 0 .. i + lk - lq of lk.
+ * out [total_q, H, D] contiguous; lse fp32 [H, total_q], nullable.  A row without an allowed key gets out = 0 and
+ * lse = -inf, as do the rows behind the last sequence.  Non-finite values of k and v stay within their own sequence.
+ * max_q: no sequence has more query rows (0: unknown).  It may only choose the kernel: a longer sequence sets the status
+ * word and its rows further on are not written.
+ * Requirements: D <= 128 and a multiple of 8, H a multiple of Hk, H <= 65535; 16-byte aligned pointers and strides;
+ *               scale > 0.  workspace: gw_packed_attn_fwd_workspace_bytes(same arguments) bytes (null where that is 0).
+ * No reference counterpart: there the dense blocks call the framework's own dense attention.
+ * ---------------------------------------------------------------------------------------------- */
+size_t gw_packed_attn_fwd_workspace_bytes(int dtype, int nseq, int64_t total_q, int64_t total_k, int H, int Hk, int D, int64_t max_q);
+int gw_packed_attn_fwd(const void* q, const void* k, const void* v, int dtype, const int32_t* cu_q, const int32_t* cu_k, int nseq,
+                       int64_t total_q, int64_t total_k, int H, int Hk, int D, const int64_t* q_strides, const int64_t* k_strides,
+                       const int64_t* v_strides, float scale, int causal, int64_t max_q, void* out, float* lse, void* workspace,
+                       size_t workspace_bytes, int* status_dev, gw_stream_t stream);
+
+/* Its backward pass.  out and lse are the forward's results, d_out [total_q, H, D] the gradient (strides as q's); dq, dk, dv
+ * are contiguous and like q, k, v:
+ *   D = rowsum(d_out * out),  dS = P * (d_out v^T - D) * scale,  dq = dS k,  dk = sum over the key head's query heads dS^T q,
+ *   dv = the same sum of P^T d_out.
+ * P is made again from q, k and lse.  No atomics: the results do not depend on timing.  workspace holds D:
+ * gw_packed_attn_bwd_workspace_bytes(total_q, H) bytes.  Everything else as gw_packed_attn_fwd. */
+size_t gw_packed_attn_bwd_workspace_bytes(int64_t total_q, int H);
+int gw_packed_attn_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* d_out, int dtype,
+                       const int32_t* cu_q, const int32_t* cu_k, int nseq, int64_t total_q, int64_t total_k, int H, int Hk, int D,
+                       const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* d_out_strides,
+                       float scale, int causal, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                       int* status_dev, gw_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Rotary positions with several axes (time, height, width).  Axis a owns widths[a] neighbouring columns of every head;
+ * inside it column j pairs with column j + widths[a] / 2 and the pair turns by the angle whose cosine and sine stand in row
+ * pos[token, a] of the tables (fp32 [table_rows, sum(widths) / 2], the axes' angles side by side).  Columns behind the
+ * last axis are copied.  inverse != 0 turns the other way: the backward pass.
+ * q [B, N, H, D], k [B, N, Hk, D] (Hk = 0: no k) of `dtype`, element strides {batch, token, head}, contiguous D; pos int64 or
+ * int32 [B, N, axes] contiguous; q_out, k_out contiguous.  A position outside the tables sets the status word and counts as 0.
+ * widths is a HOST array.  Requirements: 1 <= axes <= 4, even widths, sum(widths) <= D <= 256.
+ * Replaces, for widths {D/2, D/2}: easyvolcap/official_vggt/layers/rope.py:134-188 (RotaryPositionEmbedding2D).
+ * ---------------------------------------------------------------------------------------------- */
+int gw_rotary_axes(const void* q, const void* k, int dtype, int B, int64_t N, int H, int Hk, int D, const int64_t* q_strides,
+                   const int64_t* k_strides, const void* pos, int pos_is_64, int axes, const int* widths, const float* cos_tab,
+                   const float* sin_tab, int table_rows, int inverse, void* q_out, void* k_out, int* status_dev, gw_stream_t stream);
+
 /* Diagnostics: the gather of gw_sparse_attn_fwd without its arithmetic -- for every query the K row and the V row
  * (row_bytes <= 2048, a multiple of 16; rows k_row_stride_bytes / v_row_stride_bytes apart) of each valid entry of
  * kv_pos int32 [T,K] is bulk-copied into shared memory and dropped.  Timed by the caller, it gives the rate this
