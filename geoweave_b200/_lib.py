@@ -182,7 +182,9 @@ def status_word(device) -> torch.Tensor:
     key = torch.device(device).index
     t = _status.get(key)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=device)
+        # kept across calls, so it must not be an inference tensor, which could not be reset outside inference mode
+        with torch.inference_mode(False):
+            t = torch.zeros(1, dtype=torch.int32, device=device)
         _status[key] = t
     return t
 

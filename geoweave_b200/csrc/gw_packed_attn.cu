@@ -1,5 +1,5 @@
 // C entry points of the attention over packed sequences: argument checks and the choice of kernel.
-#include "gw_packed.cuh"
+#include "gw_packed_mma.cuh"
 
 using namespace gw;
 
@@ -56,7 +56,14 @@ extern "C" int gw_packed_attn_fwd(const void* q, const void* k, const void* v, i
   const int rc = check_packed(p, dtype);
   if (rc != GW_OK) return rc;
   if (total_q == 0) return GW_OK;
-  return packed_plain_fwd(p, dtype, reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == GW_F32) return packed_plain_fwd(p, dtype, st);
+  int dev = 0;
+  DeviceFacts facts;
+  const int rf = device_facts(&dev, &facts);
+  if (rf != GW_OK) return rf;
+  if (total_k == 0) return packed_plain_fwd(p, dtype, st);
+  return packed_mma_fwd(p, dtype, facts.sms, dev, st);
 }
 
 extern "C" size_t gw_packed_attn_bwd_workspace_bytes(int64_t total_q, int H) {
