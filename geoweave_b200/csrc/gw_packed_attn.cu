@@ -91,5 +91,11 @@ extern "C" int gw_packed_attn_bwd(const void* q, const void* k, const void* v, c
     if (s <= 0 || s * static_cast<int64_t>(dtype_size(dtype)) % 16 != 0) return GW_ERR_INVALID_ARG;
   if (total_q > 0 && (!workspace || workspace_bytes < gw_packed_attn_bwd_workspace_bytes(total_q, H))) return GW_ERR_WORKSPACE;
   p.delta = static_cast<float*>(workspace);
-  return packed_plain_bwd(p, dtype, reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == GW_F32 || total_q == 0 || total_k == 0) return packed_plain_bwd(p, dtype, st);
+  int dev = 0;
+  DeviceFacts facts;
+  rc = device_facts(&dev, &facts);
+  if (rc != GW_OK) return rc;
+  return packed_mma_bwd(p, dtype, facts.sms, dev, st);
 }

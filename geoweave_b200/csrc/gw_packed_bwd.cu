@@ -1,0 +1,541 @@
+// Backward pass of the attention over packed sequences on the tcgen05 tensor cores, 16-bit operands, head dim up to 128.
+//
+//   P = 2^(c S - lse log2 e),  D = rowsum(d_o * o),  dP = d_o v^T,  dS = P * (dP - D)
+//   dq = scale dS k,   dk = scale sum dS^T q,   dv = sum P^T d_o
+//
+// Two kernels, so that every sum is made by one block in a fixed order and nothing needs atomics (results do not depend on
+// timing): one owns 128 query rows and walks the keys (dq, and D on the way), one owns 128 key rows and walks the queries of all
+// heads that read them (dk, dv).  S and dP are made in both: seven products instead of five, against 32-bit atomic traffic of
+// one query tile for every pair of tiles.
+//
+// Each 128 x 128 tile pair: S and dP from shared-memory operands into tensor memory; two groups of four warps, 64 columns each,
+// make P and dS in registers (a thread owns one row of its half) and put them back into tensor memory as 16-bit A operands of
+// the accumulating products, whose B operand is the tile that is in shared memory already, read along its rows.  The key-side
+// kernel works on the transposes (rows are keys), so neither P nor dS is ever transposed.
+#include "gw_packed_mma.cuh"
+
+namespace gw {
+namespace {
+
+constexpr int kBwdThreads = 320;  // warps 0-3: columns 0-63, 4-7: columns 64-127, 8: loads, 9: products
+
+template <int DP>
+struct BwdShape {
+  static constexpr int kStages = DP == 64 ? 4 : 2;
+  static constexpr int kTileBytes = DP / 64 * kBoxBytes;
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(2 + 2 * kStages) * kTileBytes + 512 + kStages * 2 * kTile * 4;
+};
+
+struct BwdShared {
+  uint64_t own_full, s_full, dp_full, loaded, p_full, ds_full, ds_done, all_done;
+  uint64_t a_full[4], a_empty[4], b_full[4], b_empty[4], st_full[4];
+  PackedSeq seq;
+  int64_t tiles, end;
+  int found;
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+static_assert(sizeof(BwdShared) <= 512, "shared bookkeeping");
+
+// Barriers, the block's tile and tensor memory; the same in both kernels.
+__device__ __forceinline__ uint32_t bwd_setup(BwdShared* sh, const PackedParams& p, bool key_side, int warp, int lane) {
+  if (warp == 8) {
+    PackedSeq s{};
+    int64_t tiles = 0, end = 0;
+    const bool found = packed_find(p, key_side, kTile, blockIdx.x, &s, &tiles, &end);
+    if (lane == 0) {
+      sh->seq = s;
+      sh->tiles = tiles;
+      sh->end = end;
+      sh->found = found;
+      for (uint64_t* b : {&sh->own_full, &sh->s_full, &sh->dp_full, &sh->ds_done, &sh->all_done}) mbar_init(b, 1);
+      for (uint64_t* b : {&sh->loaded, &sh->p_full, &sh->ds_full}) mbar_init(b, 8);
+      for (int i = 0; i < 4; ++i) {
+        mbar_init(&sh->a_full[i], 1);
+        mbar_init(&sh->a_empty[i], 1);
+        mbar_init(&sh->b_full[i], 1);
+        mbar_init(&sh->b_empty[i], 1);
+        mbar_init(&sh->st_full[i], 1);
+      }
+      sh->abort_flag = 0;
+      mbar_fence_init();
+      fence_proxy_async_smem();
+    }
+  }
+  if (warp == 9) tmem_alloc(&sh->tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  return __shfl_sync(0xffffffffu, sh->tmem_base, 0);
+}
+
+// columns [from, to) of one row of an accumulator in this thread's TMEM lane, times mul, as 16-bit values (zeros if !any)
+template <typename T>
+__device__ __forceinline__ void store_acc(T* dst, uint32_t addr, int from, int to, int D, float mul, bool live, bool any) {
+#pragma unroll 1
+  for (int b = from; b < to; b += 32) {
+    if (b >= D) break;
+    float o[32];
+    if (any) {
+      tmem_load32(addr + b, o);
+      tmem_wait_ld();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint4 w;
+      uint32_t* e = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) e[k] = any ? pack_half2<T>(o[8 * i + 2 * k] * mul, o[8 * i + 2 * k + 1] * mul) : 0u;
+      if (live && b + 8 * i < D) *reinterpret_cast<uint4*>(dst + b + 8 * i) = w;
+    }
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                 const __grid_constant__ CUtensorMap tmG, const PackedParams p, const int ab_format) {
+  constexpr int ST = BwdShape<DP>::kStages, TB = BwdShape<DP>::kTileBytes;
+  constexpr uint32_t kS = 0, kDp = 128, kDs = 256, kDq = 384;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* q_smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  unsigned char* g_smem = q_smem + TB;
+  unsigned char* k_smem = g_smem + TB;
+  unsigned char* v_smem = k_smem + ST * TB;
+  BwdShared* sh = reinterpret_cast<BwdShared*>(v_smem + ST * TB);
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const int head = blockIdx.y, kv = head / (p.H / p.Hk);
+  const uint32_t tmem = bwd_setup(sh, p, false, warp, lane);
+  if (!sh->found) {
+    packed_zero_rows<T>(p.dq, nullptr, sh->end, p.total_q, p.H, head, p.D, blockIdx.x - sh->tiles, gridDim.x - sh->tiles);
+  } else {
+    const PackedSeq s = sh->seq;
+    const int off = s.lk - s.lq;
+    const int tile = p.causal ? (s.lq + kTile - 1) / kTile - 1 - s.tile : s.tile;  // longest first
+    const int r0 = tile * kTile;
+    const int keys = p.causal ? max(0, min(s.lk, min(r0 + kTile, s.lq) + off)) : s.lk;
+    const int n = (keys + kTile - 1) / kTile;
+
+    if (warp == 8) {
+      if (lane == 0 && n > 0) {
+        bool ok = true;
+        int j = 0;
+        mbar_arrive_expect_tx(&sh->own_full, 2 * TB);
+        load_rows<DP>(q_smem, &tmQ, head, s.q0 + r0, &sh->own_full);
+        load_rows<DP>(g_smem, &tmG, head, s.q0 + r0, &sh->own_full);
+        for (; j < n; ++j) {
+          const int st = j % ST;
+          const uint32_t par = ((j / ST) & 1u) ^ 1u;
+          ok = mbar_wait_bounded(&sh->a_empty[st], par) && mbar_wait_bounded(&sh->b_empty[st], par);
+          if (!ok || sh->abort_flag) break;
+          mbar_arrive_expect_tx(&sh->a_full[st], TB);
+          load_rows<DP>(k_smem + st * TB, &tmK, kv, s.k0 + j * kTile, &sh->a_full[st]);
+          mbar_arrive_expect_tx(&sh->b_full[st], TB);
+          load_rows<DP>(v_smem + st * TB, &tmV, kv, s.k0 + j * kTile, &sh->b_full[st]);
+        }
+        if (!ok) sh->abort_flag = 1;
+        if (sh->abort_flag) {  // let the copies in flight land before the shared memory is given up
+          mbar_wait_limit(&sh->own_full, 0, kDrainLimitNs);
+          for (int u = max(0, j - ST); u < j; ++u) {
+            mbar_wait_limit(&sh->a_full[u % ST], (u / ST) & 1u, kDrainLimitNs);
+            mbar_wait_limit(&sh->b_full[u % ST], (u / ST) & 1u, kDrainLimitNs);
+          }
+          report_status(p.status, GW_ERR_TIMEOUT);
+        }
+      }
+    } else if (warp == 9) {
+      const uint32_t idesc_s = make_idesc_mn(ab_format, kTile, kTile);
+      const uint32_t idesc_o = make_idesc_mn(ab_format, kTile, DP) | kBMajorMN;
+      const uint64_t qd = make_smem_desc(smem_u32(q_smem)), gd = make_smem_desc(smem_u32(g_smem));
+      const uint64_t kd = make_smem_desc(smem_u32(k_smem)), vd = make_smem_desc(smem_u32(v_smem));
+      const uint64_t kd_mn = make_smem_desc_mn(smem_u32(k_smem));
+      bool ok = n == 0 || mbar_wait_bounded(&sh->own_full, 0);
+      auto products = [&](int j) {  // S and dP of key tile j
+        const int st = j % ST;
+        ok = mbar_wait_bounded(&sh->a_full[st], (j / ST) & 1) && mbar_wait_bounded(&sh->b_full[st], (j / ST) & 1);
+        if (!ok) return;
+        if ((j + 1) * kTile > s.lk) zero_rows_from<DP>(k_smem + st * TB, s.lk - j * kTile);  // K is also dq's operand
+        if (j > 0) ok = mbar_wait_bounded(&sh->loaded, (j - 1) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        if (lane == 0) {
+          mma_rows<DP>(tmem + kS, qd, kd + st * (TB >> 4), idesc_s);
+          tc_commit(&sh->s_full);
+          mma_rows<DP>(tmem + kDp, gd, vd + st * (TB >> 4), idesc_s);
+          tc_commit(&sh->dp_full);
+          tc_commit(&sh->b_empty[st]);
+        }
+      };
+      if (n > 0 && ok) products(0);
+      for (int j = 0; j < n && ok && !sh->abort_flag; ++j) {
+        const int st = j % ST;
+        if (j + 1 < n) products(j + 1);
+        ok = ok && mbar_wait_bounded(&sh->ds_full, j & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          const int steps = min(kTile, (keys - j * kTile + 15) & ~15) / 16;
+          for (int i = 0; i < steps; ++i)
+            tc_mma_f16_ts(tmem + kDq, tmem + kDs + i * 8, kd_mn + st * (TB >> 4) + i * (16 * 128 >> 4), idesc_o, (j > 0 || i > 0) ? 1u : 0u);
+          tc_commit(&sh->a_empty[st]);
+          tc_commit(&sh->ds_done);
+        }
+      }
+      if (!ok) {
+        sh->abort_flag = 1;
+        if (lane == 0) report_status(p.status, GW_ERR_TIMEOUT);
+      }
+    } else {
+      const int half = warp >> 2;
+      const int row = r0 + (warp & 3) * 32 + lane;
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const bool live = row < s.lq;
+      const int64_t token = s.q0 + row;
+      // D of this row, from the saved output
+      float delta = 0.f, neg_lse = -INFINITY;
+      if (live) {
+        const T* o = static_cast<const T*>(p.o) + (token * p.H + head) * p.D;
+        const T* g = static_cast<const T*>(p.d_o) + token * p.dos[0] + head * p.dos[1];
+        for (int i = 0; i < p.D; i += 8) {
+          const uint4 ow = *reinterpret_cast<const uint4*>(o + i), gw = *reinterpret_cast<const uint4*>(g + i);
+          const uint32_t oe[4] = {ow.x, ow.y, ow.z, ow.w}, ge[4] = {gw.x, gw.y, gw.z, gw.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float a, b, c, d;
+            unpack2<T>(oe[k], a, b);
+            unpack2<T>(ge[k], c, d);
+            delta = fmaf(a, c, delta);
+            delta = fmaf(b, d, delta);
+          }
+        }
+        const int64_t at = static_cast<int64_t>(head) * p.total_q + token;
+        const float lse = p.lse[at];
+        neg_lse = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
+        if (half == 0) p.delta[at] = delta;
+      }
+      const float c = p.scale * kLog2e;
+      const uint64_t c2 = pack_f2(c, c), l2 = pack_f2(neg_lse, neg_lse), nd2 = pack_f2(-delta, -delta);
+      const int limit = (p.causal ? min(s.lk, row + off + 1) : s.lk) - half * 64;
+      const int open = p.causal ? min(s.lk, r0 + off + 1) : s.lk;
+      bool ok = true;
+      for (int j = 0; j < n; ++j) {
+        ok = mbar_wait_bounded(&sh->s_full, j & 1);
+        if (!ok || sh->abort_flag) break;
+        tc_fence_after();
+        float x[64], y[64];
+        tmem_load32(tmem + lanes + kS + half * 64, x);
+        tmem_load32(tmem + lanes + kS + half * 64 + 32, x + 32);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float a, b;
+          unpack_f2(fma_f2(pack_f2(x[2 * i], x[2 * i + 1]), c2, l2), a, b);
+          x[2 * i] = exp2_fast(a);
+          x[2 * i + 1] = exp2_fast(b);
+        }
+        ok = mbar_wait_bounded(&sh->dp_full, j & 1);
+        if (!ok) break;
+        tc_fence_after();
+        tmem_load32(tmem + lanes + kDp + half * 64, y);
+        tmem_load32(tmem + lanes + kDp + half * 64 + 32, y + 32);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->loaded);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const uint64_t d = mul_f2(pack_f2(x[2 * i], x[2 * i + 1]), add_f2(pack_f2(y[2 * i], y[2 * i + 1]), nd2));
+          unpack_f2(d, x[2 * i], x[2 * i + 1]);
+        }
+        if ((j + 1) * kTile > open) {
+          const int valid = limit - j * kTile;
+#pragma unroll
+          for (int i = 0; i < 64; ++i) x[i] = i < valid ? x[i] : 0.f;
+        }
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) w[i] = pack_half2<T>(x[2 * i], x[2 * i + 1]);
+        if (j > 0) {
+          ok = mbar_wait_bounded(&sh->ds_done, (j - 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+        }
+        tmem_store32(tmem + lanes + kDs + half * 32, w);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->ds_full);
+      }
+      if (n > 0 && ok && !sh->abort_flag) ok = mbar_wait_bounded(&sh->ds_done, (n - 1) & 1);
+      if (!ok) {
+        sh->abort_flag = 1;
+        report_status(p.status, GW_ERR_TIMEOUT);
+      }
+      tc_fence_after();
+      store_acc<T>(static_cast<T*>(p.dq) + (token * p.H + head) * p.D, tmem + lanes + kDq, half * (DP / 2), (half + 1) * (DP / 2), p.D, p.scale,
+                   live, n > 0);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const __grid_constant__ CUtensorMap tmG, const PackedParams p, const int ab_format) {
+  constexpr int ST = BwdShape<DP>::kStages, TB = BwdShape<DP>::kTileBytes;
+  constexpr uint32_t kS = 0, kDp = 128, kDv = 256, kDk = 256 + DP;
+  // fp16 holds nothing below 2^-24 and few bits below 2^-14, and a P of a long sequence is that small: it is raised by 2^12 (P <= 1)
+  // and dv lowered again; bf16 has fp32's range
+  constexpr float kLift = sizeof(T) == 2 && std::is_same<T, __half>::value ? 12.f : 0.f;
+  constexpr float kLower = kLift > 0.f ? 1.f / 4096.f : 1.f;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* k_smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  unsigned char* v_smem = k_smem + TB;
+  unsigned char* q_smem = v_smem + TB;
+  unsigned char* g_smem = q_smem + ST * TB;
+  float* stats = reinterpret_cast<float*>(g_smem + ST * TB);  // [stage][-lse log2 e + lift, -D][128]
+  BwdShared* sh = reinterpret_cast<BwdShared*>(stats + ST * 2 * kTile);
+
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const int kv = blockIdx.y, group = p.H / p.Hk;
+  const uint32_t tmem = bwd_setup(sh, p, true, warp, lane);
+  if (!sh->found) {
+    const int64_t part = blockIdx.x - sh->tiles, parts = gridDim.x - sh->tiles;
+    packed_zero_rows<T>(p.dk, nullptr, sh->end, p.total_k, p.Hk, kv, p.D, part, parts);
+    packed_zero_rows<T>(p.dv, nullptr, sh->end, p.total_k, p.Hk, kv, p.D, part, parts);
+  } else {
+    const PackedSeq s = sh->seq;
+    const int off = s.lk - s.lq;
+    const int c0 = s.tile * kTile;
+    const int q_tiles = (s.lq + kTile - 1) / kTile;
+    const int first = p.causal ? max(0, c0 - off) / kTile : 0;  // the first query tile that sees one of these keys
+    const int per_head = max(0, q_tiles - first);
+    const int n = per_head * group;
+
+    if (warp == 8) {
+      bool ok = true;
+      int i = 0;
+      if (lane == 0 && n > 0) {
+        mbar_arrive_expect_tx(&sh->own_full, 2 * TB);
+        load_rows<DP>(k_smem, &tmK, kv, s.k0 + c0, &sh->own_full);
+        load_rows<DP>(v_smem, &tmV, kv, s.k0 + c0, &sh->own_full);
+      }
+      for (; i < n; ++i) {
+        const int st = i % ST, head = kv * group + i / per_head, r0 = (first + i % per_head) * kTile;
+        ok = mbar_wait_bounded(&sh->a_empty[st], ((i / ST) & 1u) ^ 1u);
+        if (!ok || sh->abort_flag) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sh->a_full[st], TB);
+          load_rows<DP>(q_smem + st * TB, &tmQ, head, s.q0 + r0, &sh->a_full[st]);
+          mbar_arrive_expect_tx(&sh->b_full[st], TB);
+          load_rows<DP>(g_smem + st * TB, &tmG, head, s.q0 + r0, &sh->b_full[st]);
+        }
+        float* dst = stats + st * 2 * kTile;
+        const int64_t base = static_cast<int64_t>(head) * p.total_q + s.q0 + r0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = lane + 32 * k;
+          float l = -INFINITY, d = 0.f;  // rows behind the end: P = 0, dS = 0
+          if (r0 + r < s.lq) {
+            l = p.lse[base + r];
+            l = l == -INFINITY ? -INFINITY : fmaf(-l, kLog2e, kLift);
+            d = -p.delta[base + r];
+          }
+          dst[r] = l;
+          dst[kTile + r] = d;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->st_full[st]);
+      }
+      if (!ok) sh->abort_flag = 1;
+      if (sh->abort_flag && lane == 0) {  // let the copies in flight land before the shared memory is given up
+        if (n > 0) mbar_wait_limit(&sh->own_full, 0, kDrainLimitNs);
+        for (int u = max(0, i - ST); u < i; ++u) {
+          mbar_wait_limit(&sh->a_full[u % ST], (u / ST) & 1u, kDrainLimitNs);
+          mbar_wait_limit(&sh->b_full[u % ST], (u / ST) & 1u, kDrainLimitNs);
+        }
+        report_status(p.status, GW_ERR_TIMEOUT);
+      }
+    } else if (warp == 9) {
+      const uint32_t idesc_s = make_idesc_mn(ab_format, kTile, kTile);
+      const uint32_t idesc_o = make_idesc_mn(ab_format, kTile, DP) | kBMajorMN;
+      const uint64_t kd = make_smem_desc(smem_u32(k_smem)), vd = make_smem_desc(smem_u32(v_smem));
+      const uint64_t qd = make_smem_desc(smem_u32(q_smem)), gd = make_smem_desc(smem_u32(g_smem));
+      const uint64_t qd_mn = make_smem_desc_mn(smem_u32(q_smem)), gd_mn = make_smem_desc_mn(smem_u32(g_smem));
+      bool ok = n == 0 || mbar_wait_bounded(&sh->own_full, 0);
+      // S^T = K Q^T / dP^T = V d_o^T of query tile i; rows behind the sequence's end become zeros first
+      auto product = [&](int i, uint64_t* full, unsigned char* tiles, uint64_t a, uint64_t b, uint32_t d, uint64_t* done) {
+        const int st = i % ST, left = s.lq - (first + i % per_head) * kTile;
+        ok = mbar_wait_bounded(&full[st], (i / ST) & 1);
+        if (!ok) return;
+        if (left < kTile) zero_rows_from<DP>(tiles + st * TB, left);
+        tc_fence_after();
+        if (lane == 0) {
+          mma_rows<DP>(d, a, b + st * (TB >> 4), idesc_s);
+          tc_commit(done);
+        }
+      };
+      // accumulator += (P or dS)^T (d_o or Q): the A operand's two halves of 64 queries are 64 columns apart
+      auto accumulate = [&](int i, uint32_t acc, uint32_t a, uint64_t b) {
+        const uint64_t at = b + (i % ST) * (TB >> 4);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          tc_mma_f16_ts(acc, a + (k >> 2) * 64 + (k & 3) * 8, at + k * (16 * 128 >> 4), idesc_o, (i > 0 || k > 0) ? 1u : 0u);
+      };
+      if (n > 0 && ok) {
+        product(0, sh->a_full, q_smem, kd, qd, tmem + kS, &sh->s_full);
+        if (ok) product(0, sh->b_full, g_smem, vd, gd, tmem + kDp, &sh->dp_full);
+      }
+      for (int i = 0; i < n && ok && !sh->abort_flag; ++i) {
+        ok = mbar_wait_bounded(&sh->p_full, i & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) accumulate(i, tmem + kDv, tmem + kS, gd_mn);
+        if (i + 1 < n) product(i + 1, sh->a_full, q_smem, kd, qd, tmem + kS, &sh->s_full);
+        ok = ok && mbar_wait_bounded(&sh->ds_full, i & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (lane == 0) {
+          accumulate(i, tmem + kDk, tmem + kDp, qd_mn);
+          tc_commit(&sh->a_empty[i % ST]);
+        }
+        if (i + 1 < n) product(i + 1, sh->b_full, g_smem, vd, gd, tmem + kDp, &sh->dp_full);
+      }
+      if (n > 0 && lane == 0) tc_commit(&sh->all_done);
+      if (!ok) {
+        sh->abort_flag = 1;
+        if (lane == 0) report_status(p.status, GW_ERR_TIMEOUT);
+      }
+    } else {
+      const int half = warp >> 2;
+      const int row = c0 + (warp & 3) * 32 + lane;
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t s_addr = tmem + lanes + kS + half * 64, d_addr = tmem + lanes + kDp + half * 64;
+      const bool live = row < s.lk;
+      const float c = p.scale * kLog2e;
+      const uint64_t c2 = pack_f2(c, c), lower2 = pack_f2(kLower, kLower);
+      bool ok = true;
+      for (int i = 0; i < n; ++i) {
+        const int st = i % ST, r0 = (first + i % per_head) * kTile;
+        const ulonglong2* l2 = reinterpret_cast<const ulonglong2*>(stats + st * 2 * kTile + half * 64);
+        const ulonglong2* d2 = reinterpret_cast<const ulonglong2*>(stats + st * 2 * kTile + kTile + half * 64);
+        const bool edge = p.causal && c0 + kTile - 1 > r0 + off;  // some pair of the tiles is masked
+        const int from = row - off - r0 - half * 64;              // the first column that sees this key
+        ok = mbar_wait_bounded(&sh->st_full[st], (i / ST) & 1) && mbar_wait_bounded(&sh->s_full, i & 1);
+        if (!ok || sh->abort_flag) break;
+        tc_fence_after();
+        float x[64], y[64];
+        uint32_t w[32];
+        tmem_load32(s_addr, x);
+        tmem_load32(s_addr + 32, x + 32);
+        tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const ulonglong2 l = l2[k];
+          float a, b, e, f;
+          unpack_f2(fma_f2(pack_f2(x[4 * k], x[4 * k + 1]), c2, l.x), a, b);
+          unpack_f2(fma_f2(pack_f2(x[4 * k + 2], x[4 * k + 3]), c2, l.y), e, f);
+          x[4 * k] = exp2_fast(a);
+          x[4 * k + 1] = exp2_fast(b);
+          x[4 * k + 2] = exp2_fast(e);
+          x[4 * k + 3] = exp2_fast(f);
+        }
+        if (edge) {
+#pragma unroll
+          for (int k = 0; k < 64; ++k) x[k] = k >= from ? x[k] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) w[k] = pack_half2<T>(x[2 * k], x[2 * k + 1]);
+        tmem_store32(s_addr, w);  // P takes S's place: every thread its own lane, behind its own loads
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->p_full);
+
+        ok = mbar_wait_bounded(&sh->dp_full, i & 1);
+        if (!ok) break;
+        tc_fence_after();
+        tmem_load32(d_addr, y);
+        tmem_load32(d_addr + 32, y + 32);
+        tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const ulonglong2 d = d2[k];
+          uint64_t a = mul_f2(pack_f2(x[4 * k], x[4 * k + 1]), add_f2(pack_f2(y[4 * k], y[4 * k + 1]), d.x));
+          uint64_t b = mul_f2(pack_f2(x[4 * k + 2], x[4 * k + 3]), add_f2(pack_f2(y[4 * k + 2], y[4 * k + 3]), d.y));
+          if (kLift > 0.f) {
+            a = mul_f2(a, lower2);
+            b = mul_f2(b, lower2);
+          }
+          unpack_f2(a, y[4 * k], y[4 * k + 1]);
+          unpack_f2(b, y[4 * k + 2], y[4 * k + 3]);
+        }
+        if (edge) {
+#pragma unroll
+          for (int k = 0; k < 64; ++k) y[k] = k >= from ? y[k] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) w[k] = pack_half2<T>(y[2 * k], y[2 * k + 1]);
+        tmem_store32(d_addr, w);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->ds_full);
+      }
+      if (n > 0 && ok && !sh->abort_flag) ok = mbar_wait_bounded(&sh->all_done, 0);
+      if (!ok) {
+        sh->abort_flag = 1;
+        report_status(p.status, GW_ERR_TIMEOUT);
+      }
+      tc_fence_after();
+      const int64_t at = (static_cast<int64_t>(s.k0 + row) * p.Hk + kv) * p.D;
+      if (half == 0)
+        store_acc<T>(static_cast<T*>(p.dv) + at, tmem + lanes + kDv, 0, DP, p.D, kLower, live, n > 0);
+      else
+        store_acc<T>(static_cast<T*>(p.dk) + at, tmem + lanes + kDk, 0, DP, p.D, p.scale, live, n > 0);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int DP>
+int launch_bwd(const PackedParams& p, int dtype, int dev, cudaStream_t st) {
+  CUtensorMap mq, mk, mv, mg;
+  GW_CUDA_TRY(cudaSetDevice(dev));  // a thread that has launched nothing yet has no context to encode tensor maps in
+  int rc = make_token_map(&mq, p.q, dtype, p.total_q, p.H, p.D, p.qs[0], p.qs[1]);
+  if (rc == GW_OK) rc = make_token_map(&mk, p.k, dtype, p.total_k, p.Hk, p.D, p.ks[0], p.ks[1]);
+  if (rc == GW_OK) rc = make_token_map(&mv, p.v, dtype, p.total_k, p.Hk, p.D, p.vs[0], p.vs[1]);
+  if (rc == GW_OK) rc = make_token_map(&mg, p.d_o, dtype, p.total_q, p.H, p.D, p.dos[0], p.dos[1]);
+  static OncePerDevice once_q, once_k;
+  constexpr size_t smem = BwdShape<DP>::kSmem;
+  if (rc == GW_OK) rc = ensure_dynamic_smem(packed_dq_kernel<T, DP>, smem, once_q, dev);
+  if (rc == GW_OK) rc = ensure_dynamic_smem(packed_dkv_kernel<T, DP>, smem, once_k, dev);
+  if (rc != GW_OK) return rc;
+  const int format = dtype == GW_BF16 ? 1 : 0;
+  packed_dq_kernel<T, DP><<<dim3(static_cast<unsigned>(packed_tile_bound(p.total_q, kTile, p.nseq)), p.H), kBwdThreads, smem, st>>>(
+      mq, mk, mv, mg, p, format);
+  GW_LAUNCH_CHECK();
+  packed_dkv_kernel<T, DP><<<dim3(static_cast<unsigned>(packed_tile_bound(p.total_k, kTile, p.nseq)), p.Hk), kBwdThreads, smem, st>>>(
+      mq, mk, mv, mg, p, format);
+  GW_LAUNCH_CHECK();
+  return GW_OK;
+}
+
+}  // namespace
+
+int packed_mma_bwd(const PackedParams& p, int dtype, int sms, int dev, cudaStream_t st) {
+  if (dtype == GW_BF16) return p.D <= 64 ? launch_bwd<__nv_bfloat16, 64>(p, dtype, dev, st) : launch_bwd<__nv_bfloat16, 128>(p, dtype, dev, st);
+  return p.D <= 64 ? launch_bwd<__half, 64>(p, dtype, dev, st) : launch_bwd<__half, 128>(p, dtype, dev, st);
+}
+
+}  // namespace gw
