@@ -1,6 +1,7 @@
 """ctypes binding of libgeoweave_b200.so.  There is no fallback: a missing library or a failing call raises."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -147,6 +148,14 @@ def ptr(t) -> int | None:
 
 def stream_ptr(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(dev: torch.device):
+    """``torch.cuda.device(dev)``, or nothing where that is the current device already (the usual case, and the cheaper one)."""
+    return _SAME_DEVICE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def require_cuda(*tensors) -> torch.device:

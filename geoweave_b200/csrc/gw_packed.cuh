@@ -10,6 +10,9 @@
 
 namespace gw {
 
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
 struct PackedParams {
   const void *q, *k, *v;
   const int32_t *cu_q, *cu_k;
@@ -101,7 +104,16 @@ __device__ __forceinline__ void packed_zero_rows(void* out, float* lse, int64_t 
 
 inline int64_t packed_tile_bound(int64_t total, int tile_rows, int nseq) { return total / tile_rows + nseq + 1; }
 
-int packed_plain_fwd(const PackedParams& p, int dtype, cudaStream_t st);
-int packed_plain_bwd(const PackedParams& p, int dtype, cudaStream_t st);
+// fp32 tensors (gw_packed_plain.cu)
+int packed_plain_fwd(const PackedParams& p, cudaStream_t st);
+int packed_plain_bwd(const PackedParams& p, cudaStream_t st);
+int packed_plain_split(const PackedParams& p, int chunk, int64_t slots, float* part_o, float* part_ml, cudaStream_t st);
+// 16-bit tensors (gw_packed_fwd.cu, gw_packed_bwd.cu)
+int packed_mma_fwd(const PackedParams& p, int dtype, int dev, cudaStream_t st);
+int packed_mma_bwd(const PackedParams& p, int dtype, int dev, cudaStream_t st);
+// few query rows, divided along the keys (gw_packed_split.cu)
+bool packed_split_fits(const PackedParams& p, int64_t max_q);
+size_t packed_split_bytes(const PackedParams& p, int sms);
+int packed_split_fwd(const PackedParams& p, int dtype, int64_t max_q, int sms, void* workspace, cudaStream_t st);
 
 }  // namespace gw

@@ -1,11 +1,11 @@
 // C entry points of the attention over packed sequences: argument checks and the choice of kernel.
-#include "gw_packed_mma.cuh"
+#include "gw_packed.cuh"
 
 using namespace gw;
 
 namespace {
 
-int check_packed(const PackedParams& p, int dtype) {
+int check_packed(const PackedParams& p, int dtype, int* dev, DeviceFacts* facts) {
   if (!p.q || !p.k || !p.v || !p.cu_q || !p.cu_k || p.nseq < 0 || p.total_q < 0 || p.total_k < 0) return GW_ERR_INVALID_ARG;
   if (p.H <= 0 || p.Hk <= 0 || p.H % p.Hk != 0 || p.D <= 0) return GW_ERR_INVALID_ARG;
   if (!(p.scale > 0.f) || p.scale > 3.0e38f) return GW_ERR_INVALID_ARG;
@@ -17,11 +17,9 @@ int check_packed(const PackedParams& p, int dtype) {
     if (!aligned16(t)) return GW_ERR_INVALID_ARG;
   for (const int64_t s : {p.qs[0], p.qs[1], p.ks[0], p.ks[1], p.vs[0], p.vs[1]})
     if (s <= 0 || s * es % 16 != 0) return GW_ERR_INVALID_ARG;
-  int dev = 0;
-  DeviceFacts facts;
-  const int rc = device_facts(&dev, &facts);
+  const int rc = device_facts(dev, facts);
   if (rc != GW_OK) return rc;
-  return facts.cc_major == 10 ? GW_OK : GW_ERR_NO_SM100;
+  return facts->cc_major == 10 ? GW_OK : GW_ERR_NO_SM100;
 }
 
 PackedParams make_params(const void* q, const void* k, const void* v, const int32_t* cu_q, const int32_t* cu_k, int nseq, int64_t total_q,
@@ -40,9 +38,17 @@ PackedParams make_params(const void* q, const void* k, const void* v, const int3
 
 }  // namespace
 
+// Up to 16 rows (query rows x heads of a group) of a key head: the kernel that divides the keys, and its workspace.
 extern "C" size_t gw_packed_attn_fwd_workspace_bytes(int dtype, int nseq, int64_t total_q, int64_t total_k, int H, int Hk, int D,
                                                      int64_t max_q) {
-  return 0;
+  if (nseq < 0 || total_q <= 0 || total_k < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || D <= 0 || D > 128) return 0;
+  (void)dtype;  // partial results are fp32 whatever the type
+  PackedParams p{};
+  p.nseq = nseq; p.total_k = total_k; p.H = H; p.Hk = Hk; p.D = D;
+  int dev = 0;
+  DeviceFacts facts;
+  if (!packed_split_fits(p, max_q) || device_facts(&dev, &facts) != GW_OK) return 0;
+  return packed_split_bytes(p, facts.sms);
 }
 
 extern "C" int gw_packed_attn_fwd(const void* q, const void* k, const void* v, int dtype, const int32_t* cu_q, const int32_t* cu_k, int nseq,
@@ -52,18 +58,18 @@ extern "C" int gw_packed_attn_fwd(const void* q, const void* k, const void* v, i
   PackedParams p = make_params(q, k, v, cu_q, cu_k, nseq, total_q, total_k, H, Hk, D, q_strides, k_strides, v_strides, scale, causal, status_dev);
   p.o = out;
   p.lse = lse;
-  if (!out) return GW_ERR_INVALID_ARG;
-  const int rc = check_packed(p, dtype);
+  if (!out || max_q < 0) return GW_ERR_INVALID_ARG;
+  int dev = 0;
+  DeviceFacts facts;
+  const int rc = check_packed(p, dtype, &dev, &facts);
   if (rc != GW_OK) return rc;
   if (total_q == 0) return GW_OK;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == GW_F32) return packed_plain_fwd(p, dtype, st);
-  int dev = 0;
-  DeviceFacts facts;
-  const int rf = device_facts(&dev, &facts);
-  if (rf != GW_OK) return rf;
-  if (total_k == 0) return packed_plain_fwd(p, dtype, st);
-  return packed_mma_fwd(p, dtype, facts.sms, dev, st);
+  if (packed_split_fits(p, max_q)) {
+    if (!workspace || !aligned16(workspace) || workspace_bytes < packed_split_bytes(p, facts.sms)) return GW_ERR_WORKSPACE;
+    return packed_split_fwd(p, dtype, max_q, facts.sms, workspace, st);
+  }
+  return dtype == GW_F32 ? packed_plain_fwd(p, st) : packed_mma_fwd(p, dtype, dev, st);
 }
 
 extern "C" size_t gw_packed_attn_bwd_workspace_bytes(int64_t total_q, int H) {
@@ -83,7 +89,9 @@ extern "C" int gw_packed_attn_bwd(const void* q, const void* k, const void* v, c
   p.dq = dq; p.dk = dk; p.dv = dv;
   p.dos[0] = d_out_strides[0];
   p.dos[1] = d_out_strides[1];
-  int rc = check_packed(p, dtype);
+  int dev = 0;
+  DeviceFacts facts;
+  const int rc = check_packed(p, dtype, &dev, &facts);
   if (rc != GW_OK) return rc;
   for (const void* t : {d_out, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
     if (!aligned16(t)) return GW_ERR_INVALID_ARG;
@@ -92,10 +100,5 @@ extern "C" int gw_packed_attn_bwd(const void* q, const void* k, const void* v, c
   if (total_q > 0 && (!workspace || workspace_bytes < gw_packed_attn_bwd_workspace_bytes(total_q, H))) return GW_ERR_WORKSPACE;
   p.delta = static_cast<float*>(workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == GW_F32 || total_q == 0 || total_k == 0) return packed_plain_bwd(p, dtype, st);
-  int dev = 0;
-  DeviceFacts facts;
-  rc = device_facts(&dev, &facts);
-  if (rc != GW_OK) return rc;
-  return packed_mma_bwd(p, dtype, facts.sms, dev, st);
+  return dtype == GW_F32 ? packed_plain_bwd(p, st) : packed_mma_bwd(p, dtype, dev, st);
 }

@@ -533,7 +533,7 @@ int launch_bwd(const PackedParams& p, int dtype, int dev, cudaStream_t st) {
 
 }  // namespace
 
-int packed_mma_bwd(const PackedParams& p, int dtype, int sms, int dev, cudaStream_t st) {
+int packed_mma_bwd(const PackedParams& p, int dtype, int dev, cudaStream_t st) {
   if (dtype == GW_BF16) return p.D <= 64 ? launch_bwd<__nv_bfloat16, 64>(p, dtype, dev, st) : launch_bwd<__nv_bfloat16, 128>(p, dtype, dev, st);
   return p.D <= 64 ? launch_bwd<__half, 64>(p, dtype, dev, st) : launch_bwd<__half, 128>(p, dtype, dev, st);
 }

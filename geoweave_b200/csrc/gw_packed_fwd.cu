@@ -26,7 +26,7 @@ int make_token_map(CUtensorMap* map, const void* base, int dtype, int64_t tokens
     return q == cudaDriverEntryPointSuccess ? reinterpret_cast<EncodeTiledFn>(ptr) : (EncodeTiledFn) nullptr;
   }();
   if (!fn) return GW_ERR_CUDA;
-  const cuuint64_t gdim[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+  const cuuint64_t gdim[3] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens > 0 ? tokens : 1)};
   const cuuint64_t gstride[2] = {static_cast<cuuint64_t>(head_stride) * 2, static_cast<cuuint64_t>(token_stride) * 2};
   const cuuint32_t box[3] = {64, 1, kTile};
   const cuuint32_t estr[3] = {1, 1, 1};
@@ -365,7 +365,7 @@ int launch_fwd(const PackedParams& p, int dtype, int dev, cudaStream_t st) {
 
 }  // namespace
 
-int packed_mma_fwd(const PackedParams& p, int dtype, int sms, int dev, cudaStream_t st) {
+int packed_mma_fwd(const PackedParams& p, int dtype, int dev, cudaStream_t st) {
   if (dtype == GW_BF16) return p.D <= 64 ? launch_fwd<__nv_bfloat16, 64>(p, dtype, dev, st) : launch_fwd<__nv_bfloat16, 128>(p, dtype, dev, st);
   return p.D <= 64 ? launch_fwd<__half, 64>(p, dtype, dev, st) : launch_fwd<__half, 128>(p, dtype, dev, st);
 }

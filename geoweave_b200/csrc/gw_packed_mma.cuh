@@ -9,11 +9,8 @@
 
 namespace gw {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kTile = 128;                     // rows of an operand tile = TMEM lanes
 constexpr int kBoxBytes = kTile * 64 * 2;      // 128 rows x 64 16-bit columns: one TMA box, rows of 128 bytes, 128-byte swizzle
-constexpr uint32_t kStep = 16;                 // contraction depth of one kind::f16 instruction
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
@@ -141,17 +138,7 @@ __device__ __forceinline__ void zero_rows_from(unsigned char* tile, int from) {
 }
 
 // [tokens, heads, D] tensor of 16-bit elements with any 16-byte strides; a box is 64 columns of 128 tokens of one head, what lies
-// outside the tensor reads as zero
+// outside the tensor reads as zero (a side without tokens is never loaded)
 int make_token_map(CUtensorMap* map, const void* base, int dtype, int64_t tokens, int heads, int D, int64_t token_stride, int64_t head_stride);
-
-template <int DP>
-__device__ __forceinline__ void store_row16(void* dst, const float* v, int col0, int D) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (col0 + i * 8 < D) reinterpret_cast<uint4*>(dst)[i] = *reinterpret_cast<const uint4*>(v + 4 * i);
-}
-
-int packed_mma_fwd(const PackedParams& p, int dtype, int sms, int dev, cudaStream_t st);
-int packed_mma_bwd(const PackedParams& p, int dtype, int sms, int dev, cudaStream_t st);
 
 }  // namespace gw

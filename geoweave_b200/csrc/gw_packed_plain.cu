@@ -15,35 +15,33 @@ namespace {
 constexpr int BT = 64;        // rows and columns of a tile
 constexpr int NT = 256;       // threads: 16 x 16
 constexpr int WP = BT + 4;    // padded row of a 64 x 64 tile in shared memory
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 // [64 rows][DP + 4] fp32 tile of rows row0.. (rows at or beyond `rows`, columns beyond D: zero)
-template <typename T, int DP>
+template <int DP>
 __device__ __forceinline__ void load_tile(float* dst, const void* base, int64_t token0, int rows, int64_t ts, int64_t hs, int head, int D) {
-  const T* src = static_cast<const T*>(base) + head * hs + token0 * ts;
+  const float* src = static_cast<const float*>(base) + head * hs + token0 * ts;
   for (int i = threadIdx.x; i < BT * DP; i += NT) {
     const int r = i / DP, c = i % DP;
-    dst[r * (DP + 4) + c] = (r < rows && c < D) ? to_float(src[r * ts + c]) : 0.f;
+    dst[r * (DP + 4) + c] = (r < rows && c < D) ? src[r * ts + c] : 0.f;
   }
 }
 
-// acc[i][j] = <a row ty*4+i, b row tx+16*j>
-template <int DP>
-__device__ __forceinline__ void dot_tile(float (&acc)[4][4], const float* a, const float* b, int ty, int tx) {
+// acc[i][j] = <a row ty*R+i, b row tx+16*j>
+template <int DP, int R>
+__device__ __forceinline__ void dot_tile(float (&acc)[R][4], const float* a, const float* b, int ty, int tx) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
 #pragma unroll 4
   for (int d = 0; d < DP; d += 4) {
-    float4 av[4], bv[4];
+    float4 av[R], bv[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) av[i] = *reinterpret_cast<const float4*>(a + (ty * 4 + i) * (DP + 4) + d);
+    for (int i = 0; i < R; ++i) av[i] = *reinterpret_cast<const float4*>(a + (ty * R + i) * (DP + 4) + d);
 #pragma unroll
     for (int j = 0; j < 4; ++j) bv[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * (DP + 4) + d);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         acc[i][j] = fmaf(av[i].x, bv[j].x, acc[i][j]);
@@ -54,21 +52,21 @@ __device__ __forceinline__ void dot_tile(float (&acc)[4][4], const float* a, con
   }
 }
 
-// acc[i][c] += sum_k w[ty*4+i][k] * m[k][column c of this thread]; columns tx*4 + 64*(c/4) + c%4
-template <int DP>
-__device__ __forceinline__ void accumulate(float (&acc)[4][DP / 16], const float* w, const float* m, int ty, int tx) {
+// acc[i][c] += sum_k w[ty*R+i][k] * m[k][column c of this thread]; columns tx*4 + 64*(c/4) + c%4
+template <int DP, int R>
+__device__ __forceinline__ void accumulate(float (&acc)[R][DP / 16], const float* w, const float* m, int ty, int tx) {
 #pragma unroll 4
   for (int k = 0; k < BT; k += 4) {
-    float4 wv[4];
+    float4 wv[R];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) wv[i] = *reinterpret_cast<const float4*>(w + (ty * 4 + i) * WP + k);
+    for (int i = 0; i < R; ++i) wv[i] = *reinterpret_cast<const float4*>(w + (ty * R + i) * WP + k);
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
       for (int c = 0; c < DP / 16; c += 4) {
         const float4 mv = *reinterpret_cast<const float4*>(m + (k + kk) * (DP + 4) + tx * 4 + 16 * c);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < R; ++i) {
           const float x = kk == 0 ? wv[i].x : kk == 1 ? wv[i].y : kk == 2 ? wv[i].z : wv[i].w;
           acc[i][c] = fmaf(x, mv.x, acc[i][c]);
           acc[i][c + 1] = fmaf(x, mv.y, acc[i][c + 1]);
@@ -79,10 +77,10 @@ __device__ __forceinline__ void accumulate(float (&acc)[4][DP / 16], const float
   }
 }
 
-template <typename T, int DP>
+template <int DP>
 __device__ __forceinline__ void store_rows(void* out, const float (&acc)[4][DP / 16], const float (&mul)[4], int64_t token0, int rows, int heads,
                                            int head, int D, int ty, int tx) {
-  T* dst = static_cast<T*>(out);
+  float* dst = static_cast<float*>(out);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = ty * 4 + i;
@@ -90,7 +88,7 @@ __device__ __forceinline__ void store_rows(void* out, const float (&acc)[4][DP /
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const int col = tx * 4 + 16 * (c & ~3) + (c & 3);
-      if (col < D) dst[((token0 + r) * heads + head) * D + col] = from_float<T>(mul[i] == 0.f ? 0.f : acc[i][c] * mul[i]);
+      if (col < D) dst[((token0 + r) * heads + head) * D + col] = mul[i] == 0.f ? 0.f : acc[i][c] * mul[i];
     }
   }
 }
@@ -107,27 +105,26 @@ __device__ __forceinline__ float reduce16_sum(float x) {
 }
 
 // The block's work; false when it has none (then the rows behind the last sequence have been dealt with).
-template <typename T>
 __device__ __forceinline__ bool block_tile(const PackedParams& p, bool key_side, int head, PackedSeq* s, void* out, void* out2, float* lse) {
   int64_t tiles, end;
   if (packed_find(p, key_side, BT, blockIdx.x, s, &tiles, &end)) return true;
   const int64_t total = key_side ? p.total_k : p.total_q, parts = gridDim.x - tiles, part = blockIdx.x - tiles;
   const int heads = key_side ? p.Hk : p.H;
-  packed_zero_rows<T>(out, lse, end, total, heads, head, p.D, part, parts);
-  if (out2 != nullptr) packed_zero_rows<T>(out2, nullptr, end, total, heads, head, p.D, part, parts);
+  packed_zero_rows<float>(out, lse, end, total, heads, head, p.D, part, parts);
+  if (out2 != nullptr) packed_zero_rows<float>(out2, nullptr, end, total, heads, head, p.D, part, parts);
   return false;
 }
 
-template <typename T, int DP>
+template <int DP>
 __global__ void __launch_bounds__(NT) plain_fwd_kernel(const PackedParams p) {
   extern __shared__ float smem[];
   float *qt = smem, *kt = qt + BT * (DP + 4), *w = kt + BT * (DP + 4);
   const int head = blockIdx.y, kv = head / (p.H / p.Hk), ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   PackedSeq s;
-  if (!block_tile<T>(p, false, head, &s, p.o, nullptr, p.lse)) return;
+  if (!block_tile(p, false, head, &s, p.o, nullptr, p.lse)) return;
   const int r0 = s.tile * BT, rows = min(BT, s.lq - r0), off = s.lk - s.lq;
   const int keys = p.causal ? max(0, min(s.lk, r0 + rows + off)) : s.lk;  // keys that the tile's last row sees
-  load_tile<T, DP>(qt, p.q, s.q0 + r0, rows, p.qs[0], p.qs[1], head, p.D);
+  load_tile<DP>(qt, p.q, s.q0 + r0, rows, p.qs[0], p.qs[1], head, p.D);
   float m[4], l[4], acc[4][DP / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -139,12 +136,12 @@ __global__ void __launch_bounds__(NT) plain_fwd_kernel(const PackedParams p) {
   const float c2 = p.scale * kLog2e;
   for (int k0 = 0; k0 < keys; k0 += BT) {
     __syncthreads();
-    load_tile<T, DP>(kt, p.k, s.k0 + k0, s.lk - k0, p.ks[0], p.ks[1], kv, p.D);
+    load_tile<DP>(kt, p.k, s.k0 + k0, s.lk - k0, p.ks[0], p.ks[1], kv, p.D);
     __syncthreads();
     float sc[4][4];
-    dot_tile<DP>(sc, qt, kt, ty, tx);
+    dot_tile<DP, 4>(sc, qt, kt, ty, tx);
     __syncthreads();
-    load_tile<T, DP>(kt, p.v, s.k0 + k0, s.lk - k0, p.vs[0], p.vs[1], kv, p.D);  // v takes k's place
+    load_tile<DP>(kt, p.v, s.k0 + k0, s.lk - k0, p.vs[0], p.vs[1], kv, p.D);  // v takes k's place
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = r0 + ty * 4 + i;
@@ -171,7 +168,7 @@ __global__ void __launch_bounds__(NT) plain_fwd_kernel(const PackedParams p) {
       for (int c = 0; c < DP / 16; ++c) acc[i][c] *= shrink;
     }
     __syncthreads();
-    accumulate<DP>(acc, w, kt, ty, tx);
+    accumulate<DP, 4>(acc, w, kt, ty, tx);
   }
   float mul[4];
 #pragma unroll
@@ -181,7 +178,7 @@ __global__ void __launch_bounds__(NT) plain_fwd_kernel(const PackedParams p) {
     if (p.lse != nullptr && tx == 0 && r < rows)
       p.lse[head * p.total_q + s.q0 + r0 + r] = l[i] == 0.f ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
   }
-  store_rows<T, DP>(p.o, acc, mul, s.q0 + r0, rows, p.H, head, p.D, ty, tx);
+  store_rows<DP>(p.o, acc, mul, s.q0 + r0, rows, p.H, head, p.D, ty, tx);
 }
 
 // P of a 4 x 4 piece; rows of the piece are query rows (this kernel's lse per row) or key rows (lse per column)
@@ -189,17 +186,17 @@ __device__ __forceinline__ float prob(float s, float c2, float lse) {
   return lse == -INFINITY ? 0.f : exp2f(fmaf(s, c2, -lse * kLog2e));
 }
 
-template <typename T, int DP>
+template <int DP>
 __global__ void __launch_bounds__(NT) plain_dq_kernel(const PackedParams p) {
   extern __shared__ float smem[];
   float *qt = smem, *dt = qt + BT * (DP + 4), *kt = dt + BT * (DP + 4), *vt = kt + BT * (DP + 4), *w = vt + BT * (DP + 4);
   const int head = blockIdx.y, kv = head / (p.H / p.Hk), ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   PackedSeq s;
-  if (!block_tile<T>(p, false, head, &s, p.dq, nullptr, nullptr)) return;
+  if (!block_tile(p, false, head, &s, p.dq, nullptr, nullptr)) return;
   const int r0 = s.tile * BT, rows = min(BT, s.lq - r0), off = s.lk - s.lq;
   const int keys = p.causal ? max(0, min(s.lk, r0 + rows + off)) : s.lk;
-  load_tile<T, DP>(qt, p.o, s.q0 + r0, rows, static_cast<int64_t>(p.H) * p.D, p.D, head, p.D);
-  load_tile<T, DP>(dt, p.d_o, s.q0 + r0, rows, p.dos[0], p.dos[1], head, p.D);
+  load_tile<DP>(qt, p.o, s.q0 + r0, rows, static_cast<int64_t>(p.H) * p.D, p.D, head, p.D);
+  load_tile<DP>(dt, p.d_o, s.q0 + r0, rows, p.dos[0], p.dos[1], head, p.D);
   __syncthreads();
   float lse[4], delta[4], acc[4][DP / 16];
 #pragma unroll
@@ -214,16 +211,16 @@ __global__ void __launch_bounds__(NT) plain_dq_kernel(const PackedParams p) {
     for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
   }
   __syncthreads();
-  load_tile<T, DP>(qt, p.q, s.q0 + r0, rows, p.qs[0], p.qs[1], head, p.D);
+  load_tile<DP>(qt, p.q, s.q0 + r0, rows, p.qs[0], p.qs[1], head, p.D);
   const float c2 = p.scale * kLog2e;
   for (int k0 = 0; k0 < keys; k0 += BT) {
     __syncthreads();
-    load_tile<T, DP>(kt, p.k, s.k0 + k0, s.lk - k0, p.ks[0], p.ks[1], kv, p.D);
-    load_tile<T, DP>(vt, p.v, s.k0 + k0, s.lk - k0, p.vs[0], p.vs[1], kv, p.D);
+    load_tile<DP>(kt, p.k, s.k0 + k0, s.lk - k0, p.ks[0], p.ks[1], kv, p.D);
+    load_tile<DP>(vt, p.v, s.k0 + k0, s.lk - k0, p.vs[0], p.vs[1], kv, p.D);
     __syncthreads();
     float sc[4][4], dp[4][4];
-    dot_tile<DP>(sc, qt, kt, ty, tx);
-    dot_tile<DP>(dp, dt, vt, ty, tx);
+    dot_tile<DP, 4>(sc, qt, kt, ty, tx);
+    dot_tile<DP, 4>(dp, dt, vt, ty, tx);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = r0 + ty * 4 + i;
@@ -233,24 +230,24 @@ __global__ void __launch_bounds__(NT) plain_dq_kernel(const PackedParams p) {
         w[(ty * 4 + i) * WP + tx + 16 * j] = (tx + 16 * j < limit) ? prob(sc[i][j], c2, lse[i]) * (dp[i][j] - delta[i]) : 0.f;
     }
     __syncthreads();
-    accumulate<DP>(acc, w, kt, ty, tx);
+    accumulate<DP, 4>(acc, w, kt, ty, tx);
   }
   const float mul[4] = {p.scale, p.scale, p.scale, p.scale};
-  store_rows<T, DP>(p.dq, acc, mul, s.q0 + r0, rows, p.H, head, p.D, ty, tx);
+  store_rows<DP>(p.dq, acc, mul, s.q0 + r0, rows, p.H, head, p.D, ty, tx);
 }
 
-template <typename T, int DP>
+template <int DP>
 __global__ void __launch_bounds__(NT) plain_dkv_kernel(const PackedParams p) {
   extern __shared__ float smem[];
   float *kt = smem, *vt = kt + BT * (DP + 4), *qt = vt + BT * (DP + 4), *dt = qt + BT * (DP + 4), *w = dt + BT * (DP + 4);
   float* st = w + BT * WP;  // lse, delta of the tile's 64 queries
   const int kv = blockIdx.y, group = p.H / p.Hk, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   PackedSeq s;
-  if (!block_tile<T>(p, true, kv, &s, p.dk, p.dv, nullptr)) return;
+  if (!block_tile(p, true, kv, &s, p.dk, p.dv, nullptr)) return;
   const int c0 = s.tile * BT, rows = min(BT, s.lk - c0), off = s.lk - s.lq;
   const int first = p.causal ? max(0, c0 - off) / BT * BT : 0;  // the first query tile that sees one of these keys
-  load_tile<T, DP>(kt, p.k, s.k0 + c0, rows, p.ks[0], p.ks[1], kv, p.D);
-  load_tile<T, DP>(vt, p.v, s.k0 + c0, rows, p.vs[0], p.vs[1], kv, p.D);
+  load_tile<DP>(kt, p.k, s.k0 + c0, rows, p.ks[0], p.ks[1], kv, p.D);
+  load_tile<DP>(vt, p.v, s.k0 + c0, rows, p.vs[0], p.vs[1], kv, p.D);
   float ak[4][DP / 16], av[4][DP / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -260,8 +257,8 @@ __global__ void __launch_bounds__(NT) plain_dkv_kernel(const PackedParams p) {
   for (int head = kv * group; head < (kv + 1) * group; ++head)
     for (int r0 = first; r0 < s.lq; r0 += BT) {
       __syncthreads();
-      load_tile<T, DP>(qt, p.q, s.q0 + r0, s.lq - r0, p.qs[0], p.qs[1], head, p.D);
-      load_tile<T, DP>(dt, p.d_o, s.q0 + r0, s.lq - r0, p.dos[0], p.dos[1], head, p.D);
+      load_tile<DP>(qt, p.q, s.q0 + r0, s.lq - r0, p.qs[0], p.qs[1], head, p.D);
+      load_tile<DP>(dt, p.d_o, s.q0 + r0, s.lq - r0, p.dos[0], p.dos[1], head, p.D);
       if (threadIdx.x < 2 * BT) {
         const int r = threadIdx.x & (BT - 1);
         const bool live = r0 + r < s.lq;
@@ -270,8 +267,8 @@ __global__ void __launch_bounds__(NT) plain_dkv_kernel(const PackedParams p) {
       }
       __syncthreads();
       float sc[4][4], dp[4][4];
-      dot_tile<DP>(sc, kt, qt, ty, tx);
-      dot_tile<DP>(dp, vt, dt, ty, tx);
+      dot_tile<DP, 4>(sc, kt, qt, ty, tx);
+      dot_tile<DP, 4>(dp, vt, dt, ty, tx);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = c0 + ty * 4 + i;
@@ -285,63 +282,134 @@ __global__ void __launch_bounds__(NT) plain_dkv_kernel(const PackedParams p) {
         }
       }
       __syncthreads();
-      accumulate<DP>(av, w, dt, ty, tx);
+      accumulate<DP, 4>(av, w, dt, ty, tx);
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[(ty * 4 + i) * WP + tx + 16 * j] = dp[i][j];
       __syncthreads();
-      accumulate<DP>(ak, w, qt, ty, tx);
+      accumulate<DP, 4>(ak, w, qt, ty, tx);
     }
   const float mul[4] = {p.scale, p.scale, p.scale, p.scale}, one[4] = {1.f, 1.f, 1.f, 1.f};
-  store_rows<T, DP>(p.dk, ak, mul, s.k0 + c0, rows, p.Hk, kv, p.D, ty, tx);
-  store_rows<T, DP>(p.dv, av, one, s.k0 + c0, rows, p.Hk, kv, p.D, ty, tx);
+  store_rows<DP>(p.dk, ak, mul, s.k0 + c0, rows, p.Hk, kv, p.D, ty, tx);
+  store_rows<DP>(p.dv, av, one, s.k0 + c0, rows, p.Hk, kv, p.D, ty, tx);
+}
+
+// The forward for at most 16 rows of one key head and one chunk of keys (see gw_packed_split.cu): a thread holds one row.
+// The rows come first in the tile's 64 x (DP + 4) place; partial results are joined by the caller.
+template <int DP>
+__global__ void __launch_bounds__(NT) plain_split_kernel(const PackedParams p, const int chunk, float* part_o, float* part_ml) {
+  extern __shared__ float smem[];
+  float *qt = smem, *kt = qt + 16 * (DP + 4), *vt = kt + BT * (DP + 4), *w = vt + BT * (DP + 4);
+  const int kv = blockIdx.y, group = p.H / p.Hk, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  PackedSeq s;
+  int64_t tiles, end;
+  if (!packed_find(p, true, chunk, blockIdx.x, &s, &tiles, &end)) return;
+  const int rows = min(16, s.lq * group);
+  if (rows == 0) return;
+  const int from = s.tile * chunk, to = min(s.lk, from + chunk);
+  for (int i = threadIdx.x; i < 16 * DP; i += NT) {
+    const int r = i / DP, c = i % DP;
+    qt[r * (DP + 4) + c] =
+        r < rows && c < p.D ? static_cast<const float*>(p.q)[(s.q0 + r / group) * p.qs[0] + (kv * group + r % group) * p.qs[1] + c] : 0.f;
+  }
+  const int limit = ty < rows ? (p.causal ? min(to, ty / group + s.lk - s.lq + 1) : to) : 0;  // keys this row sees
+  const float c2 = p.scale * kLog2e;
+  float m = -INFINITY, l = 0.f, acc[1][DP / 16];
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) acc[0][c] = 0.f;
+  for (int k0 = from; k0 < to; k0 += BT) {
+    __syncthreads();
+    load_tile<DP>(kt, p.k, s.k0 + k0, to - k0, p.ks[0], p.ks[1], kv, p.D);
+    load_tile<DP>(vt, p.v, s.k0 + k0, to - k0, p.vs[0], p.vs[1], kv, p.D);
+    __syncthreads();
+    float sc[1][4];
+    dot_tile<DP, 1>(sc, qt, kt, ty, tx);
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      sc[0][j] = k0 + tx + 16 * j < limit ? sc[0][j] * c2 : -INFINITY;
+      top = fmaxf(top, sc[0][j]);
+    }
+    top = fmaxf(m, reduce16_max(top));
+    const float base = top == -INFINITY ? 0.f : top, shrink = exp2f(m - base);
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float e = exp2f(sc[0][j] - base);
+      w[ty * WP + tx + 16 * j] = e;
+      sum += e;
+    }
+    l = l * shrink + reduce16_sum(sum);
+    m = top;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) acc[0][c] *= shrink;
+    __syncwarp();  // a row's weights are written and read by one warp
+    accumulate<DP, 1>(acc, w, vt, ty, tx);
+  }
+  if (ty >= rows) return;
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * p.Hk + kv) * 16 + ty;
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) {
+    const int col = tx * 4 + 16 * (c & ~3) + (c & 3);
+    if (col < p.D) part_o[at * p.D + col] = acc[0][c];
+  }
+  if (tx == 0) {
+    part_ml[at * 2] = m;
+    part_ml[at * 2 + 1] = l;
+  }
 }
 
 template <int DP>
 constexpr size_t tiles_bytes(int tiles) { return static_cast<size_t>(tiles) * BT * (DP + 4) * 4 + BT * WP * 4 + 2 * BT * 4; }
 
-template <typename T, int DP>
+template <int DP>
 int launch_fwd(const PackedParams& p, cudaStream_t st) {
   int dev = 0;
   GW_CUDA_TRY(cudaGetDevice(&dev));
   static OncePerDevice once;
-  const int rc = ensure_dynamic_smem(plain_fwd_kernel<T, DP>, tiles_bytes<DP>(2), once, dev);
+  const int rc = ensure_dynamic_smem(plain_fwd_kernel<DP>, tiles_bytes<DP>(2), once, dev);
   if (rc != GW_OK) return rc;
-  plain_fwd_kernel<T, DP><<<dim3(static_cast<unsigned>(packed_tile_bound(p.total_q, BT, p.nseq)), p.H), NT, tiles_bytes<DP>(2), st>>>(p);
+  plain_fwd_kernel<DP><<<dim3(static_cast<unsigned>(packed_tile_bound(p.total_q, BT, p.nseq)), p.H), NT, tiles_bytes<DP>(2), st>>>(p);
   GW_LAUNCH_CHECK();
   return GW_OK;
 }
 
-template <typename T, int DP>
+template <int DP>
 int launch_bwd(const PackedParams& p, cudaStream_t st) {
   int dev = 0;
   GW_CUDA_TRY(cudaGetDevice(&dev));
   static OncePerDevice once_q, once_k;
-  int rc = ensure_dynamic_smem(plain_dq_kernel<T, DP>, tiles_bytes<DP>(4), once_q, dev);
+  int rc = ensure_dynamic_smem(plain_dq_kernel<DP>, tiles_bytes<DP>(4), once_q, dev);
   if (rc != GW_OK) return rc;
-  rc = ensure_dynamic_smem(plain_dkv_kernel<T, DP>, tiles_bytes<DP>(4), once_k, dev);
+  rc = ensure_dynamic_smem(plain_dkv_kernel<DP>, tiles_bytes<DP>(4), once_k, dev);
   if (rc != GW_OK) return rc;
-  plain_dq_kernel<T, DP><<<dim3(static_cast<unsigned>(packed_tile_bound(p.total_q, BT, p.nseq)), p.H), NT, tiles_bytes<DP>(4), st>>>(p);
+  plain_dq_kernel<DP><<<dim3(static_cast<unsigned>(packed_tile_bound(p.total_q, BT, p.nseq)), p.H), NT, tiles_bytes<DP>(4), st>>>(p);
   GW_LAUNCH_CHECK();
-  plain_dkv_kernel<T, DP><<<dim3(static_cast<unsigned>(packed_tile_bound(p.total_k, BT, p.nseq)), p.Hk), NT, tiles_bytes<DP>(4), st>>>(p);
+  plain_dkv_kernel<DP><<<dim3(static_cast<unsigned>(packed_tile_bound(p.total_k, BT, p.nseq)), p.Hk), NT, tiles_bytes<DP>(4), st>>>(p);
+  GW_LAUNCH_CHECK();
+  return GW_OK;
+}
+
+template <int DP>
+int launch_split(const PackedParams& p, int chunk, int64_t slots, float* part_o, float* part_ml, cudaStream_t st) {
+  int dev = 0;
+  GW_CUDA_TRY(cudaGetDevice(&dev));
+  static OncePerDevice once;
+  const int rc = ensure_dynamic_smem(plain_split_kernel<DP>, tiles_bytes<DP>(3), once, dev);
+  if (rc != GW_OK) return rc;
+  plain_split_kernel<DP><<<dim3(static_cast<unsigned>(slots), p.Hk), NT, tiles_bytes<DP>(3), st>>>(p, chunk, part_o, part_ml);
   GW_LAUNCH_CHECK();
   return GW_OK;
 }
 
 }  // namespace
 
-int packed_plain_fwd(const PackedParams& p, int dtype, cudaStream_t st) {
-  if (dtype == GW_F32) return p.D <= 64 ? launch_fwd<float, 64>(p, st) : launch_fwd<float, 128>(p, st);
-  if (dtype == GW_BF16) return p.D <= 64 ? launch_fwd<__nv_bfloat16, 64>(p, st) : launch_fwd<__nv_bfloat16, 128>(p, st);
-  return p.D <= 64 ? launch_fwd<__half, 64>(p, st) : launch_fwd<__half, 128>(p, st);
-}
-
-int packed_plain_bwd(const PackedParams& p, int dtype, cudaStream_t st) {
-  if (dtype == GW_F32) return p.D <= 64 ? launch_bwd<float, 64>(p, st) : launch_bwd<float, 128>(p, st);
-  if (dtype == GW_BF16) return p.D <= 64 ? launch_bwd<__nv_bfloat16, 64>(p, st) : launch_bwd<__nv_bfloat16, 128>(p, st);
-  return p.D <= 64 ? launch_bwd<__half, 64>(p, st) : launch_bwd<__half, 128>(p, st);
+int packed_plain_fwd(const PackedParams& p, cudaStream_t st) { return p.D <= 64 ? launch_fwd<64>(p, st) : launch_fwd<128>(p, st); }
+int packed_plain_bwd(const PackedParams& p, cudaStream_t st) { return p.D <= 64 ? launch_bwd<64>(p, st) : launch_bwd<128>(p, st); }
+int packed_plain_split(const PackedParams& p, int chunk, int64_t slots, float* part_o, float* part_ml, cudaStream_t st) {
+  return p.D <= 64 ? launch_split<64>(p, chunk, slots, part_o, part_ml, st) : launch_split<128>(p, chunk, slots, part_o, part_ml, st);
 }
 
 }  // namespace gw

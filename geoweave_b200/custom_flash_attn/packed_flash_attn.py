@@ -102,7 +102,7 @@ def packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=Fa
     most = T if max_seqlen_q is None else min(T, int(max_seqlen_q))
     lib = _lib.load()
     nbytes = int(lib.gw_packed_attn_fwd_workspace_bytes(code, nseq, T, S, H, Hk, D, most))
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         rc = lib.gw_packed_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), code, cu_q.data_ptr(), cu_k.data_ptr(), nseq, T, S, H, Hk, D,
                                     _strides(q), _strides(k), _strides(v), scale, int(bool(causal)), most, o.data_ptr(), _lib.ptr(lse),
@@ -135,7 +135,7 @@ def packed_attention_backward(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, d_out
     nseq = cu_q.numel() - 1
     lib = _lib.load()
     nbytes = int(lib.gw_packed_attn_bwd_workspace_bytes(T, H))
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         rc = lib.gw_packed_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), d_out.data_ptr(),
                                     _lib.dtype_code(q), cu_q.data_ptr(), cu_k.data_ptr(), nseq, T, S, H, Hk, D, _strides(q), _strides(k),
@@ -183,10 +183,10 @@ def packed_flash_attn_func(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal: boo
         return packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, causal, softmax_scale, max_seqlen_q)[0]
 
 
-@torch.inference_mode()
 def packed_flash_attn_inference_func(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal: bool = False,
                                      softmax_scale: Optional[float] = None, max_seqlen_q: Optional[int] = None,
                                      return_lse: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """As ``packed_flash_attn_func`` without gradients: ``(o, lse | None)``, ``lse`` fp32 ``[H, total_q]`` (natural logarithm,
     ``-inf`` for rows without an allowed key)."""
-    return packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, causal, softmax_scale, max_seqlen_q, return_lse)
+    return packed_attention_forward(q.detach(), k.detach(), v.detach(), cu_seqlens_q, cu_seqlens_k, causal, softmax_scale, max_seqlen_q,
+                                    return_lse)

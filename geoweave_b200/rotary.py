@@ -87,7 +87,7 @@ def _rotate(q, k, pos, axes: RotaryAxes, inverse: bool):
     def strides(x):  # a dimension of one element may carry any stride
         return _lib.i64x3([x.stride(d) if x.shape[d] > 1 else 0 for d in range(3)])
 
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         rc = lib.gw_rotary_axes(q4.data_ptr(), _lib.ptr(k4), _lib.dtype_code(q), B, N, H, Hk, D, strides(q4),
                                 None if k is None else strides(k4), pos.data_ptr(), int(pos.dtype == torch.int64), len(widths),
                                 (c_int * len(widths))(*widths), cos.data_ptr(), sin.data_ptr(), cos.shape[0], int(inverse),
