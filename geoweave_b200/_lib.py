@@ -147,6 +147,8 @@ def ptr(t) -> int | None:
 
 
 def stream_ptr(device) -> int:
+    if device.index is not None:  # the same handle without building a stream object, which costs several times the call
+        return torch._C._cuda_getCurrentRawStream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -155,7 +157,7 @@ _SAME_DEVICE = contextlib.nullcontext()
 
 def on_device(dev: torch.device):
     """``torch.cuda.device(dev)``, or nothing where that is the current device already (the usual case, and the cheaper one)."""
-    return _SAME_DEVICE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _SAME_DEVICE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 def require_cuda(*tensors) -> torch.device:
@@ -188,7 +190,7 @@ _workspaces: dict = {}
 
 
 def status_word(device) -> torch.Tensor:
-    key = torch.device(device).index
+    key = device.index if isinstance(device, torch.device) else torch.device(device).index
     t = _status.get(key)
     if t is None:
         # kept across calls, so it must not be an inference tensor, which could not be reset outside inference mode

@@ -29,17 +29,20 @@ def _scale(softmax_scale, D):
     return scale
 
 
-def _usable(x):
-    """The kernels copy 16-byte pieces: contiguous head dim, base and strides on 16-byte boundaries, no broadcast dims."""
-    es = x.element_size()
-    return (x.stride(2) == 1 and x.data_ptr() % 16 == 0 and
-            all(x.shape[d] == 1 or (x.stride(d) > 0 and (x.stride(d) * es) % 16 == 0) for d in (0, 1)))
-
-
-def _strides(x):
-    """Element strides {token, head}; a dimension of one element may carry any stride, so it gets that of a contiguous tensor."""
+def _prepared(x):
+    """``x`` as the kernels can copy it in 16-byte pieces -- contiguous head dim, base and strides on 16-byte boundaries, no
+    broadcast dims; a copy if it is not -- and its element strides {token, head}."""
     T, H, D = x.shape
-    return _lib.i64x2([x.stride(0) if T > 1 else H * D, x.stride(1) if H > 1 else D])
+    if not x.is_contiguous():
+        st, es = x.stride(), x.element_size()
+        # a dimension of one element may carry any stride, so it gets that of a contiguous tensor
+        token, head = st[0] if T > 1 else H * D, st[1] if H > 1 else D
+        if st[2] == 1 and x.data_ptr() % 16 == 0 and token > 0 and head > 0 and token * es % 16 == 0 and head * es % 16 == 0:
+            return x, _lib.i64x2((token, head))
+        x = x.contiguous()
+    if x.data_ptr() % 16 != 0:  # a contiguous tensor may still start off a 16-byte boundary
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x, _lib.i64x2((H * D, D))
 
 
 def _borders(cu, name, dev):
@@ -61,7 +64,7 @@ def _checked(q, k, v, cu_seqlens_q, cu_seqlens_k):
     _lib.dtype_code(q)
     T, H, D = q.shape
     S, Hk = k.shape[:2]
-    if tuple(k.shape) != (S, Hk, D) or tuple(v.shape) != (S, Hk, D):
+    if k.shape[2] != D or v.shape != k.shape:
         raise ValueError(f"k/v shape {tuple(k.shape)}/{tuple(v.shape)} does not match q {tuple(q.shape)}")
     if H < 1 or Hk < 1 or H % Hk != 0:
         raise ValueError(f"the number of query heads ({H}) must be a multiple of the number of key heads ({Hk})")
@@ -75,10 +78,7 @@ def _checked(q, k, v, cu_seqlens_q, cu_seqlens_k):
         raise ValueError("without cu_seqlens_k the keys are the queries' own tokens: q and k must have the same length")
     if cu_q.numel() != cu_k.numel():
         raise ValueError(f"cu_seqlens_q and cu_seqlens_k name different numbers of sequences ({cu_q.numel() - 1} and {cu_k.numel() - 1})")
-    q, k, v = [x if _usable(x) else x.contiguous() for x in (q, k, v)]
-    # a contiguous tensor may still start off a 16-byte boundary
-    q, k, v = [x if x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format) for x in (q, k, v)]
-    return dev, q, k, v, cu_q, cu_k
+    return dev, T, S, H, Hk, D, cu_q, cu_k
 
 
 def packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=False, softmax_scale=None, max_seqlen_q=None,
@@ -87,9 +87,7 @@ def packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=Fa
     scale = _scale(softmax_scale, q.shape[-1])
     if max_seqlen_q is not None and int(max_seqlen_q) < 0:
         raise ValueError(f"max_seqlen_q must not be negative, got {max_seqlen_q}")
-    dev, q, k, v, cu_q, cu_k = _checked(q, k, v, cu_seqlens_q, cu_seqlens_k)
-    T, H, D = q.shape
-    S, Hk = k.shape[:2]
+    dev, T, S, H, Hk, D, cu_q, cu_k = _checked(q, k, v, cu_seqlens_q, cu_seqlens_k)
     o = torch.empty((T, H, D), device=dev, dtype=q.dtype)
     lse = torch.empty((H, T), device=dev, dtype=torch.float32) if return_lse else None
     if T == 0:
@@ -98,14 +96,15 @@ def packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=Fa
         if lse is not None:
             lse.fill_(float("-inf"))
         return o.zero_(), lse
-    nseq, code = cu_q.numel() - 1, _lib.dtype_code(q)
+    (q, qs), (k, ks), (v, vs) = _prepared(q), _prepared(k), _prepared(v)
+    nseq, code = cu_q.shape[0] - 1, _lib.dtype_code(q)
     most = T if max_seqlen_q is None else min(T, int(max_seqlen_q))
     lib = _lib.load()
-    nbytes = int(lib.gw_packed_attn_fwd_workspace_bytes(code, nseq, T, S, H, Hk, D, most))
     with _lib.on_device(dev):
+        nbytes = lib.gw_packed_attn_fwd_workspace_bytes(code, nseq, T, S, H, Hk, D, most)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         rc = lib.gw_packed_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), code, cu_q.data_ptr(), cu_k.data_ptr(), nseq, T, S, H, Hk, D,
-                                    _strides(q), _strides(k), _strides(v), scale, int(bool(causal)), most, o.data_ptr(), _lib.ptr(lse),
+                                    qs, ks, vs, scale, int(bool(causal)), most, o.data_ptr(), _lib.ptr(lse),
                                     _lib.ptr(ws), nbytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "gw_packed_attn_fwd")
     if _lib.debug_enabled():
@@ -117,10 +116,8 @@ def packed_attention_backward(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, d_out
     """Gradients ``(dq, dk, dv)`` of the forward, contiguous and of the inputs' dtype.  The sums run in a fixed order
     (one kernel owns query rows, another key rows; no atomics), so results are reproducible."""
     scale = _scale(softmax_scale, q.shape[-1])
-    dev, q, k, v, cu_q, cu_k = _checked(q, k, v, cu_seqlens_q, cu_seqlens_k)
+    dev, T, S, H, Hk, D, cu_q, cu_k = _checked(q, k, v, cu_seqlens_q, cu_seqlens_k)
     _lib.require_cuda(q, o, lse, d_out)
-    T, H, D = q.shape
-    S, Hk = k.shape[:2]
     if tuple(o.shape) != (T, H, D) or tuple(d_out.shape) != (T, H, D) or tuple(lse.shape) != (H, T):
         raise ValueError("o, d_out and lse must be the forward's: [tokens, heads, head_dim] twice and [heads, tokens]")
     if lse.dtype != torch.float32 or o.dtype != q.dtype:
@@ -129,18 +126,16 @@ def packed_attention_backward(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, d_out
     dk, dv = [torch.empty((S, Hk, D), device=dev, dtype=q.dtype) for _ in range(2)]
     if T == 0 or S == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    d_out = d_out.to(q.dtype)
-    d_out = d_out if _usable(d_out) else d_out.clone(memory_format=torch.contiguous_format)
-    o, lse = o.contiguous(), lse.contiguous()
+    (q, qs), (k, ks), (v, vs), (d_out, ds) = _prepared(q), _prepared(k), _prepared(v), _prepared(d_out.to(q.dtype))
+    o, lse = _prepared(o.contiguous())[0], lse.contiguous()
     nseq = cu_q.numel() - 1
     lib = _lib.load()
-    nbytes = int(lib.gw_packed_attn_bwd_workspace_bytes(T, H))
+    nbytes = lib.gw_packed_attn_bwd_workspace_bytes(T, H)
     with _lib.on_device(dev):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         rc = lib.gw_packed_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), d_out.data_ptr(),
-                                    _lib.dtype_code(q), cu_q.data_ptr(), cu_k.data_ptr(), nseq, T, S, H, Hk, D, _strides(q), _strides(k),
-                                    _strides(v), _strides(d_out), scale, int(bool(causal)), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                    ws.data_ptr(), nbytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
+                                    _lib.dtype_code(q), cu_q.data_ptr(), cu_k.data_ptr(), nseq, T, S, H, Hk, D, qs, ks, vs, ds,
+                                    scale, int(bool(causal)), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nbytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "gw_packed_attn_bwd")
     if _lib.debug_enabled():
         _lib.check_status(dev)
