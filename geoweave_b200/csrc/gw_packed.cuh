@@ -89,16 +89,100 @@ __device__ __forceinline__ bool packed_find(const PackedParams& p, bool key_side
   return false;
 }
 
-// The rows of one head behind the last sequence, shared by the blocks `part` of `parts`.
+// Tiles of a sequence whose work is at least x (in tiles of the other side); the work of a tile is the number of keys (key side:
+// queries) that its rows see.  Under a causal mask work grows towards the last query tile and falls from the first key tile.
+__device__ __forceinline__ int packed_at_least(const PackedParams& p, bool key_side, int R, int lq, int lk, int x) {
+  const int n = ((key_side ? lk : lq) + R - 1) / R, other = key_side ? lq : lk;
+  if (x <= 0) return n;
+  const int64_t below = static_cast<int64_t>(x - 1) * R;  // work of x tiles: more than this
+  if (!p.causal) return other > below ? n : 0;
+  if (key_side) {
+    if (lq <= below || lk <= below) return 0;
+    return min(n, static_cast<int>((lk - below + R - 1) / R));
+  }
+  if (lk <= below) return 0;
+  const int64_t y = below - (lk - lq);  // the tile's last query must lie behind this
+  return y < 0 ? n : n - static_cast<int>(y / R);
+}
+
+// As packed_find, but tile `rank` in falling order of work, so that blocks which start late have little left to do.  For up to
+// kSortedSeqs sequences; with more of them each is a small part of the whole and the order of the arrays serves as well.
+constexpr int kSortedSeqs = 64;
+__device__ __forceinline__ bool packed_find_sorted(const PackedParams& p, bool key_side, int R, int64_t rank, PackedSeq* out, int64_t* tiles,
+                                                   int64_t* end) {
+  if (p.nseq > kSortedSeqs) {
+    if (!packed_find(p, key_side, R, rank, out, tiles, end)) return false;
+    if (p.causal && !key_side) out->tile = (out->lq + R - 1) / R - 1 - out->tile;
+    return true;
+  }
+  const int lane = threadIdx.x & 31;
+  constexpr int SETS = kSortedSeqs / 32;
+  int q0[SETS], lq[SETS], k0[SETS], lk[SETS], top = 0;
+#pragma unroll
+  for (int i = 0; i < SETS; ++i) {
+    const int b = i * 32 + lane;
+    q0[i] = lq[i] = k0[i] = lk[i] = 0;
+    if (b < p.nseq) {
+      q0[i] = packed_border(p.cu_q, b, p.total_q);
+      k0[i] = packed_border(p.cu_k, b, p.total_k);
+      lq[i] = max(0, packed_border(p.cu_q, b + 1, p.total_q) - q0[i]);
+      lk[i] = max(0, packed_border(p.cu_k, b + 1, p.total_k) - k0[i]);
+    }
+    top = max(top, ((key_side ? lq[i] : lk[i]) + R - 1) / R);
+  }
+  top = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<unsigned>(top)));
+  auto count = [&](int x) {  // totals fit 32 bits: fewer than 2^31 tokens, and each tile holds one at least
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < SETS; ++i) n += packed_at_least(p, key_side, R, lq[i], lk[i], x);
+    return static_cast<int64_t>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(n)));
+  };
+  if (rank >= count(0)) return packed_find(p, key_side, R, rank, out, tiles, end);
+  int lo = 0, hi = top;  // the largest x with more than `rank` tiles of that much work
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (count(mid) > rank)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  int64_t left = rank - count(lo + 1);
+#pragma unroll
+  for (int i = 0; i < SETS; ++i) {
+    const int ge = packed_at_least(p, key_side, R, lq[i], lk[i], lo), more = packed_at_least(p, key_side, R, lq[i], lk[i], lo + 1);
+    int incl = ge - more;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += up;
+    }
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    if (left < total) {
+      const int src = __ffs(__ballot_sync(0xffffffffu, left < incl)) - 1;
+      const int at = static_cast<int>(left) - (incl - (ge - more));
+      const int n = ((key_side ? lk[i] : lq[i]) + R - 1) / R;
+      out->q0 = __shfl_sync(0xffffffffu, q0[i], src);
+      out->lq = __shfl_sync(0xffffffffu, lq[i], src);
+      out->k0 = __shfl_sync(0xffffffffu, k0[i], src);
+      out->lk = __shfl_sync(0xffffffffu, lk[i], src);
+      out->tile = __shfl_sync(0xffffffffu, key_side ? more + at : n - ge + at, src);
+      return true;
+    }
+    left -= total;
+  }
+  return false;  // not reached: the counts above say that the tile exists
+}
+
+// The rows of one head behind the last sequence, shared by the blocks `part` of `parts`, each with its first `threads` threads.
 template <typename T>
 __device__ __forceinline__ void packed_zero_rows(void* out, float* lse, int64_t from, int64_t to, int heads, int head, int D, int64_t part,
-                                                 int64_t parts) {
+                                                 int64_t parts, int threads) {
   T* dst = static_cast<T*>(out);
   const int64_t n = (to - from) * D;
-  for (int64_t i = part * blockDim.x + threadIdx.x; i < n; i += parts * blockDim.x)
+  for (int64_t i = part * threads + threadIdx.x; i < n; i += parts * threads)
     dst[((from + i / D) * heads + head) * D + i % D] = from_float<T>(0.f);
   if (lse != nullptr)
-    for (int64_t i = from + part * blockDim.x + threadIdx.x; i < to; i += parts * blockDim.x)
+    for (int64_t i = from + part * threads + threadIdx.x; i < to; i += parts * threads)
       lse[static_cast<int64_t>(head) * to + i] = -INFINITY;
 }
 
@@ -109,7 +193,7 @@ int packed_plain_fwd(const PackedParams& p, cudaStream_t st);
 int packed_plain_bwd(const PackedParams& p, cudaStream_t st);
 int packed_plain_split(const PackedParams& p, int chunk, int64_t slots, float* part_o, float* part_ml, cudaStream_t st);
 // 16-bit tensors (gw_packed_fwd.cu, gw_packed_bwd.cu)
-int packed_mma_fwd(const PackedParams& p, int dtype, int dev, cudaStream_t st);
+int packed_mma_fwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t st);
 int packed_mma_bwd(const PackedParams& p, int dtype, int dev, cudaStream_t st);
 // few query rows, divided along the keys (gw_packed_split.cu)
 bool packed_split_fits(const PackedParams& p, int64_t max_q);

@@ -69,7 +69,7 @@ extern "C" int gw_packed_attn_fwd(const void* q, const void* k, const void* v, i
     if (!workspace || !aligned16(workspace) || workspace_bytes < packed_split_bytes(p, facts.sms)) return GW_ERR_WORKSPACE;
     return packed_split_fwd(p, dtype, max_q, facts.sms, workspace, st);
   }
-  return dtype == GW_F32 ? packed_plain_fwd(p, st) : packed_mma_fwd(p, dtype, dev, st);
+  return dtype == GW_F32 ? packed_plain_fwd(p, st) : packed_mma_fwd(p, dtype, dev, facts.sms, st);
 }
 
 extern "C" size_t gw_packed_attn_bwd_workspace_bytes(int64_t total_q, int H) {

@@ -109,7 +109,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const int head = blockIdx.y, kv = head / (p.H / p.Hk);
   const uint32_t tmem = bwd_setup(sh, p, false, warp, lane);
   if (!sh->found) {
-    packed_zero_rows<T>(p.dq, nullptr, sh->end, p.total_q, p.H, head, p.D, blockIdx.x - sh->tiles, gridDim.x - sh->tiles);
+    packed_zero_rows<T>(p.dq, nullptr, sh->end, p.total_q, p.H, head, p.D, blockIdx.x - sh->tiles, gridDim.x - sh->tiles, blockDim.x);
   } else {
     const PackedSeq s = sh->seq;
     const int off = s.lk - s.lq;
@@ -308,8 +308,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const uint32_t tmem = bwd_setup(sh, p, true, warp, lane);
   if (!sh->found) {
     const int64_t part = blockIdx.x - sh->tiles, parts = gridDim.x - sh->tiles;
-    packed_zero_rows<T>(p.dk, nullptr, sh->end, p.total_k, p.Hk, kv, p.D, part, parts);
-    packed_zero_rows<T>(p.dv, nullptr, sh->end, p.total_k, p.Hk, kv, p.D, part, parts);
+    packed_zero_rows<T>(p.dk, nullptr, sh->end, p.total_k, p.Hk, kv, p.D, part, parts, blockDim.x);
+    packed_zero_rows<T>(p.dv, nullptr, sh->end, p.total_k, p.Hk, kv, p.D, part, parts, blockDim.x);
   } else {
     const PackedSeq s = sh->seq;
     const int off = s.lk - s.lq;

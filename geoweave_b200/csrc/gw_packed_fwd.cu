@@ -8,8 +8,12 @@
 // 2^8 (P then lies within 2^8, where both 16-bit types keep their full precision, and l in fp32), which after the first tiles
 // hardly ever happens, so the rescaling pass over O is off the critical path.
 //
-// Warps 0-3 and 4-7 are the softmax of the two tiles, warp 8 loads, warp 9 issues the products.  The two tiles alternate:
-// while one is in its softmax the tensor cores make the other's S and O.
+// A persistent block takes its items (256 rows of a head) from a list in falling order of work, one in every gridDim: the loads of
+// the next item run under the last products and the output of this one.  Warps 0-3 and 4-7 are the softmax of the two tiles,
+// warp 8 makes the work list and loads, the rest issue products.  While one tile is in its softmax the tensor cores make the
+// other's S and O, and its own next S where P has room beside S (head dims up to 64: one issuing warp for each tile, so
+// that neither waits for the other).  For wide heads P sits on S, the tensor cores are busy all the time, and one warp issues
+// for both tiles in turn, which keeps them half a period apart; with two issuers their products interleave and the tiles fall into step.
 #include "gw_packed_mma.cuh"
 
 namespace gw {
@@ -42,217 +46,310 @@ int make_token_map(CUtensorMap* map, const void* base, int dtype, int64_t tokens
 
 namespace {
 
-constexpr int kFwdThreads = 320;
 constexpr float kLag = 8.f;  // a maximum may grow by this much (as a power of two) before O is rescaled
+constexpr int kTiles = 2;    // query tiles of a block
+constexpr int kWarps = 4 * kTiles;
+constexpr int kLoad = kWarps, kIssue = kWarps + 1;  // warps: softmax first, then one that loads, then those that issue products
 
 template <int DP>
 struct FwdShape {
-  static constexpr int kStages = DP == 64 ? 4 : 2;       // K and V rings
+  static constexpr int kIssuers = DP == 64 ? 2 : 1;
+  static constexpr int kThreads = (kIssue + kIssuers) * 32;
+  static constexpr int kStages = DP == 64 ? 4 : 2;  // K and V rings
   static constexpr int kTileBytes = DP / 64 * kBoxBytes;
   // tensor memory: S of both tiles, then P where it has room of its own (it takes S's place for wide heads), then O
   static constexpr uint32_t kS = 0, kP = DP == 64 ? 256 : 0, kPStride = DP == 64 ? 64 : 128, kO = DP == 64 ? 384 : 256;
-  static constexpr size_t kSmem = 1024 + static_cast<size_t>(2 + 2 * kStages) * kTileBytes + 512;
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kTiles + 2 * kStages) * kTileBytes + 512;
 };
 
-template <int STAGES>
+enum { kItemRows, kItemTail, kItemEnd };
+struct FwdItem {  // 256 rows of a head; or some rows behind the last sequence; or the end of the list
+  int kind, head, q0, lq, k0, lk, r0;
+  int keys[kTiles], n[kTiles], most;  // keys that any row of each tile sees; key tiles of each, of both
+  int64_t part, parts, end;
+};
+
 struct FwdShared {
-  uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
-  uint64_t k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES];
-  PackedSeq seq;
-  int64_t tiles, end;
-  int found;
+  uint64_t q_full[kTiles], q_empty[kTiles], s_full[kTiles], s_read[kTiles], p_full[kTiles], o_done[kTiles];
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t item_full[2], item_empty[2];
+  FwdItem item[2];
   uint32_t tmem_base;
   volatile int abort_flag;
 };
+static_assert(sizeof(FwdShared) <= 512, "shared bookkeeping");
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+__global__ void __launch_bounds__(FwdShape<DP>::kThreads, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                  const PackedParams p, const int ab_format) {
+                  const PackedParams p, const int64_t slots, const int ab_format) {
   using Shape = FwdShape<DP>;
-  constexpr int ST = Shape::kStages, TB = Shape::kTileBytes;
+  constexpr int ST = Shape::kStages, TB = Shape::kTileBytes, NI = Shape::kIssuers;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* q_smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  unsigned char* k_smem = q_smem + 2 * TB;
+  unsigned char* k_smem = q_smem + kTiles * TB;
   unsigned char* v_smem = k_smem + ST * TB;
-  FwdShared<ST>* sh = reinterpret_cast<FwdShared<ST>*>(v_smem + ST * TB);
-  static_assert(sizeof(FwdShared<ST>) <= 512, "shared bookkeeping");
+  FwdShared* sh = reinterpret_cast<FwdShared*>(v_smem + ST * TB);
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
-  const int head = blockIdx.y, kv = head / (p.H / p.Hk);
 
-  if (warp == 8) {
-    PackedSeq s{};
-    int64_t tiles = 0, end = 0;
-    const bool found = packed_find(p, false, 2 * kTile, blockIdx.x, &s, &tiles, &end);
-    if (lane == 0) {
-      sh->seq = s;
-      sh->tiles = tiles;
-      sh->end = end;
-      sh->found = found;
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&sh->q_full[i], 1);
-        mbar_init(&sh->s_full[i], 1);
-        mbar_init(&sh->p_full[i], 4);
-        mbar_init(&sh->o_done[i], 1);
-      }
-      for (int i = 0; i < ST; ++i) {
-        mbar_init(&sh->k_full[i], 1);
-        mbar_init(&sh->k_empty[i], 1);
-        mbar_init(&sh->v_full[i], 1);
-        mbar_init(&sh->v_empty[i], 1);
-      }
-      sh->abort_flag = 0;
-      mbar_fence_init();
-      fence_proxy_async_smem();
+  if (warp == kLoad && lane == 0) {
+    for (int i = 0; i < kTiles; ++i) {
+      mbar_init(&sh->q_full[i], 1);
+      mbar_init(&sh->q_empty[i], 1);
+      mbar_init(&sh->s_full[i], 1);
+      mbar_init(&sh->s_read[i], 4);
+      mbar_init(&sh->p_full[i], 4);
+      mbar_init(&sh->o_done[i], 1);
     }
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&sh->k_full[i], 1);
+      mbar_init(&sh->k_empty[i], NI);
+      mbar_init(&sh->v_full[i], 1);
+      mbar_init(&sh->v_empty[i], NI);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh->item_full[i], 1);
+      mbar_init(&sh->item_empty[i], kWarps + NI);
+    }
+    sh->abort_flag = 0;
+    mbar_fence_init();
+    fence_proxy_async_smem();
   }
-  if (warp == 9) tmem_alloc(&sh->tmem_base, 512);
+  if (warp == kIssue) tmem_alloc(&sh->tmem_base, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh->tmem_base, 0);
-  if (!sh->found) {
-    packed_zero_rows<T>(p.o, p.lse, sh->end, p.total_q, p.H, head, p.D, blockIdx.x - sh->tiles, gridDim.x - sh->tiles);
-  } else {
-    const PackedSeq s = sh->seq;
-    const int off = s.lk - s.lq;
-    // longest first: under a causal mask the later tiles of a sequence see more keys
-    const int tile = p.causal ? (s.lq + 2 * kTile - 1) / (2 * kTile) - 1 - s.tile : s.tile;
-    const int r0 = tile * 2 * kTile;
-    int keys[2], n[2];  // keys that any row of each tile sees; key tiles
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int last = min(r0 + (t + 1) * kTile, s.lq);
-      keys[t] = last <= r0 + t * kTile ? 0 : p.causal ? max(0, min(s.lk, last + off)) : s.lk;
-      n[t] = (keys[t] + kTile - 1) / kTile;
-    }
-    const int most = max(n[0], n[1]);
+  bool ok = true;
 
-    if (warp == 8) {
-      // ------------------------------ loads ------------------------------
-      if (lane == 0) {
-        bool ok = true;
-        int j = 0;
-        for (int t = 0; t < 2; ++t)
-          if (n[t] > 0) {
-            mbar_arrive_expect_tx(&sh->q_full[t], TB);
-            load_rows<DP>(q_smem + t * TB, &tmQ, head, s.q0 + r0 + t * kTile, &sh->q_full[t]);
-          }
-        for (; j < most; ++j) {
-          const int st = j % ST;
-          const uint32_t par = ((j / ST) & 1u) ^ 1u;
-          ok = mbar_wait_bounded(&sh->k_empty[st], par);
-          if (!ok || sh->abort_flag) break;
-          mbar_arrive_expect_tx(&sh->k_full[st], TB);
-          load_rows<DP>(k_smem + st * TB, &tmK, kv, s.k0 + j * kTile, &sh->k_full[st]);
-          ok = mbar_wait_bounded(&sh->v_empty[st], par);
-          mbar_arrive_expect_tx(&sh->v_full[st], TB);
-          load_rows<DP>(v_smem + st * TB, &tmV, kv, s.k0 + j * kTile, &sh->v_full[st]);
-          if (!ok || sh->abort_flag) { ++j; break; }
+  if (warp == kLoad) {
+    // ------------------------------ work list and loads ------------------------------
+    uint32_t ring = 0, q_use[kTiles] = {};  // key tiles and query tiles loaded so far
+    int i = 0;
+    for (int64_t at = blockIdx.x; ok && !sh->abort_flag; at += gridDim.x, ++i) {
+      FwdItem w{};
+      w.head = static_cast<int>(at % p.H);
+      const int64_t rank = at / p.H;
+      PackedSeq seq{};
+      int64_t tiles = 0;
+      if (rank >= slots) {
+        w.kind = kItemEnd;
+      } else if (packed_find_sorted(p, false, kTiles * kTile, rank, &seq, &tiles, &w.end)) {
+        w.kind = kItemRows;
+        w.q0 = seq.q0;
+        w.lq = seq.lq;
+        w.k0 = seq.k0;
+        w.lk = seq.lk;
+        w.r0 = seq.tile * kTiles * kTile;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          const int last = min(w.r0 + (t + 1) * kTile, w.lq);
+          w.keys[t] = last <= w.r0 + t * kTile ? 0 : p.causal ? max(0, min(w.lk, last + w.lk - w.lq)) : w.lk;
+          w.n[t] = (w.keys[t] + kTile - 1) / kTile;
+          w.most = max(w.most, w.n[t]);
         }
-        if (!ok) sh->abort_flag = 1;
-        if (sh->abort_flag) {  // let the copies in flight land before the shared memory is given up
-          for (int t = 0; t < 2; ++t)
-            if (n[t] > 0) mbar_wait_limit(&sh->q_full[t], 0, kDrainLimitNs);
-          for (int u = max(0, j - ST); u < j; ++u) {
-            mbar_wait_limit(&sh->k_full[u % ST], (u / ST) & 1u, kDrainLimitNs);
-            mbar_wait_limit(&sh->v_full[u % ST], (u / ST) & 1u, kDrainLimitNs);
-          }
-          report_status(p.status, GW_ERR_TIMEOUT);
+      } else {
+        w.kind = kItemTail;
+        w.part = rank - tiles;
+        w.parts = slots - tiles;
+      }
+      ok = mbar_wait_bounded(&sh->item_empty[i & 1], ((i >> 1) & 1) ^ 1);
+      if (!ok) break;
+      if (lane == 0) {
+        sh->item[i & 1] = w;
+        mbar_arrive(&sh->item_full[i & 1]);
+      }
+      if (w.kind == kItemEnd) break;
+      if (w.kind == kItemTail) continue;
+      const int kv = w.head / (p.H / p.Hk);
+      auto load_q = [&](int t) {
+        ok = ok && mbar_wait_bounded(&sh->q_empty[t], (q_use[t] & 1) ^ 1);
+        if (!ok) return;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sh->q_full[t], TB);
+          load_rows<DP>(q_smem + t * TB, &tmQ, w.head, w.q0 + w.r0 + t * kTile, &sh->q_full[t]);
+        }
+        ++q_use[t];
+      };
+      for (int j = 0; j < w.most && ok && !sh->abort_flag; ++j, ++ring) {
+        const int st = ring % ST;
+        const uint32_t par = ((ring / ST) & 1u) ^ 1u;
+        if (j == 0 && w.n[0] > 0) load_q(0);
+        ok = ok && mbar_wait_bounded(&sh->k_empty[st], par);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&sh->k_full[st], TB);
+          load_rows<DP>(k_smem + st * TB, &tmK, kv, w.k0 + j * kTile, &sh->k_full[st]);
+        }
+        if (j == 0 && w.n[1] > 0) load_q(1);
+        ok = ok && mbar_wait_bounded(&sh->v_empty[st], par);
+        if (lane == 0) {  // also after a wait that ran out, so that the drain below finds both copies of the stage
+          mbar_arrive_expect_tx(&sh->v_full[st], TB);
+          load_rows<DP>(v_smem + st * TB, &tmV, kv, w.k0 + j * kTile, &sh->v_full[st]);
         }
       }
-    } else if (warp == 9) {
-      // ------------------------------ products ------------------------------
-      const uint32_t idesc_s = make_idesc_mn(ab_format, kTile, kTile);
-      const uint32_t idesc_o = make_idesc_mn(ab_format, kTile, DP) | kBMajorMN;
-      const uint64_t qd = make_smem_desc(smem_u32(q_smem)), kd = make_smem_desc(smem_u32(k_smem)), vd = make_smem_desc_mn(smem_u32(v_smem));
-      bool ok = true;
-      auto scores = [&](int t, int j) {
+    }
+    if (!ok) sh->abort_flag = 1;
+    if (sh->abort_flag && lane == 0) {  // let the copies in flight land before the shared memory is given up
+      for (int t = 0; t < kTiles; ++t)
+        if (q_use[t] > 0) mbar_wait_limit(&sh->q_full[t], (q_use[t] - 1) & 1, kDrainLimitNs);
+      for (uint32_t u = ring > ST ? ring - ST : 0u; u <= ring; ++u) {
+        mbar_wait_limit(&sh->k_full[u % ST], (u / ST) & 1u, kDrainLimitNs);
+        mbar_wait_limit(&sh->v_full[u % ST], (u / ST) & 1u, kDrainLimitNs);
+      }
+      report_status(p.status, GW_ERR_TIMEOUT);
+    }
+  } else if (warp >= kIssue) {
+    // ------------------------------ products: of one tile, or of both in turn ------------------------------
+    const int w0 = warp - kIssue;
+    const uint32_t idesc_s = make_idesc_mn(ab_format, kTile, kTile);
+    const uint32_t idesc_o = make_idesc_mn(ab_format, kTile, DP) | kBMajorMN;
+    const uint64_t qd = make_smem_desc(smem_u32(q_smem)), kd = make_smem_desc(smem_u32(k_smem));
+    const uint64_t vd = make_smem_desc_mn(smem_u32(v_smem));
+    uint32_t ring = 0, done[kTiles] = {}, q_use[kTiles] = {};  // key tiles in the ring before this item; of each tile; query tiles
+    for (int i = 0; ok && !sh->abort_flag; ++i) {
+      ok = mbar_wait_bounded(&sh->item_full[i & 1], (i >> 1) & 1);
+      if (!ok) break;
+      const FwdItem* item = &sh->item[i & 1];
+      const int kind = item->kind, most = item->most, lk = item->lk;
+      int n[kTiles], keys[kTiles];
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        n[t] = item->n[t];
+        keys[t] = item->keys[t];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->item_empty[i & 1]);
+      if (kind == kItemEnd) break;
+      if (kind == kItemTail) continue;
+      auto scores = [&](int t, int j) {  // S of key tile j; S has been read: for wide heads P, which sits on it, has been used
+        const uint32_t at = ring + j, c = done[t] + j;
+        if (j == 0) ok = ok && mbar_wait_bounded(&sh->q_full[t], q_use[t] & 1);
+        ok = ok && mbar_wait_bounded(&sh->k_full[at % ST], (at / ST) & 1);
+        if (DP == 64 && c > 0) ok = ok && mbar_wait_bounded(&sh->s_read[t], (c - 1) & 1);
+        if (!ok) return;
+        tc_fence_after();
         if (lane == 0) {
-          mma_rows<DP>(tmem + Shape::kS + t * kTile, qd + t * (TB >> 4), kd + (j % ST) * (TB >> 4), idesc_s);
+          mma_rows<DP>(tmem + Shape::kS + t * kTile, qd + t * (TB >> 4), kd + (at % ST) * (TB >> 4), idesc_s);
           tc_commit(&sh->s_full[t]);
+          if (j + 1 == n[t]) tc_commit(&sh->q_empty[t]);
         }
       };
-      if (most > 0) {
-        ok = mbar_wait_bounded(&sh->k_full[0], 0);
-        for (int t = 0; t < 2 && ok; ++t)
-          if (n[t] > 0) {
-            ok = mbar_wait_bounded(&sh->q_full[t], 0);
-            tc_fence_after();
-            if (ok) scores(t, 0);
-          }
-        if (lane == 0) tc_commit(&sh->k_empty[0]);
+      int mine = 0;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        if (t % NI != w0 || n[t] == 0) continue;
+        mine = max(mine, n[t]);
+        scores(t, 0);
+      }
+      // A stage goes back once for each issuer.  One whose tile does not read it still waits until it is full: running ahead
+      // of the loads it would count twice in one phase of the barrier.
+      auto pass_on = [&](uint64_t* full, uint64_t* empty, uint32_t at) {
+        ok = ok && mbar_wait_bounded(&full[at % ST], (at / ST) & 1);
+        if (ok && lane == 0) mbar_arrive(&empty[at % ST]);
+      };
+      if (mine > 0) {
+        if (lane == 0) tc_commit(&sh->k_empty[ring % ST]);
+      } else if (most > 0) {
+        pass_on(sh->k_full, sh->k_empty, ring);
       }
       for (int j = 0; j < most && ok && !sh->abort_flag; ++j) {
-        const int st = j % ST;
-        bool v_here = false, k_next = false;
-        for (int t = 0; t < 2; ++t) {
-          if (j >= n[t]) continue;
-          ok = ok && mbar_wait_bounded(&sh->p_full[t], j & 1);
-          if (ok && j + 1 < n[t] && !k_next) {
-            ok = mbar_wait_bounded(&sh->k_full[(j + 1) % ST], ((j + 1) / ST) & 1);
-            k_next = true;
-          }
-          if (ok && !v_here) {
-            ok = mbar_wait_bounded(&sh->v_full[st], (j / ST) & 1);
+        const uint32_t st = (ring + j) % ST, st_next = (ring + j + 1) % ST;
+        bool v_here = false;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          if (t % NI != w0 || j >= n[t]) continue;
+          const uint32_t c = done[t] + j;
+          if (DP == 64 && j + 1 < n[t]) scores(t, j + 1);  // P has its own place: ahead of this tile's softmax
+          if (!v_here) {
+            ok = ok && mbar_wait_bounded(&sh->v_full[st], ((ring + j) / ST) & 1);
+            if (ok && (j + 1) * kTile > lk) zero_rows_from<DP>(v_smem + st * TB, lk - j * kTile);
             v_here = true;
-            if (ok && (j + 1) * kTile > s.lk) zero_rows_from<DP>(v_smem + st * TB, s.lk - j * kTile);
           }
+          ok = ok && mbar_wait_bounded(&sh->p_full[t], c & 1);
           if (!ok) break;
           tc_fence_after();
-          // narrow heads have S free as soon as P is written elsewhere; for wide heads P sits on S
-          if (DP == 64 && j + 1 < n[t]) scores(t, j + 1);
           if (lane == 0) {
             const int steps = min(kTile, (keys[t] - j * kTile + 15) & ~15) / 16;
-            for (int i = 0; i < steps; ++i)
-              tc_mma_f16_ts(tmem + Shape::kO + t * DP, tmem + Shape::kP + t * Shape::kPStride + i * 8,
-                            vd + st * (TB >> 4) + i * (16 * 128 >> 4), idesc_o, (j > 0 || i > 0) ? 1u : 0u);
+            for (int k = 0; k < steps; ++k)
+              tc_mma_f16_ts(tmem + Shape::kO + t * DP, tmem + Shape::kP + t * Shape::kPStride + k * 8,
+                            vd + st * (TB >> 4) + k * (16 * 128 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
             tc_commit(&sh->o_done[t]);
           }
           if (DP != 64 && j + 1 < n[t]) scores(t, j + 1);
         }
-        if (lane == 0 && ok) {
-          tc_commit(&sh->v_empty[st]);
-          if (k_next) tc_commit(&sh->k_empty[(j + 1) % ST]);
+        if (j < mine) {
+          if (lane == 0 && ok) tc_commit(&sh->v_empty[st]);
+        } else {
+          pass_on(sh->v_full, sh->v_empty, ring + j);
+        }
+        if (j + 1 < mine) {
+          if (lane == 0 && ok) tc_commit(&sh->k_empty[st_next]);
+        } else if (j + 1 < most) {
+          pass_on(sh->k_full, sh->k_empty, ring + j + 1);
         }
       }
-      if (!ok) {
-        sh->abort_flag = 1;
-        if (lane == 0) report_status(p.status, GW_ERR_TIMEOUT);
+      ring += most;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        done[t] += n[t];
+        q_use[t] += n[t] > 0 ? 1 : 0;
       }
-    } else {
-      // ------------------------------ softmax and output ------------------------------
-      const int t = warp >> 2;
-      const int row = r0 + t * kTile + (warp & 3) * 32 + lane;
-      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const uint32_t s_addr = tmem + lanes + Shape::kS + t * kTile, p_addr = tmem + lanes + Shape::kP + t * Shape::kPStride;
-      const uint32_t o_addr = tmem + lanes + Shape::kO + t * DP;
-      const float c = p.scale * kLog2e;
-      const int limit = p.causal ? min(s.lk, row + off + 1) : s.lk;  // keys this row sees
-      const int open = p.causal ? min(s.lk, r0 + t * kTile + off + 1) : s.lk;  // keys that every row of the tile sees
-      const int tiles = n[t];
+    }
+    if (!ok) {
+      sh->abort_flag = 1;
+      if (lane == 0) report_status(p.status, GW_ERR_TIMEOUT);
+    }
+  } else {
+    // ------------------------------ softmax and output ------------------------------
+    const int t = warp >> 2;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + Shape::kS + t * kTile, p_addr = tmem + lanes + Shape::kP + t * Shape::kPStride;
+    const uint32_t o_addr = tmem + lanes + Shape::kO + t * DP;
+    const float c = p.scale * kLog2e;
+    uint32_t done = 0;  // key tiles of this tile so far
+    for (int i = 0; ok && !sh->abort_flag; ++i) {
+      ok = mbar_wait_bounded(&sh->item_full[i & 1], (i >> 1) & 1);
+      if (!ok) break;
+      const FwdItem* item = &sh->item[i & 1];  // given back behind the output
+      const int kind = item->kind;
+      if (kind == kItemEnd) break;
+      if (kind == kItemTail) {
+        packed_zero_rows<T>(p.o, p.lse, item->end, p.total_q, p.H, item->head, p.D, item->part, item->parts, kWarps * 32);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->item_empty[i & 1]);
+        continue;
+      }
+      const int lk = item->lk, off = lk - item->lq, first = item->r0 + t * kTile, row = first + (warp & 3) * 32 + lane;
+      const int limit = p.causal ? min(lk, row + off + 1) : lk;   // keys this row sees
+      const int open = p.causal ? min(lk, first + off + 1) : lk;  // keys that every row of the tile sees
+      const int tiles = item->n[t];
       float m = -INFINITY, l = 0.f;
-      bool ok = true;
-      for (int j = 0; j < tiles; ++j) {
-        ok = mbar_wait_bounded(&sh->s_full[t], j & 1);
+      for (int j = 0; j < tiles; ++j, ++done) {
+        ok = mbar_wait_bounded(&sh->s_full[t], done & 1);
         if (!ok || sh->abort_flag) break;
         tc_fence_after();
         float x[128];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_load32(s_addr + 32 * i, x + 32 * i);
+        for (int k = 0; k < 4; ++k) tmem_load32(s_addr + 32 * k, x + 32 * k);
         tmem_wait_ld();
+        if (DP == 64) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->s_read[t]);
+        }
         if ((j + 1) * kTile > open) {
           const int valid = limit - j * kTile;
 #pragma unroll
-          for (int i = 0; i < 128; ++i) x[i] = i < valid ? x[i] : -INFINITY;
+          for (int k = 0; k < 128; ++k) x[k] = k < valid ? x[k] : -INFINITY;
         }
         float top[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int i = 4; i < 128; i += 8) {
+        for (int k = 4; k < 128; k += 8) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], fmaxf(x[i + k], i + 4 + k < 128 ? x[i + 4 + k] : x[i + k]));
+          for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(x[k + e], k + 4 + e < 128 ? x[k + 4 + e] : x[k + e]));
         }
         const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         bool o_ready = false;
@@ -264,18 +361,18 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const float shrink = grown ? exp2_fast((m - mx) * c) : 1.f;
             l *= shrink;
             if (grown) m = mx;
-            ok = mbar_wait_bounded(&sh->o_done[t], (j - 1) & 1);
+            ok = mbar_wait_bounded(&sh->o_done[t], (done - 1) & 1);
             if (!ok) break;
             o_ready = true;
             tc_fence_after();
 #pragma unroll 1
-            for (int b = 0; b < DP / 32; ++b) {
-              float o[32];
-              tmem_load32(o_addr + 32 * b, o);
+            for (int b = 0; b < DP / 8; ++b) {  // narrow pieces: the row's 128 scores are in registers
+              uint32_t o[8];
+              tmem_ld_x8(o_addr + 8 * b, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] *= shrink;
-              tmem_store32(o_addr + 32 * b, reinterpret_cast<const uint32_t*>(o));
+              for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * shrink);
+              tmem_store8(o_addr + 8 * b, o);
             }
             tmem_wait_st();
           }
@@ -285,20 +382,20 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         uint64_t sum[2] = {0, 0};
         uint32_t pk[64];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
+        for (int k = 0; k < 64; ++k) {
           float a, b;
-          unpack_f2(fma_f2(pack_f2(x[2 * i], x[2 * i + 1]), c2, base2), a, b);
+          unpack_f2(fma_f2(pack_f2(x[2 * k], x[2 * k + 1]), c2, base2), a, b);
           a = exp2_fast(a);
           b = exp2_fast(b);
-          sum[i & 1] = add_f2(sum[i & 1], pack_f2(a, b));
-          pk[i] = pack_half2<T>(a, b);
+          sum[k & 1] = add_f2(sum[k & 1], pack_f2(a, b));
+          pk[k] = pack_half2<T>(a, b);
         }
         float s0, s1, s2, s3;
         unpack_f2(sum[0], s0, s1);
         unpack_f2(sum[1], s2, s3);
         l += (s0 + s1) + (s2 + s3);
         if (DP == 64 && j > 0 && !o_ready) {  // the previous product still reads P (for wide heads S, and so P, waited for it)
-          ok = mbar_wait_bounded(&sh->o_done[t], (j - 1) & 1);
+          ok = mbar_wait_bounded(&sh->o_done[t], (done - 1) & 1);
           if (!ok) break;
           tc_fence_after();
         }
@@ -309,46 +406,52 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->p_full[t]);
       }
-      if (tiles > 0 && ok && !sh->abort_flag) ok = mbar_wait_bounded(&sh->o_done[t], (tiles - 1) & 1);
-      if (!ok) {
-        sh->abort_flag = 1;
-        report_status(p.status, GW_ERR_TIMEOUT);
+      if (!ok || sh->abort_flag) break;
+      if (tiles > 0) {
+        ok = mbar_wait_bounded(&sh->o_done[t], (done - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
       }
-      tc_fence_after();
-      const bool live = row < s.lq;
+      const bool live = row < item->lq;
+      const int64_t token = item->q0 + row;
+      const int head = item->head;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->item_empty[i & 1]);
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      T* dst = static_cast<T*>(p.o) + (static_cast<int64_t>(s.q0 + row) * p.H + head) * p.D;
+      T* dst = static_cast<T*>(p.o) + (token * p.H + head) * p.D;
 #pragma unroll 1
       for (int b = 0; b < DP / 32; ++b) {
         if (32 * b >= p.D) break;
         float o[32];
-        if (tiles > 0) {
-          tmem_load32(o_addr + 32 * b, o);
-          tmem_wait_ld();
-        }
+        tmem_load32(o_addr + 32 * b, o);  // without a key: whatever is there, and unused
+        tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint4 w;
-          uint32_t* e = reinterpret_cast<uint32_t*>(&w);
+        for (int k = 0; k < 4; ++k) {
+          uint4 out;
+          uint32_t* e = reinterpret_cast<uint32_t*>(&out);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            e[k] = l == 0.f ? 0u : pack_half2<T>(o[8 * i + 2 * k] * inv, o[8 * i + 2 * k + 1] * inv);
-          if (live && 32 * b + 8 * i < p.D) *reinterpret_cast<uint4*>(dst + 32 * b + 8 * i) = w;
+          for (int h = 0; h < 4; ++h) e[h] = l == 0.f ? 0u : pack_half2<T>(o[8 * k + 2 * h] * inv, o[8 * k + 2 * h + 1] * inv);
+          if (live && 32 * b + 8 * k < p.D) *reinterpret_cast<uint4*>(dst + 32 * b + 8 * k) = out;
         }
       }
+      tc_fence_before();  // O may be written again once this item's successor has its first P
       if (live && p.lse != nullptr)
-        p.lse[static_cast<int64_t>(head) * p.total_q + s.q0 + row] = l == 0.f ? -INFINITY : fmaf(m, p.scale, log2f(l) * kLn2);
+        p.lse[head * p.total_q + token] = l == 0.f ? -INFINITY : fmaf(m, p.scale, log2f(l) * kLn2);
+    }
+    if (!ok) {
+      sh->abort_flag = 1;
+      report_status(p.status, GW_ERR_TIMEOUT);
     }
   }
 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == kIssue) tmem_dealloc(tmem, 512);
 }
 
 template <typename T, int DP>
-int launch_fwd(const PackedParams& p, int dtype, int dev, cudaStream_t st) {
+int launch_fwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
   GW_CUDA_TRY(cudaSetDevice(dev));  // a thread that has launched nothing yet has no context to encode tensor maps in
   int rc = make_token_map(&mq, p.q, dtype, p.total_q, p.H, p.D, p.qs[0], p.qs[1]);
@@ -357,17 +460,18 @@ int launch_fwd(const PackedParams& p, int dtype, int dev, cudaStream_t st) {
   static OncePerDevice once;
   if (rc == GW_OK) rc = ensure_dynamic_smem(packed_fwd_kernel<T, DP>, FwdShape<DP>::kSmem, once, dev);
   if (rc != GW_OK) return rc;
-  const dim3 grid(static_cast<unsigned>(packed_tile_bound(p.total_q, 2 * kTile, p.nseq)), p.H);
-  packed_fwd_kernel<T, DP><<<grid, kFwdThreads, FwdShape<DP>::kSmem, st>>>(mq, mk, mv, p, dtype == GW_BF16 ? 1 : 0);
+  const int64_t slots = packed_tile_bound(p.total_q, kTiles * kTile, p.nseq), items = slots * p.H;
+  packed_fwd_kernel<T, DP><<<static_cast<unsigned>(items < sms ? items : sms), FwdShape<DP>::kThreads, FwdShape<DP>::kSmem, st>>>(
+      mq, mk, mv, p, slots, dtype == GW_BF16 ? 1 : 0);
   GW_LAUNCH_CHECK();
   return GW_OK;
 }
 
 }  // namespace
 
-int packed_mma_fwd(const PackedParams& p, int dtype, int dev, cudaStream_t st) {
-  if (dtype == GW_BF16) return p.D <= 64 ? launch_fwd<__nv_bfloat16, 64>(p, dtype, dev, st) : launch_fwd<__nv_bfloat16, 128>(p, dtype, dev, st);
-  return p.D <= 64 ? launch_fwd<__half, 64>(p, dtype, dev, st) : launch_fwd<__half, 128>(p, dtype, dev, st);
+int packed_mma_fwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t st) {
+  if (dtype == GW_BF16) return p.D <= 64 ? launch_fwd<__nv_bfloat16, 64>(p, dtype, dev, sms, st) : launch_fwd<__nv_bfloat16, 128>(p, dtype, dev, sms, st);
+  return p.D <= 64 ? launch_fwd<__half, 64>(p, dtype, dev, sms, st) : launch_fwd<__half, 128>(p, dtype, dev, sms, st);
 }
 
 }  // namespace gw

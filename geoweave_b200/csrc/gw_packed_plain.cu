@@ -110,8 +110,8 @@ __device__ __forceinline__ bool block_tile(const PackedParams& p, bool key_side,
   if (packed_find(p, key_side, BT, blockIdx.x, s, &tiles, &end)) return true;
   const int64_t total = key_side ? p.total_k : p.total_q, parts = gridDim.x - tiles, part = blockIdx.x - tiles;
   const int heads = key_side ? p.Hk : p.H;
-  packed_zero_rows<float>(out, lse, end, total, heads, head, p.D, part, parts);
-  if (out2 != nullptr) packed_zero_rows<float>(out2, nullptr, end, total, heads, head, p.D, part, parts);
+  packed_zero_rows<float>(out, lse, end, total, heads, head, p.D, part, parts, blockDim.x);
+  if (out2 != nullptr) packed_zero_rows<float>(out2, nullptr, end, total, heads, head, p.D, part, parts, blockDim.x);
   return false;
 }
 

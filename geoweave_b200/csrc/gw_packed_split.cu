@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_join_kernel(const SplitPa
     PackedSeq s;
     int64_t tiles, end;
     packed_find(p, false, 1, static_cast<int64_t>(0x7fffffffffffffff), &s, &tiles, &end);
-    for (int h = kv * group; h < (kv + 1) * group; ++h) packed_zero_rows<T>(p.o, p.lse, end, p.total_q, p.H, h, p.D, 0, 1);
+    for (int h = kv * group; h < (kv + 1) * group; ++h) packed_zero_rows<T>(p.o, p.lse, end, p.total_q, p.H, h, p.D, 0, 1, blockDim.x);
     return;
   }
   // chunks in front of this sequence

@@ -81,6 +81,16 @@ def test_many_short_sequences(dtype, D):
     _check(lens, lens, 2, 1, D, dtype, True, seed=5)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float16, 128), (torch.bfloat16, 40)])
+def test_more_work_than_blocks(dtype, D, causal):
+    """Several hundred items of every kind (full, half, and empty second tiles, no keys, more than eight key tiles), so that each
+    block takes several in a row."""
+    lens_q = [270, 17, 256, 129, 700, 0, 128, 1, 385, 513, 90, 260] * 3
+    lens_k = [270, 17, 300, 129, 1200, 5, 0, 640, 100, 513, 128, 260] * 3
+    _check(lens_q, lens_k, 16, 4, D, dtype, causal, seed=30)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("causal", [False, True])
 def test_rows_behind_the_last_sequence_are_zeros(dtype, causal):
