@@ -38,11 +38,11 @@ struct BwdShared {
 static_assert(sizeof(BwdShared) <= 512, "shared bookkeeping");
 
 // Barriers, the block's tile and tensor memory; the same in both kernels.
-__device__ __forceinline__ uint32_t bwd_setup(BwdShared* sh, const PackedParams& p, bool key_side, int warp, int lane) {
+__device__ __forceinline__ uint32_t bwd_setup(BwdShared* sh, const PackedParams& p, bool key_side, int heads, int warp, int lane) {
   if (warp == 8) {
     PackedSeq s{};
     int64_t tiles = 0, end = 0;
-    const bool found = packed_find(p, key_side, kTile, blockIdx.x, &s, &tiles, &end);
+    const bool found = packed_find_sorted(p, key_side, kTile, blockIdx.x / heads, &s, &tiles, &end);
     if (lane == 0) {
       sh->seq = s;
       sh->tiles = tiles;
@@ -106,15 +106,15 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
-  const int head = blockIdx.y, kv = head / (p.H / p.Hk);
-  const uint32_t tmem = bwd_setup(sh, p, false, warp, lane);
+  const int head = blockIdx.x % p.H, kv = head / (p.H / p.Hk);
+  const uint32_t tmem = bwd_setup(sh, p, false, p.H, warp, lane);
   if (!sh->found) {
-    packed_zero_rows<T>(p.dq, nullptr, sh->end, p.total_q, p.H, head, p.D, blockIdx.x - sh->tiles, gridDim.x - sh->tiles, blockDim.x);
+    packed_zero_rows<T>(p.dq, nullptr, sh->end, p.total_q, p.H, head, p.D, blockIdx.x / p.H - sh->tiles, gridDim.x / p.H - sh->tiles,
+                        blockDim.x);
   } else {
-    const PackedSeq s = sh->seq;
+    const PackedSeq s = {uniform(sh->seq.q0), uniform(sh->seq.lq), uniform(sh->seq.k0), uniform(sh->seq.lk), uniform(sh->seq.tile)};
     const int off = s.lk - s.lq;
-    const int tile = p.causal ? (s.lq + kTile - 1) / kTile - 1 - s.tile : s.tile;  // longest first
-    const int r0 = tile * kTile;
+    const int r0 = s.tile * kTile;
     const int keys = p.causal ? max(0, min(s.lk, min(r0 + kTile, s.lq) + off)) : s.lk;
     const int n = (keys + kTile - 1) / kTile;
 
@@ -160,7 +160,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (j > 0) ok = mbar_wait_bounded(&sh->loaded, (j - 1) & 1);
         if (!ok) return;
         tc_fence_after();
-        if (lane == 0) {
+        if (elect_one()) {
           mma_rows<DP>(tmem + kS, qd, kd + st * (TB >> 4), idesc_s);
           tc_commit(&sh->s_full);
           mma_rows<DP>(tmem + kDp, gd, vd + st * (TB >> 4), idesc_s);
@@ -175,9 +175,9 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         ok = ok && mbar_wait_bounded(&sh->ds_full, j & 1);
         if (!ok) break;
         tc_fence_after();
-        if (lane == 0) {
-          const int steps = min(kTile, (keys - j * kTile + 15) & ~15) / 16;
-          for (int i = 0; i < steps; ++i)
+        if (elect_one()) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
             tc_mma_f16_ts(tmem + kDq, tmem + kDs + i * 8, kd_mn + st * (TB >> 4) + i * (16 * 128 >> 4), idesc_o, (j > 0 || i > 0) ? 1u : 0u);
           tc_commit(&sh->a_empty[st]);
           tc_commit(&sh->ds_done);
@@ -304,14 +304,14 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
-  const int kv = blockIdx.y, group = p.H / p.Hk;
-  const uint32_t tmem = bwd_setup(sh, p, true, warp, lane);
+  const int kv = blockIdx.x % p.Hk, group = p.H / p.Hk;
+  const uint32_t tmem = bwd_setup(sh, p, true, p.Hk, warp, lane);
   if (!sh->found) {
-    const int64_t part = blockIdx.x - sh->tiles, parts = gridDim.x - sh->tiles;
+    const int64_t part = blockIdx.x / p.Hk - sh->tiles, parts = gridDim.x / p.Hk - sh->tiles;
     packed_zero_rows<T>(p.dk, nullptr, sh->end, p.total_k, p.Hk, kv, p.D, part, parts, blockDim.x);
     packed_zero_rows<T>(p.dv, nullptr, sh->end, p.total_k, p.Hk, kv, p.D, part, parts, blockDim.x);
   } else {
-    const PackedSeq s = sh->seq;
+    const PackedSeq s = {uniform(sh->seq.q0), uniform(sh->seq.lq), uniform(sh->seq.k0), uniform(sh->seq.lk), uniform(sh->seq.tile)};
     const int off = s.lk - s.lq;
     const int c0 = s.tile * kTile;
     const int q_tiles = (s.lq + kTile - 1) / kTile;
@@ -377,7 +377,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (!ok) return;
         if (left < kTile) zero_rows_from<DP>(tiles + st * TB, left);
         tc_fence_after();
-        if (lane == 0) {
+        if (elect_one()) {
           mma_rows<DP>(d, a, b + st * (TB >> 4), idesc_s);
           tc_commit(done);
         }
@@ -397,18 +397,18 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         ok = mbar_wait_bounded(&sh->p_full, i & 1);
         if (!ok) break;
         tc_fence_after();
-        if (lane == 0) accumulate(i, tmem + kDv, tmem + kS, gd_mn);
+        if (elect_one()) accumulate(i, tmem + kDv, tmem + kS, gd_mn);
         if (i + 1 < n) product(i + 1, sh->a_full, q_smem, kd, qd, tmem + kS, &sh->s_full);
         ok = ok && mbar_wait_bounded(&sh->ds_full, i & 1);
         if (!ok) break;
         tc_fence_after();
-        if (lane == 0) {
+        if (elect_one()) {
           accumulate(i, tmem + kDk, tmem + kDp, qd_mn);
           tc_commit(&sh->a_empty[i % ST]);
         }
         if (i + 1 < n) product(i + 1, sh->b_full, g_smem, vd, gd, tmem + kDp, &sh->dp_full);
       }
-      if (n > 0 && lane == 0) tc_commit(&sh->all_done);
+      if (n > 0 && elect_one()) tc_commit(&sh->all_done);
       if (!ok) {
         sh->abort_flag = 1;
         if (lane == 0) report_status(p.status, GW_ERR_TIMEOUT);
@@ -522,11 +522,11 @@ int launch_bwd(const PackedParams& p, int dtype, int dev, cudaStream_t st) {
   if (rc == GW_OK) rc = ensure_dynamic_smem(packed_dkv_kernel<T, DP>, smem, once_k, dev);
   if (rc != GW_OK) return rc;
   const int format = dtype == GW_BF16 ? 1 : 0;
-  packed_dq_kernel<T, DP><<<dim3(static_cast<unsigned>(packed_tile_bound(p.total_q, kTile, p.nseq)), p.H), kBwdThreads, smem, st>>>(
-      mq, mk, mv, mg, p, format);
+  const int64_t q_items = packed_tile_bound(p.total_q, kTile, p.nseq) * p.H, k_items = packed_tile_bound(p.total_k, kTile, p.nseq) * p.Hk;
+  if (q_items > 0x7fffffff || k_items > 0x7fffffff) return GW_ERR_UNSUPPORTED;
+  packed_dq_kernel<T, DP><<<static_cast<unsigned>(q_items), kBwdThreads, smem, st>>>(mq, mk, mv, mg, p, format);
   GW_LAUNCH_CHECK();
-  packed_dkv_kernel<T, DP><<<dim3(static_cast<unsigned>(packed_tile_bound(p.total_k, kTile, p.nseq)), p.Hk), kBwdThreads, smem, st>>>(
-      mq, mk, mv, mg, p, format);
+  packed_dkv_kernel<T, DP><<<static_cast<unsigned>(k_items), kBwdThreads, smem, st>>>(mq, mk, mv, mg, p, format);
   GW_LAUNCH_CHECK();
   return GW_OK;
 }

@@ -55,7 +55,7 @@ template <int DP>
 struct FwdShape {
   static constexpr int kIssuers = DP == 64 ? 2 : 1;
   static constexpr int kThreads = (kIssue + kIssuers) * 32;
-  static constexpr int kStages = DP == 64 ? 4 : 2;  // K and V rings
+  static constexpr int kStages = DP == 64 ? 3 : 2;  // K and V rings
   static constexpr int kTileBytes = DP / 64 * kBoxBytes;
   // tensor memory: S of both tiles, then P where it has room of its own (it takes S's place for wide heads), then O
   static constexpr uint32_t kS = 0, kP = DP == 64 ? 256 : 0, kPStride = DP == 64 ? 64 : 128, kO = DP == 64 ? 384 : 256;
@@ -213,12 +213,12 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       ok = mbar_wait_bounded(&sh->item_full[i & 1], (i >> 1) & 1);
       if (!ok) break;
       const FwdItem* item = &sh->item[i & 1];
-      const int kind = item->kind, most = item->most, lk = item->lk;
+      const int kind = uniform(item->kind), most = uniform(item->most), lk = uniform(item->lk);
       int n[kTiles], keys[kTiles];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
-        n[t] = item->n[t];
-        keys[t] = item->keys[t];
+        n[t] = uniform(item->n[t]);
+        keys[t] = uniform(item->keys[t]);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->item_empty[i & 1]);
@@ -227,11 +227,11 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       auto scores = [&](int t, int j) {  // S of key tile j; S has been read: for wide heads P, which sits on it, has been used
         const uint32_t at = ring + j, c = done[t] + j;
         if (j == 0) ok = ok && mbar_wait_bounded(&sh->q_full[t], q_use[t] & 1);
-        ok = ok && mbar_wait_bounded(&sh->k_full[at % ST], (at / ST) & 1);
+        if (DP == 64 || j == 0) ok = ok && mbar_wait_bounded(&sh->k_full[at % ST], (at / ST) & 1);
         if (DP == 64 && c > 0) ok = ok && mbar_wait_bounded(&sh->s_read[t], (c - 1) & 1);
         if (!ok) return;
         tc_fence_after();
-        if (lane == 0) {
+        if (elect_one()) {
           mma_rows<DP>(tmem + Shape::kS + t * kTile, qd + t * (TB >> 4), kd + (at % ST) * (TB >> 4), idesc_s);
           tc_commit(&sh->s_full[t]);
           if (j + 1 == n[t]) tc_commit(&sh->q_empty[t]);
@@ -251,7 +251,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (ok && lane == 0) mbar_arrive(&empty[at % ST]);
       };
       if (mine > 0) {
-        if (lane == 0) tc_commit(&sh->k_empty[ring % ST]);
+        if (elect_one()) tc_commit(&sh->k_empty[ring % ST]);
       } else if (most > 0) {
         pass_on(sh->k_full, sh->k_empty, ring);
       }
@@ -265,28 +265,34 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           if (DP == 64 && j + 1 < n[t]) scores(t, j + 1);  // P has its own place: ahead of this tile's softmax
           if (!v_here) {
             ok = ok && mbar_wait_bounded(&sh->v_full[st], ((ring + j) / ST) & 1);
+            if (DP != 64 && j + 1 < mine) ok = ok && mbar_wait_bounded(&sh->k_full[st_next], ((ring + j + 1) / ST) & 1);
             if (ok && (j + 1) * kTile > lk) zero_rows_from<DP>(v_smem + st * TB, lk - j * kTile);
             v_here = true;
           }
           ok = ok && mbar_wait_bounded(&sh->p_full[t], c & 1);
           if (!ok) break;
           tc_fence_after();
-          if (lane == 0) {
+          if (elect_one()) {
             const int steps = min(kTile, (keys[t] - j * kTile + 15) & ~15) / 16;
-            for (int k = 0; k < steps; ++k)
-              tc_mma_f16_ts(tmem + Shape::kO + t * DP, tmem + Shape::kP + t * Shape::kPStride + k * 8,
-                            vd + st * (TB >> 4) + k * (16 * 128 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+            const uint32_t oa = tmem + Shape::kO + t * DP, pa = tmem + Shape::kP + t * Shape::kPStride;
+            const uint64_t va = vd + st * (TB >> 4);
+            if (steps == 8) {
+#pragma unroll
+              for (int k = 0; k < 8; ++k) tc_mma_f16_ts(oa, pa + k * 8, va + k * (16 * 128 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+            } else {
+              for (int k = 0; k < steps; ++k) tc_mma_f16_ts(oa, pa + k * 8, va + k * (16 * 128 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+            }
             tc_commit(&sh->o_done[t]);
           }
           if (DP != 64 && j + 1 < n[t]) scores(t, j + 1);
         }
         if (j < mine) {
-          if (lane == 0 && ok) tc_commit(&sh->v_empty[st]);
+          if (ok && elect_one()) tc_commit(&sh->v_empty[st]);
         } else {
           pass_on(sh->v_full, sh->v_empty, ring + j);
         }
         if (j + 1 < mine) {
-          if (lane == 0 && ok) tc_commit(&sh->k_empty[st_next]);
+          if (ok && elect_one()) tc_commit(&sh->k_empty[st_next]);
         } else if (j + 1 < most) {
           pass_on(sh->k_full, sh->k_empty, ring + j + 1);
         }
