@@ -8,8 +8,8 @@
 // heads that read them (dk, dv).  S and dP are made in both: seven products instead of five, against 32-bit atomic traffic of
 // one query tile for every pair of tiles.
 //
-// Each 128 x 128 tile pair: S and dP from shared-memory operands into tensor memory; two groups of four warps, 64 columns each,
-// make P and dS in registers (a thread owns one row of its half) and put them back into tensor memory as 16-bit A operands of
+// Each pair of tiles: S and dP from shared-memory operands into tensor memory; groups of four warps, 64 columns each,
+// make P and dS in registers (a thread owns a row of its 64 columns) and put them back into tensor memory as 16-bit A operands of
 // the accumulating products, whose B operand is the tile that is in shared memory already, read along its rows.  The key-side
 // kernel works on the transposes (rows are keys), so neither P nor dS is ever transposed.
 #include "gw_packed_mma.cuh"
@@ -17,13 +17,20 @@
 namespace gw {
 namespace {
 
-constexpr int kBwdThreads = 320;  // warps 0-3: columns 0-63, 4-7: columns 64-127, 8: loads, 9: products
-
+// A block owns 128 rows and walks the other side in tiles of kWalk rows.  Narrow heads: 64, so that the accumulators need half of the
+// tensor memory and two blocks share an SM; one's softmax, loads and output then run under the other's products.  Wide heads:
+// 128, one block an SM.  Four warps for each 64 columns make P and dS, then one warp loads and one issues products.
 template <int DP>
 struct BwdShape {
+  static constexpr int kWalk = DP == 64 ? 64 : 128;
+  static constexpr int kHalves = kWalk / 64;
+  static constexpr int kLoad = 4 * kHalves, kIssue = kLoad + 1;
+  static constexpr int kThreads = (kIssue + 1) * 32;
+  static constexpr int kBlocks = DP == 64 ? 2 : 1;
   static constexpr int kStages = DP == 64 ? 4 : 2;
-  static constexpr int kTileBytes = DP / 64 * kBoxBytes;
-  static constexpr size_t kSmem = 1024 + static_cast<size_t>(2 + 2 * kStages) * kTileBytes + 512 + kStages * 2 * kTile * 4;
+  static constexpr int kOwnBytes = DP / 64 * kBoxBytes, kWalkBytes = kWalk * DP * 2;
+  static constexpr uint32_t kColumns = DP == 64 ? 256 : 512;
+  static constexpr size_t kSmem = 1024 + 2 * kOwnBytes + static_cast<size_t>(2 * kStages) * kWalkBytes + 512 + kStages * 2 * kWalk * 4;
 };
 
 struct BwdShared {
@@ -38,8 +45,10 @@ struct BwdShared {
 static_assert(sizeof(BwdShared) <= 512, "shared bookkeeping");
 
 // Barriers, the block's tile and tensor memory; the same in both kernels.
+template <int DP>
 __device__ __forceinline__ uint32_t bwd_setup(BwdShared* sh, const PackedParams& p, bool key_side, int heads, int warp, int lane) {
-  if (warp == 8) {
+  using Shape = BwdShape<DP>;
+  if (warp == Shape::kLoad) {
     PackedSeq s{};
     int64_t tiles = 0, end = 0;
     const bool found = packed_find_sorted(p, key_side, kTile, blockIdx.x / heads, &s, &tiles, &end);
@@ -49,7 +58,7 @@ __device__ __forceinline__ uint32_t bwd_setup(BwdShared* sh, const PackedParams&
       sh->end = end;
       sh->found = found;
       for (uint64_t* b : {&sh->own_full, &sh->s_full, &sh->dp_full, &sh->ds_done, &sh->all_done}) mbar_init(b, 1);
-      for (uint64_t* b : {&sh->loaded, &sh->p_full, &sh->ds_full}) mbar_init(b, 8);
+      for (uint64_t* b : {&sh->loaded, &sh->p_full, &sh->ds_full}) mbar_init(b, Shape::kLoad);
       for (int i = 0; i < 4; ++i) {
         mbar_init(&sh->a_full[i], 1);
         mbar_init(&sh->a_empty[i], 1);
@@ -62,7 +71,7 @@ __device__ __forceinline__ uint32_t bwd_setup(BwdShared* sh, const PackedParams&
       fence_proxy_async_smem();
     }
   }
-  if (warp == 9) tmem_alloc(&sh->tmem_base, 512);
+  if (warp == Shape::kIssue) tmem_alloc(&sh->tmem_base, Shape::kColumns);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -92,22 +101,23 @@ __device__ __forceinline__ void store_acc(T* dst, uint32_t addr, int from, int t
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kBlocks)
 packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                  const __grid_constant__ CUtensorMap tmG, const PackedParams p, const int ab_format) {
-  constexpr int ST = BwdShape<DP>::kStages, TB = BwdShape<DP>::kTileBytes;
-  constexpr uint32_t kS = 0, kDp = 128, kDs = 256, kDq = 384;
+  using Shape = BwdShape<DP>;
+  constexpr int ST = Shape::kStages, TB = Shape::kOwnBytes, W = Shape::kWalk, WB = Shape::kWalkBytes;
+  constexpr uint32_t kS = 0, kDp = W, kDs = 2 * W, kDq = Shape::kColumns - DP;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* q_smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char* g_smem = q_smem + TB;
   unsigned char* k_smem = g_smem + TB;
-  unsigned char* v_smem = k_smem + ST * TB;
-  BwdShared* sh = reinterpret_cast<BwdShared*>(v_smem + ST * TB);
+  unsigned char* v_smem = k_smem + ST * WB;
+  BwdShared* sh = reinterpret_cast<BwdShared*>(v_smem + ST * WB);
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const int head = blockIdx.x % p.H, kv = head / (p.H / p.Hk);
-  const uint32_t tmem = bwd_setup(sh, p, false, p.H, warp, lane);
+  const uint32_t tmem = bwd_setup<DP>(sh, p, false, p.H, warp, lane);
   if (!sh->found) {
     packed_zero_rows<T>(p.dq, nullptr, sh->end, p.total_q, p.H, head, p.D, blockIdx.x / p.H - sh->tiles, gridDim.x / p.H - sh->tiles,
                         blockDim.x);
@@ -116,9 +126,9 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int off = s.lk - s.lq;
     const int r0 = s.tile * kTile;
     const int keys = p.causal ? max(0, min(s.lk, min(r0 + kTile, s.lq) + off)) : s.lk;
-    const int n = (keys + kTile - 1) / kTile;
+    const int n = (keys + W - 1) / W;
 
-    if (warp == 8) {
+    if (warp == Shape::kLoad) {
       if (lane == 0 && n > 0) {
         bool ok = true;
         int j = 0;
@@ -130,10 +140,10 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           const uint32_t par = ((j / ST) & 1u) ^ 1u;
           ok = mbar_wait_bounded(&sh->a_empty[st], par) && mbar_wait_bounded(&sh->b_empty[st], par);
           if (!ok || sh->abort_flag) break;
-          mbar_arrive_expect_tx(&sh->a_full[st], TB);
-          load_rows<DP>(k_smem + st * TB, &tmK, kv, s.k0 + j * kTile, &sh->a_full[st]);
-          mbar_arrive_expect_tx(&sh->b_full[st], TB);
-          load_rows<DP>(v_smem + st * TB, &tmV, kv, s.k0 + j * kTile, &sh->b_full[st]);
+          mbar_arrive_expect_tx(&sh->a_full[st], WB);
+          load_rows<DP, W>(k_smem + st * WB, &tmK, kv, s.k0 + j * W, &sh->a_full[st]);
+          mbar_arrive_expect_tx(&sh->b_full[st], WB);
+          load_rows<DP, W>(v_smem + st * WB, &tmV, kv, s.k0 + j * W, &sh->b_full[st]);
         }
         if (!ok) sh->abort_flag = 1;
         if (sh->abort_flag) {  // let the copies in flight land before the shared memory is given up
@@ -145,8 +155,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           report_status(p.status, GW_ERR_TIMEOUT);
         }
       }
-    } else if (warp == 9) {
-      const uint32_t idesc_s = make_idesc_mn(ab_format, kTile, kTile);
+    } else if (warp == Shape::kIssue) {
+      const uint32_t idesc_s = make_idesc_mn(ab_format, kTile, W);
       const uint32_t idesc_o = make_idesc_mn(ab_format, kTile, DP) | kBMajorMN;
       const uint64_t qd = make_smem_desc(smem_u32(q_smem)), gd = make_smem_desc(smem_u32(g_smem));
       const uint64_t kd = make_smem_desc(smem_u32(k_smem)), vd = make_smem_desc(smem_u32(v_smem));
@@ -156,14 +166,14 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const int st = j % ST;
         ok = mbar_wait_bounded(&sh->a_full[st], (j / ST) & 1) && mbar_wait_bounded(&sh->b_full[st], (j / ST) & 1);
         if (!ok) return;
-        if ((j + 1) * kTile > s.lk) zero_rows_from<DP>(k_smem + st * TB, s.lk - j * kTile);  // K is also dq's operand
+        if ((j + 1) * W > s.lk) zero_rows_from<DP, W>(k_smem + st * WB, s.lk - j * W);  // K is also dq's operand
         if (j > 0) ok = mbar_wait_bounded(&sh->loaded, (j - 1) & 1);
         if (!ok) return;
         tc_fence_after();
         if (elect_one()) {
-          mma_rows<DP>(tmem + kS, qd, kd + st * (TB >> 4), idesc_s);
+          mma_rows<DP>(tmem + kS, qd, kd + st * (WB >> 4), idesc_s);
           tc_commit(&sh->s_full);
-          mma_rows<DP>(tmem + kDp, gd, vd + st * (TB >> 4), idesc_s);
+          mma_rows<DP>(tmem + kDp, gd, vd + st * (WB >> 4), idesc_s);
           tc_commit(&sh->dp_full);
           tc_commit(&sh->b_empty[st]);
         }
@@ -177,8 +187,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            tc_mma_f16_ts(tmem + kDq, tmem + kDs + i * 8, kd_mn + st * (TB >> 4) + i * (16 * 128 >> 4), idesc_o, (j > 0 || i > 0) ? 1u : 0u);
+          for (int i = 0; i < W / 16; ++i)
+            tc_mma_f16_ts(tmem + kDq, tmem + kDs + i * 8, kd_mn + st * (WB >> 4) + i * (16 * 128 >> 4), idesc_o, (j > 0 || i > 0) ? 1u : 0u);
           tc_commit(&sh->a_empty[st]);
           tc_commit(&sh->ds_done);
         }
@@ -249,8 +259,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           const uint64_t d = mul_f2(pack_f2(x[2 * i], x[2 * i + 1]), add_f2(pack_f2(y[2 * i], y[2 * i + 1]), nd2));
           unpack_f2(d, x[2 * i], x[2 * i + 1]);
         }
-        if ((j + 1) * kTile > open) {
-          const int valid = limit - j * kTile;
+        if ((j + 1) * W > open) {
+          const int valid = limit - j * W;
 #pragma unroll
           for (int i = 0; i < 64; ++i) x[i] = i < valid ? x[i] : 0.f;
         }
@@ -274,22 +284,23 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         report_status(p.status, GW_ERR_TIMEOUT);
       }
       tc_fence_after();
-      store_acc<T>(static_cast<T*>(p.dq) + (token * p.H + head) * p.D, tmem + lanes + kDq, half * (DP / 2), (half + 1) * (DP / 2), p.D, p.scale,
+      store_acc<T>(static_cast<T*>(p.dq) + (token * p.H + head) * p.D, tmem + lanes + kDq, half * (DP / Shape::kHalves), (half + 1) * (DP / Shape::kHalves), p.D, p.scale,
                    live, n > 0);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == Shape::kIssue) tmem_dealloc(tmem, Shape::kColumns);
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kBlocks)
 packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const __grid_constant__ CUtensorMap tmG, const PackedParams p, const int ab_format) {
-  constexpr int ST = BwdShape<DP>::kStages, TB = BwdShape<DP>::kTileBytes;
-  constexpr uint32_t kS = 0, kDp = 128, kDv = 256, kDk = 256 + DP;
+  using Shape = BwdShape<DP>;
+  constexpr int ST = Shape::kStages, TB = Shape::kOwnBytes, W = Shape::kWalk, WB = Shape::kWalkBytes;
+  constexpr uint32_t kS = 0, kDp = W, kDv = 2 * W, kDk = 2 * W + DP;
   // fp16 holds nothing below 2^-24 and few bits below 2^-14, and a P of a long sequence is that small: it is raised by 2^12 (P <= 1)
   // and dv lowered again; bf16 has fp32's range
   constexpr float kLift = sizeof(T) == 2 && std::is_same<T, __half>::value ? 12.f : 0.f;
@@ -298,14 +309,14 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   unsigned char* k_smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char* v_smem = k_smem + TB;
   unsigned char* q_smem = v_smem + TB;
-  unsigned char* g_smem = q_smem + ST * TB;
-  float* stats = reinterpret_cast<float*>(g_smem + ST * TB);  // [stage][-lse log2 e + lift, -D][128]
-  BwdShared* sh = reinterpret_cast<BwdShared*>(stats + ST * 2 * kTile);
+  unsigned char* g_smem = q_smem + ST * WB;
+  float* stats = reinterpret_cast<float*>(g_smem + ST * WB);  // [stage][-lse log2 e + lift, -D][W]
+  BwdShared* sh = reinterpret_cast<BwdShared*>(stats + ST * 2 * W);
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const int kv = blockIdx.x % p.Hk, group = p.H / p.Hk;
-  const uint32_t tmem = bwd_setup(sh, p, true, p.Hk, warp, lane);
+  const uint32_t tmem = bwd_setup<DP>(sh, p, true, p.Hk, warp, lane);
   if (!sh->found) {
     const int64_t part = blockIdx.x / p.Hk - sh->tiles, parts = gridDim.x / p.Hk - sh->tiles;
     packed_zero_rows<T>(p.dk, nullptr, sh->end, p.total_k, p.Hk, kv, p.D, part, parts, blockDim.x);
@@ -314,12 +325,12 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const PackedSeq s = {uniform(sh->seq.q0), uniform(sh->seq.lq), uniform(sh->seq.k0), uniform(sh->seq.lk), uniform(sh->seq.tile)};
     const int off = s.lk - s.lq;
     const int c0 = s.tile * kTile;
-    const int q_tiles = (s.lq + kTile - 1) / kTile;
-    const int first = p.causal ? max(0, c0 - off) / kTile : 0;  // the first query tile that sees one of these keys
+    const int q_tiles = (s.lq + W - 1) / W;
+    const int first = p.causal ? max(0, c0 - off) / W : 0;  // the first query tile that sees one of these keys
     const int per_head = max(0, q_tiles - first);
     const int n = per_head * group;
 
-    if (warp == 8) {
+    if (warp == Shape::kLoad) {
       bool ok = true;
       int i = 0;
       if (lane == 0 && n > 0) {
@@ -328,19 +339,19 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         load_rows<DP>(v_smem, &tmV, kv, s.k0 + c0, &sh->own_full);
       }
       for (; i < n; ++i) {
-        const int st = i % ST, head = kv * group + i / per_head, r0 = (first + i % per_head) * kTile;
+        const int st = i % ST, head = kv * group + i / per_head, r0 = (first + i % per_head) * W;
         ok = mbar_wait_bounded(&sh->a_empty[st], ((i / ST) & 1u) ^ 1u);
         if (!ok || sh->abort_flag) break;
         if (lane == 0) {
-          mbar_arrive_expect_tx(&sh->a_full[st], TB);
-          load_rows<DP>(q_smem + st * TB, &tmQ, head, s.q0 + r0, &sh->a_full[st]);
-          mbar_arrive_expect_tx(&sh->b_full[st], TB);
-          load_rows<DP>(g_smem + st * TB, &tmG, head, s.q0 + r0, &sh->b_full[st]);
+          mbar_arrive_expect_tx(&sh->a_full[st], WB);
+          load_rows<DP, W>(q_smem + st * WB, &tmQ, head, s.q0 + r0, &sh->a_full[st]);
+          mbar_arrive_expect_tx(&sh->b_full[st], WB);
+          load_rows<DP, W>(g_smem + st * WB, &tmG, head, s.q0 + r0, &sh->b_full[st]);
         }
-        float* dst = stats + st * 2 * kTile;
+        float* dst = stats + st * 2 * W;
         const int64_t base = static_cast<int64_t>(head) * p.total_q + s.q0 + r0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < W / 32; ++k) {
           const int r = lane + 32 * k;
           float l = -INFINITY, d = 0.f;  // rows behind the end: P = 0, dS = 0
           if (r0 + r < s.lq) {
@@ -349,7 +360,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             d = -p.delta[base + r];
           }
           dst[r] = l;
-          dst[kTile + r] = d;
+          dst[W + r] = d;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->st_full[st]);
@@ -363,8 +374,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         report_status(p.status, GW_ERR_TIMEOUT);
       }
-    } else if (warp == 9) {
-      const uint32_t idesc_s = make_idesc_mn(ab_format, kTile, kTile);
+    } else if (warp == Shape::kIssue) {
+      const uint32_t idesc_s = make_idesc_mn(ab_format, kTile, W);
       const uint32_t idesc_o = make_idesc_mn(ab_format, kTile, DP) | kBMajorMN;
       const uint64_t kd = make_smem_desc(smem_u32(k_smem)), vd = make_smem_desc(smem_u32(v_smem));
       const uint64_t qd = make_smem_desc(smem_u32(q_smem)), gd = make_smem_desc(smem_u32(g_smem));
@@ -372,21 +383,21 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       bool ok = n == 0 || mbar_wait_bounded(&sh->own_full, 0);
       // S^T = K Q^T / dP^T = V d_o^T of query tile i; rows behind the sequence's end become zeros first
       auto product = [&](int i, uint64_t* full, unsigned char* tiles, uint64_t a, uint64_t b, uint32_t d, uint64_t* done) {
-        const int st = i % ST, left = s.lq - (first + i % per_head) * kTile;
+        const int st = i % ST, left = s.lq - (first + i % per_head) * W;
         ok = mbar_wait_bounded(&full[st], (i / ST) & 1);
         if (!ok) return;
-        if (left < kTile) zero_rows_from<DP>(tiles + st * TB, left);
+        if (left < W) zero_rows_from<DP, W>(tiles + st * WB, left);
         tc_fence_after();
         if (elect_one()) {
-          mma_rows<DP>(d, a, b + st * (TB >> 4), idesc_s);
+          mma_rows<DP>(d, a, b + st * (WB >> 4), idesc_s);
           tc_commit(done);
         }
       };
       // accumulator += (P or dS)^T (d_o or Q): the A operand's two halves of 64 queries are 64 columns apart
       auto accumulate = [&](int i, uint32_t acc, uint32_t a, uint64_t b) {
-        const uint64_t at = b + (i % ST) * (TB >> 4);
+        const uint64_t at = b + (i % ST) * (WB >> 4);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < W / 16; ++k)
           tc_mma_f16_ts(acc, a + (k >> 2) * 64 + (k & 3) * 8, at + k * (16 * 128 >> 4), idesc_o, (i > 0 || k > 0) ? 1u : 0u);
       };
       if (n > 0 && ok) {
@@ -423,9 +434,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const uint64_t c2 = pack_f2(c, c), lower2 = pack_f2(kLower, kLower);
       bool ok = true;
       for (int i = 0; i < n; ++i) {
-        const int st = i % ST, r0 = (first + i % per_head) * kTile;
-        const ulonglong2* l2 = reinterpret_cast<const ulonglong2*>(stats + st * 2 * kTile + half * 64);
-        const ulonglong2* d2 = reinterpret_cast<const ulonglong2*>(stats + st * 2 * kTile + kTile + half * 64);
+        const int st = i % ST, r0 = (first + i % per_head) * W;
+        const ulonglong2* l2 = reinterpret_cast<const ulonglong2*>(stats + st * 2 * W + half * 64);
+        const ulonglong2* d2 = reinterpret_cast<const ulonglong2*>(stats + st * 2 * W + W + half * 64);
         const bool edge = p.causal && c0 + kTile - 1 > r0 + off;  // some pair of the tiles is masked
         const int from = row - off - r0 - half * 64;              // the first column that sees this key
         ok = mbar_wait_bounded(&sh->st_full[st], (i / ST) & 1) && mbar_wait_bounded(&sh->s_full, i & 1);
@@ -496,26 +507,32 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       tc_fence_after();
       const int64_t at = (static_cast<int64_t>(s.k0 + row) * p.Hk + kv) * p.D;
-      if (half == 0)
-        store_acc<T>(static_cast<T*>(p.dv) + at, tmem + lanes + kDv, 0, DP, p.D, kLower, live, n > 0);
-      else
+      if (half == 0) store_acc<T>(static_cast<T*>(p.dv) + at, tmem + lanes + kDv, 0, DP, p.D, kLower, live, n > 0);
+      if (half == Shape::kHalves - 1)
         store_acc<T>(static_cast<T*>(p.dk) + at, tmem + lanes + kDk, 0, DP, p.D, p.scale, live, n > 0);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == Shape::kIssue) tmem_dealloc(tmem, Shape::kColumns);
 }
 
 template <typename T, int DP>
 int launch_bwd(const PackedParams& p, int dtype, int dev, cudaStream_t st) {
   CUtensorMap mq, mk, mv, mg;
   GW_CUDA_TRY(cudaSetDevice(dev));  // a thread that has launched nothing yet has no context to encode tensor maps in
-  int rc = make_token_map(&mq, p.q, dtype, p.total_q, p.H, p.D, p.qs[0], p.qs[1]);
-  if (rc == GW_OK) rc = make_token_map(&mk, p.k, dtype, p.total_k, p.Hk, p.D, p.ks[0], p.ks[1]);
-  if (rc == GW_OK) rc = make_token_map(&mv, p.v, dtype, p.total_k, p.Hk, p.D, p.vs[0], p.vs[1]);
-  if (rc == GW_OK) rc = make_token_map(&mg, p.d_o, dtype, p.total_q, p.H, p.D, p.dos[0], p.dos[1]);
+  // each tensor once as the side that a block owns and once as the side that it walks
+  int rc = GW_OK;
+  auto maps = [&](int q_rows, int k_rows) {
+    rc = make_token_map(&mq, p.q, dtype, p.total_q, p.H, p.D, p.qs[0], p.qs[1], q_rows);
+    if (rc == GW_OK) rc = make_token_map(&mg, p.d_o, dtype, p.total_q, p.H, p.D, p.dos[0], p.dos[1], q_rows);
+    if (rc == GW_OK) rc = make_token_map(&mk, p.k, dtype, p.total_k, p.Hk, p.D, p.ks[0], p.ks[1], k_rows);
+    if (rc == GW_OK) rc = make_token_map(&mv, p.v, dtype, p.total_k, p.Hk, p.D, p.vs[0], p.vs[1], k_rows);
+    return rc;
+  };
+  constexpr int W = BwdShape<DP>::kWalk, kThreads = BwdShape<DP>::kThreads;
+  maps(kTile, W);
   static OncePerDevice once_q, once_k;
   constexpr size_t smem = BwdShape<DP>::kSmem;
   if (rc == GW_OK) rc = ensure_dynamic_smem(packed_dq_kernel<T, DP>, smem, once_q, dev);
@@ -524,9 +541,10 @@ int launch_bwd(const PackedParams& p, int dtype, int dev, cudaStream_t st) {
   const int format = dtype == GW_BF16 ? 1 : 0;
   const int64_t q_items = packed_tile_bound(p.total_q, kTile, p.nseq) * p.H, k_items = packed_tile_bound(p.total_k, kTile, p.nseq) * p.Hk;
   if (q_items > 0x7fffffff || k_items > 0x7fffffff) return GW_ERR_UNSUPPORTED;
-  packed_dq_kernel<T, DP><<<static_cast<unsigned>(q_items), kBwdThreads, smem, st>>>(mq, mk, mv, mg, p, format);
+  packed_dq_kernel<T, DP><<<static_cast<unsigned>(q_items), kThreads, smem, st>>>(mq, mk, mv, mg, p, format);
   GW_LAUNCH_CHECK();
-  packed_dkv_kernel<T, DP><<<static_cast<unsigned>(k_items), kBwdThreads, smem, st>>>(mq, mk, mv, mg, p, format);
+  if (W != kTile && maps(W, kTile) != GW_OK) return rc;
+  packed_dkv_kernel<T, DP><<<static_cast<unsigned>(k_items), kThreads, smem, st>>>(mq, mk, mv, mg, p, format);
   GW_LAUNCH_CHECK();
   return GW_OK;
 }

@@ -19,11 +19,11 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
 }
-// all DP columns of 128 rows of one head, as DP / 64 boxes one behind the other
-template <int DP>
+// all DP columns of ROWS rows of one head, as DP / 64 boxes one behind the other
+template <int DP, int ROWS = kTile>
 __device__ __forceinline__ void load_rows(unsigned char* dst, const CUtensorMap* map, int head, int row, uint64_t* bar) {
 #pragma unroll
-  for (int b = 0; b < DP / 64; ++b) tma_load_3d(dst + b * kBoxBytes, map, 64 * b, head, row, bar);
+  for (int b = 0; b < DP / 64; ++b) tma_load_3d(dst + b * ROWS * 128, map, 64 * b, head, row, bar);
 }
 
 // Operand tile read along its rows (the contraction runs over the tokens): 64 columns are one swizzle atom wide, further
@@ -135,19 +135,20 @@ __device__ __forceinline__ bool elect_one() {
 // a value read from memory that is the same in all lanes, made known as such to the compiler
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
-// Rows from `from` on of a 128-row operand tile become zero (whole warp): the rows behind a sequence's end belong to its
+// Rows from `from` on of an operand tile become zero (whole warp): the rows behind a sequence's end belong to its
 // neighbour or to nobody, and zero times whatever stands there need not be zero.
-template <int DP>
+template <int DP, int ROWS = kTile>
 __device__ __forceinline__ void zero_rows_from(unsigned char* tile, int from) {
   const int lane = threadIdx.x & 31;
   for (int b = 0; b < DP / 64; ++b)
-    for (int i = from * 8 + lane; i < kTile * 8; i += 32) *reinterpret_cast<uint4*>(tile + b * kBoxBytes + i * 16) = make_uint4(0, 0, 0, 0);
+    for (int i = from * 8 + lane; i < ROWS * 8; i += 32) *reinterpret_cast<uint4*>(tile + b * ROWS * 128 + i * 16) = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   __syncwarp();
 }
 
-// [tokens, heads, D] tensor of 16-bit elements with any 16-byte strides; a box is 64 columns of 128 tokens of one head, what lies
+// [tokens, heads, D] tensor of 16-bit elements with any 16-byte strides; a box is 64 columns of `rows` tokens of one head, what lies
 // outside the tensor reads as zero (a side without tokens is never loaded)
-int make_token_map(CUtensorMap* map, const void* base, int dtype, int64_t tokens, int heads, int D, int64_t token_stride, int64_t head_stride);
+int make_token_map(CUtensorMap* map, const void* base, int dtype, int64_t tokens, int heads, int D, int64_t token_stride, int64_t head_stride,
+                   int rows);
 
 }  // namespace gw
