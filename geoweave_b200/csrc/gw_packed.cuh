@@ -198,6 +198,6 @@ int packed_mma_bwd(const PackedParams& p, int dtype, int dev, cudaStream_t st);
 // few query rows, divided along the keys (gw_packed_split.cu)
 bool packed_split_fits(const PackedParams& p, int64_t max_q);
 size_t packed_split_bytes(const PackedParams& p, int sms);
-int packed_split_fwd(const PackedParams& p, int dtype, int64_t max_q, int sms, void* workspace, cudaStream_t st);
+int packed_split_fwd(const PackedParams& p, int dtype, int64_t max_q, int dev, int sms, void* workspace, cudaStream_t st);
 
 }  // namespace gw

@@ -67,7 +67,7 @@ extern "C" int gw_packed_attn_fwd(const void* q, const void* k, const void* v, i
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (packed_split_fits(p, max_q)) {
     if (!workspace || !aligned16(workspace) || workspace_bytes < packed_split_bytes(p, facts.sms)) return GW_ERR_WORKSPACE;
-    return packed_split_fwd(p, dtype, max_q, facts.sms, workspace, st);
+    return packed_split_fwd(p, dtype, max_q, dev, facts.sms, workspace, st);
   }
   return dtype == GW_F32 ? packed_plain_fwd(p, st) : packed_mma_fwd(p, dtype, dev, facts.sms, st);
 }

@@ -302,10 +302,11 @@ template <int DP>
 __global__ void __launch_bounds__(NT) plain_split_kernel(const PackedParams p, const int chunk, float* part_o, float* part_ml) {
   extern __shared__ float smem[];
   float *qt = smem, *kt = qt + 16 * (DP + 4), *vt = kt + BT * (DP + 4), *w = vt + BT * (DP + 4);
-  const int kv = blockIdx.y, group = p.H / p.Hk, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const int kv = blockIdx.x % p.Hk, group = p.H / p.Hk, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const int64_t slot = blockIdx.x / p.Hk;
   PackedSeq s;
   int64_t tiles, end;
-  if (!packed_find(p, true, chunk, blockIdx.x, &s, &tiles, &end)) return;
+  if (!packed_find(p, true, chunk, slot, &s, &tiles, &end)) return;
   const int rows = min(16, s.lq * group);
   if (rows == 0) return;
   const int from = s.tile * chunk, to = min(s.lk, from + chunk);
@@ -349,7 +350,7 @@ __global__ void __launch_bounds__(NT) plain_split_kernel(const PackedParams p, c
     accumulate<DP, 1>(acc, w, vt, ty, tx);
   }
   if (ty >= rows) return;
-  const int64_t at = (static_cast<int64_t>(blockIdx.x) * p.Hk + kv) * 16 + ty;
+  const int64_t at = (slot * p.Hk + kv) * 16 + ty;
 #pragma unroll
   for (int c = 0; c < DP / 16; ++c) {
     const int col = tx * 4 + 16 * (c & ~3) + (c & 3);
@@ -399,7 +400,7 @@ int launch_split(const PackedParams& p, int chunk, int64_t slots, float* part_o,
   static OncePerDevice once;
   const int rc = ensure_dynamic_smem(plain_split_kernel<DP>, tiles_bytes<DP>(3), once, dev);
   if (rc != GW_OK) return rc;
-  plain_split_kernel<DP><<<dim3(static_cast<unsigned>(slots), p.Hk), NT, tiles_bytes<DP>(3), st>>>(p, chunk, part_o, part_ml);
+  plain_split_kernel<DP><<<static_cast<unsigned>(slots * p.Hk), NT, tiles_bytes<DP>(3), st>>>(p, chunk, part_o, part_ml);
   GW_LAUNCH_CHECK();
   return GW_OK;
 }

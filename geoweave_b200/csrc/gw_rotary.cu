@@ -10,7 +10,11 @@
 //
 // Bound by memory: q and k are read once and written once.  A thread owns one piece of the columns (V pairs, or V copied
 // columns) of one token and walks the heads, so cosines and sines are loaded once for all heads; V is the widest piece of at
-// most 16 bytes that the widths, strides and pointers allow.
+// most 16 bytes that the widths, strides and pointers allow.  Blocks stay and take tokens gridDim apart: 33 312 tokens of 16 + 16
+// heads of 64 in bf16, sliced from a projection's output, 58 us = 4.7 TB/s (64 us with a block for every four tokens; a copy of as
+// many contiguous bytes takes 45 us); fp32 5.4 TB/s.  Looked at and dropped: whole 16-byte pieces a lane with the partners
+// found through shared memory (104 us: the registers for two angles a column halve the occupancy), loads ahead of the position (96 us,
+// the same), other block sizes.  Without the position and angle loads it takes 56 us, so they are not the bound.
 #include "gw_common.cuh"
 
 namespace gw {
@@ -18,6 +22,7 @@ namespace {
 
 constexpr int kAxes = 4;
 constexpr int kThreads = 256;
+constexpr int kBlocksPerSm = 6;
 
 struct RotaryParams {
   const void *q, *k;
@@ -42,84 +47,85 @@ struct alignas(sizeof(T) * V) Piece {
 };
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) rotary_axes_kernel(const RotaryParams p) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) rotary_axes_kernel(const RotaryParams p) {
   const int pairs = p.turned / 2 / V, units = pairs + (p.D - p.turned + V - 1) / V;
   const int per_token = units * p.head_lanes;
   const int slot = threadIdx.x / per_token;
   if (slot >= p.tokens_per_block) return;
-  const int64_t t = static_cast<int64_t>(blockIdx.x) * p.tokens_per_block + slot;
-  if (t >= p.tokens) return;
   const int unit = (threadIdx.x % per_token) % units, lane = (threadIdx.x % per_token) / units;
-  const int64_t b = t / p.per_batch, n = t % p.per_batch;
-  const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + n * p.qs[1];
-  const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + n * p.ks[1];
-  T* qo = static_cast<T*>(p.q_out) + t * p.H * p.D;
-  T* ko = static_cast<T*>(p.k_out) + t * p.Hk * p.D;
   using P = Piece<T, V>;
+  const bool turns = unit < pairs;
+  int a = 0, before = 0;  // the axis of this piece, and the angles of the axes in front of it
+  while (turns && unit * V >= before + p.half[a]) before += p.half[a++];
+  // the pair's two pieces; a piece behind the axes is copied
+  const int lo = turns ? unit * V + before : p.turned + (unit - pairs) * V, hi = turns ? lo + p.half[a] : lo;
 
-  if (unit >= pairs) {  // a piece behind the axes
-    const int c = p.turned + (unit - pairs) * V;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * p.tokens_per_block;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * p.tokens_per_block + slot; t < p.tokens; t += stride) {
+    const int64_t b = t / p.per_batch, n = t % p.per_batch;
+    const T* q = static_cast<const T*>(p.q) + b * p.qs[0] + n * p.qs[1];
+    const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + n * p.ks[1];
+    T* qo = static_cast<T*>(p.q_out) + t * p.H * p.D;
+    T* ko = static_cast<T*>(p.k_out) + t * p.Hk * p.D;
+    if (!turns) {
+#pragma unroll 4
+      for (int h = lane; h < p.H + p.Hk; h += p.head_lanes) {
+        const bool is_q = h < p.H;
+        const T* src = is_q ? q + h * p.qs[2] : k + (h - p.H) * p.ks[2];
+        T* dst = is_q ? qo + h * p.D : ko + (h - p.H) * p.D;
+        *reinterpret_cast<P*>(dst + lo) = *reinterpret_cast<const P*>(src + lo);
+      }
+      continue;
+    }
+    const int64_t at = t * p.axes + a;
+    int64_t pos = p.pos64 ? static_cast<const int64_t*>(p.pos)[at] : static_cast<const int32_t*>(p.pos)[at];
+    if (pos < 0 || pos >= p.table_rows) {  // outside the tables: say so and carry on
+      report_status(p.status, GW_ERR_INVALID_ARG);
+      pos = 0;
+    }
+    const Piece<float, V> c = *reinterpret_cast<const Piece<float, V>*>(p.cos_tab + pos * (p.turned / 2) + unit * V);
+    Piece<float, V> s = *reinterpret_cast<const Piece<float, V>*>(p.sin_tab + pos * (p.turned / 2) + unit * V);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s.e[i] *= p.sign;
 #pragma unroll 4
     for (int h = lane; h < p.H + p.Hk; h += p.head_lanes) {
       const bool is_q = h < p.H;
       const T* src = is_q ? q + h * p.qs[2] : k + (h - p.H) * p.ks[2];
       T* dst = is_q ? qo + h * p.D : ko + (h - p.H) * p.D;
-      *reinterpret_cast<P*>(dst + c) = *reinterpret_cast<const P*>(src + c);
-    }
-    return;
-  }
-
-  int a = 0, before = 0;  // the axis of this piece, and the angles of the axes in front of it
-  while (unit * V >= before + p.half[a]) before += p.half[a++];
-  const int lo = unit * V + before, hi = lo + p.half[a];
-  const int64_t at = t * p.axes + a;
-  int64_t pos = p.pos64 ? static_cast<const int64_t*>(p.pos)[at] : static_cast<const int32_t*>(p.pos)[at];
-  if (pos < 0 || pos >= p.table_rows) {  // outside the tables: say so and carry on
-    report_status(p.status, GW_ERR_INVALID_ARG);
-    pos = 0;
-  }
-  const Piece<float, V> c = *reinterpret_cast<const Piece<float, V>*>(p.cos_tab + pos * (p.turned / 2) + unit * V);
-  Piece<float, V> s = *reinterpret_cast<const Piece<float, V>*>(p.sin_tab + pos * (p.turned / 2) + unit * V);
+      P x = *reinterpret_cast<const P*>(src + lo), y = *reinterpret_cast<const P*>(src + hi);
 #pragma unroll
-  for (int i = 0; i < V; ++i) s.e[i] *= p.sign;
-#pragma unroll 4
-  for (int h = lane; h < p.H + p.Hk; h += p.head_lanes) {
-    const bool is_q = h < p.H;
-    const T* src = is_q ? q + h * p.qs[2] : k + (h - p.H) * p.ks[2];
-    T* dst = is_q ? qo + h * p.D : ko + (h - p.H) * p.D;
-    P x = *reinterpret_cast<const P*>(src + lo), y = *reinterpret_cast<const P*>(src + hi);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float u = to_float(x.e[i]), w = to_float(y.e[i]);
-      x.e[i] = from_float<T>(fmaf(u, c.e[i], -w * s.e[i]));
-      y.e[i] = from_float<T>(fmaf(w, c.e[i], u * s.e[i]));
+      for (int i = 0; i < V; ++i) {
+        const float u = to_float(x.e[i]), w = to_float(y.e[i]);
+        x.e[i] = from_float<T>(fmaf(u, c.e[i], -w * s.e[i]));
+        y.e[i] = from_float<T>(fmaf(w, c.e[i], u * s.e[i]));
+      }
+      *reinterpret_cast<P*>(dst + lo) = x;
+      *reinterpret_cast<P*>(dst + hi) = y;
     }
-    *reinterpret_cast<P*>(dst + lo) = x;
-    *reinterpret_cast<P*>(dst + hi) = y;
   }
 }
 
 template <typename T, int V>
-int launch(RotaryParams p, cudaStream_t st) {
+int launch(RotaryParams p, int sms, cudaStream_t st) {
   const int units = p.turned / 2 / V + (p.D - p.turned + V - 1) / V;
   const int heads = p.H + p.Hk;
   p.head_lanes = (heads + 3) / 4;  // four heads a thread keep eight loads in flight
   if (p.head_lanes * units > kThreads) p.head_lanes = kThreads / units;
   p.tokens_per_block = kThreads / (units * p.head_lanes);
-  const int64_t grid = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block;
-  if (grid > 0x7fffffff) return GW_ERR_UNSUPPORTED;
+  const int64_t need = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block, most = static_cast<int64_t>(sms) * kBlocksPerSm;
+  const int64_t grid = need < most ? need : most;
   rotary_axes_kernel<T, V><<<static_cast<unsigned>(grid), kThreads, 0, st>>>(p);
   GW_LAUNCH_CHECK();
   return GW_OK;
 }
 
 template <typename T>
-int dispatch(const RotaryParams& p, int v, cudaStream_t st) {
+int dispatch(const RotaryParams& p, int v, int sms, cudaStream_t st) {
   if constexpr (sizeof(T) == 2)
-    if (v == 8) return launch<T, 8>(p, st);
-  if (v >= 4) return launch<T, 4>(p, st);
-  if (v == 2) return launch<T, 2>(p, st);
-  return launch<T, 1>(p, st);
+    if (v == 8) return launch<T, 8>(p, sms, st);
+  if (v >= 4) return launch<T, 4>(p, sms, st);
+  if (v == 2) return launch<T, 2>(p, sms, st);
+  return launch<T, 1>(p, sms, st);
 }
 
 }  // namespace
@@ -175,7 +181,7 @@ extern "C" int gw_rotary_axes(const void* q, const void* k, int dtype, int B, in
   if (rc != GW_OK) return rc;
   if (facts.cc_major != 10) return GW_ERR_NO_SM100;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == GW_F32) return dispatch<float>(p, v, st);
-  if (dtype == GW_BF16) return dispatch<__nv_bfloat16>(p, v, st);
-  return dispatch<__half>(p, v, st);
+  if (dtype == GW_F32) return dispatch<float>(p, v, facts.sms, st);
+  if (dtype == GW_BF16) return dispatch<__nv_bfloat16>(p, v, facts.sms, st);
+  return dispatch<__half>(p, v, facts.sms, st);
 }
