@@ -186,6 +186,10 @@ __device__ __forceinline__ void packed_zero_rows(void* out, float* lse, int64_t 
       lse[static_cast<int64_t>(head) * to + i] = -INFINITY;
 }
 
+// Programmatic launch: the kernel behind this one in the stream may start early / everything in front of this kernel is complete.
+__device__ __forceinline__ void let_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 inline int64_t packed_tile_bound(int64_t total, int tile_rows, int nseq) { return total / tile_rows + nseq + 1; }
 
 // fp32 tensors (gw_packed_plain.cu)

@@ -7,7 +7,7 @@
 // would round.  A block of 256 threads owns 64 rows and walks the other side in tiles of 64; a thread holds a 4 x 4 piece of
 // each 64 x 64 product and 4 rows x DP/16 columns of each accumulator.  The backward pass is two kernels (one owns query rows
 // and makes dq and D, one owns key rows and makes dk and dv), so no sum needs atomics and results do not depend on timing.
-#include "gw_packed.cuh"
+#include "gw_packed_mma.cuh"
 
 namespace gw {
 namespace {
@@ -16,45 +16,59 @@ constexpr int BT = 64;        // rows and columns of a tile
 constexpr int NT = 256;       // threads: 16 x 16
 constexpr int WP = BT + 4;    // padded row of a 64 x 64 tile in shared memory
 
-// [64 rows][DP + 4] fp32 tile of rows row0.. (rows at or beyond `rows`, columns beyond D: zero)
+// [64 rows][DP + 4] fp32 tile of rows row0.. (rows at or beyond `rows`, columns beyond D: zero), by asynchronous 16-byte copies:
+// complete behind tiles_here() and a barrier
 template <int DP>
 __device__ __forceinline__ void load_tile(float* dst, const void* base, int64_t token0, int rows, int64_t ts, int64_t hs, int head, int D) {
   const float* src = static_cast<const float*>(base) + head * hs + token0 * ts;
-  for (int i = threadIdx.x; i < BT * DP; i += NT) {
-    const int r = i / DP, c = i % DP;
-    dst[r * (DP + 4) + c] = (r < rows && c < D) ? src[r * ts + c] : 0.f;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < BT * DP / 4; i += NT) {
+    const int r = i / (DP / 4), c = i % (DP / 4) * 4;
+    const bool there = r < rows && c < D;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * (DP + 4) + c)), "l"(there ? src + r * ts + c : src),
+                 "r"(there ? 16 : 0)
+                 : "memory");
   }
 }
+__device__ __forceinline__ void tiles_here() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// acc[i][j] = <a row ty*R+i, b row tx+16*j>
+// acc[i][j] = <a row ty*R+i, b row tx+16*j>: two partial sums each, over the even and the odd columns, so that one packed
+// instruction makes both
 template <int DP, int R>
 __device__ __forceinline__ void dot_tile(float (&acc)[R][4], const float* a, const float* b, int ty, int tx) {
+  uint64_t sum[R][4];
 #pragma unroll
   for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) sum[i][j] = 0;
 #pragma unroll 4
   for (int d = 0; d < DP; d += 4) {
-    float4 av[R], bv[4];
+    ulonglong2 av[R], bv[4];
 #pragma unroll
-    for (int i = 0; i < R; ++i) av[i] = *reinterpret_cast<const float4*>(a + (ty * R + i) * (DP + 4) + d);
+    for (int i = 0; i < R; ++i) av[i] = *reinterpret_cast<const ulonglong2*>(a + (ty * R + i) * (DP + 4) + d);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) bv[j] = *reinterpret_cast<const float4*>(b + (tx + 16 * j) * (DP + 4) + d);
+    for (int j = 0; j < 4; ++j) bv[j] = *reinterpret_cast<const ulonglong2*>(b + (tx + 16 * j) * (DP + 4) + d);
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        acc[i][j] = fmaf(av[i].x, bv[j].x, acc[i][j]);
-        acc[i][j] = fmaf(av[i].y, bv[j].y, acc[i][j]);
-        acc[i][j] = fmaf(av[i].z, bv[j].z, acc[i][j]);
-        acc[i][j] = fmaf(av[i].w, bv[j].w, acc[i][j]);
+        sum[i][j] = fma_f2(av[i].x, bv[j].x, sum[i][j]);
+        sum[i][j] = fma_f2(av[i].y, bv[j].y, sum[i][j]);
       }
   }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float even, odd;
+      unpack_f2(sum[i][j], even, odd);
+      acc[i][j] = even + odd;
+    }
 }
 
-// acc[i][c] += sum_k w[ty*R+i][k] * m[k][column c of this thread]; columns tx*4 + 64*(c/4) + c%4
+// acc[i][c] += sum_k w[ty*R+i][k] * m[k][column c of this thread]; columns tx*4 + 64*(c/4) + c%4, two to a packed value
 template <int DP, int R>
-__device__ __forceinline__ void accumulate(float (&acc)[R][DP / 16], const float* w, const float* m, int ty, int tx) {
+__device__ __forceinline__ void accumulate(uint64_t (&acc)[R][DP / 32], const float* w, const float* m, int ty, int tx) {
 #pragma unroll 4
   for (int k = 0; k < BT; k += 4) {
     float4 wv[R];
@@ -63,22 +77,20 @@ __device__ __forceinline__ void accumulate(float (&acc)[R][DP / 16], const float
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-      for (int c = 0; c < DP / 16; c += 4) {
-        const float4 mv = *reinterpret_cast<const float4*>(m + (k + kk) * (DP + 4) + tx * 4 + 16 * c);
+      for (int c = 0; c < DP / 32; c += 2) {
+        const ulonglong2 mv = *reinterpret_cast<const ulonglong2*>(m + (k + kk) * (DP + 4) + tx * 4 + 32 * c);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
           const float x = kk == 0 ? wv[i].x : kk == 1 ? wv[i].y : kk == 2 ? wv[i].z : wv[i].w;
-          acc[i][c] = fmaf(x, mv.x, acc[i][c]);
-          acc[i][c + 1] = fmaf(x, mv.y, acc[i][c + 1]);
-          acc[i][c + 2] = fmaf(x, mv.z, acc[i][c + 2]);
-          acc[i][c + 3] = fmaf(x, mv.w, acc[i][c + 3]);
+          acc[i][c] = fma_f2(pack_f2(x, x), mv.x, acc[i][c]);
+          acc[i][c + 1] = fma_f2(pack_f2(x, x), mv.y, acc[i][c + 1]);
         }
       }
   }
 }
 
 template <int DP>
-__device__ __forceinline__ void store_rows(void* out, const float (&acc)[4][DP / 16], const float (&mul)[4], int64_t token0, int rows, int heads,
+__device__ __forceinline__ void store_rows(void* out, const uint64_t (&acc)[4][DP / 32], const float (&mul)[4], int64_t token0, int rows, int heads,
                                            int head, int D, int ty, int tx) {
   float* dst = static_cast<float*>(out);
 #pragma unroll
@@ -86,9 +98,14 @@ __device__ __forceinline__ void store_rows(void* out, const float (&acc)[4][DP /
     const int r = ty * 4 + i;
     if (r >= rows) continue;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
-      const int col = tx * 4 + 16 * (c & ~3) + (c & 3);
-      if (col < D) dst[((token0 + r) * heads + head) * D + col] = mul[i] == 0.f ? 0.f : acc[i][c] * mul[i];
+    for (int c = 0; c < DP / 32; c += 2) {
+      float v[4];
+      unpack_f2(acc[i][c], v[0], v[1]);
+      unpack_f2(acc[i][c + 1], v[2], v[3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = mul[i] == 0.f ? 0.f : v[e] * mul[i];
+      const int col = tx * 4 + 32 * c;
+      if (col < D) *reinterpret_cast<float4*>(dst + ((token0 + r) * heads + head) * D + col) = make_float4(v[0], v[1], v[2], v[3]);
     }
   }
 }
@@ -118,30 +135,31 @@ __device__ __forceinline__ bool block_tile(const PackedParams& p, bool key_side,
 template <int DP>
 __global__ void __launch_bounds__(NT) plain_fwd_kernel(const PackedParams p) {
   extern __shared__ float smem[];
-  float *qt = smem, *kt = qt + BT * (DP + 4), *w = kt + BT * (DP + 4);
+  float *qt = smem, *kt = qt + BT * (DP + 4), *vt = kt + BT * (DP + 4), *w = vt + BT * (DP + 4);
   const int head = blockIdx.y, kv = head / (p.H / p.Hk), ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   PackedSeq s;
   if (!block_tile(p, false, head, &s, p.o, nullptr, p.lse)) return;
   const int r0 = s.tile * BT, rows = min(BT, s.lq - r0), off = s.lk - s.lq;
   const int keys = p.causal ? max(0, min(s.lk, r0 + rows + off)) : s.lk;  // keys that the tile's last row sees
   load_tile<DP>(qt, p.q, s.q0 + r0, rows, p.qs[0], p.qs[1], head, p.D);
-  float m[4], l[4], acc[4][DP / 16];
+  float m[4], l[4];
+  uint64_t acc[4][DP / 32];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
+    for (int c = 0; c < DP / 32; ++c) acc[i][c] = 0;
   }
   const float c2 = p.scale * kLog2e;
   for (int k0 = 0; k0 < keys; k0 += BT) {
     __syncthreads();
     load_tile<DP>(kt, p.k, s.k0 + k0, s.lk - k0, p.ks[0], p.ks[1], kv, p.D);
+    load_tile<DP>(vt, p.v, s.k0 + k0, s.lk - k0, p.vs[0], p.vs[1], kv, p.D);
+    tiles_here();
     __syncthreads();
     float sc[4][4];
     dot_tile<DP, 4>(sc, qt, kt, ty, tx);
-    __syncthreads();
-    load_tile<DP>(kt, p.v, s.k0 + k0, s.lk - k0, p.vs[0], p.vs[1], kv, p.D);  // v takes k's place
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = r0 + ty * 4 + i;
@@ -165,10 +183,10 @@ __global__ void __launch_bounds__(NT) plain_fwd_kernel(const PackedParams p) {
       l[i] = l[i] * shrink + reduce16_sum(sum);
       m[i] = top;
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) acc[i][c] *= shrink;
+      for (int c = 0; c < DP / 32; ++c) acc[i][c] = mul_f2(acc[i][c], pack_f2(shrink, shrink));
     }
-    __syncthreads();
-    accumulate<DP, 4>(acc, w, kt, ty, tx);
+    __syncwarp();  // a row's weights are written and read by one warp
+    accumulate<DP, 4>(acc, w, vt, ty, tx);
   }
   float mul[4];
 #pragma unroll
@@ -197,8 +215,10 @@ __global__ void __launch_bounds__(NT) plain_dq_kernel(const PackedParams p) {
   const int keys = p.causal ? max(0, min(s.lk, r0 + rows + off)) : s.lk;
   load_tile<DP>(qt, p.o, s.q0 + r0, rows, static_cast<int64_t>(p.H) * p.D, p.D, head, p.D);
   load_tile<DP>(dt, p.d_o, s.q0 + r0, rows, p.dos[0], p.dos[1], head, p.D);
+  tiles_here();
   __syncthreads();
-  float lse[4], delta[4], acc[4][DP / 16];
+  float lse[4], delta[4];
+  uint64_t acc[4][DP / 32];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = ty * 4 + i;
@@ -208,7 +228,7 @@ __global__ void __launch_bounds__(NT) plain_dq_kernel(const PackedParams p) {
     lse[i] = r < rows ? p.lse[head * p.total_q + s.q0 + r0 + r] : -INFINITY;
     if (r < rows && tx == 0) p.delta[head * p.total_q + s.q0 + r0 + r] = delta[i];
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
+    for (int c = 0; c < DP / 32; ++c) acc[i][c] = 0;
   }
   __syncthreads();
   load_tile<DP>(qt, p.q, s.q0 + r0, rows, p.qs[0], p.qs[1], head, p.D);
@@ -217,6 +237,7 @@ __global__ void __launch_bounds__(NT) plain_dq_kernel(const PackedParams p) {
     __syncthreads();
     load_tile<DP>(kt, p.k, s.k0 + k0, s.lk - k0, p.ks[0], p.ks[1], kv, p.D);
     load_tile<DP>(vt, p.v, s.k0 + k0, s.lk - k0, p.vs[0], p.vs[1], kv, p.D);
+    tiles_here();
     __syncthreads();
     float sc[4][4], dp[4][4];
     dot_tile<DP, 4>(sc, qt, kt, ty, tx);
@@ -229,7 +250,7 @@ __global__ void __launch_bounds__(NT) plain_dq_kernel(const PackedParams p) {
       for (int j = 0; j < 4; ++j)
         w[(ty * 4 + i) * WP + tx + 16 * j] = (tx + 16 * j < limit) ? prob(sc[i][j], c2, lse[i]) * (dp[i][j] - delta[i]) : 0.f;
     }
-    __syncthreads();
+    __syncwarp();
     accumulate<DP, 4>(acc, w, kt, ty, tx);
   }
   const float mul[4] = {p.scale, p.scale, p.scale, p.scale};
@@ -248,11 +269,11 @@ __global__ void __launch_bounds__(NT) plain_dkv_kernel(const PackedParams p) {
   const int first = p.causal ? max(0, c0 - off) / BT * BT : 0;  // the first query tile that sees one of these keys
   load_tile<DP>(kt, p.k, s.k0 + c0, rows, p.ks[0], p.ks[1], kv, p.D);
   load_tile<DP>(vt, p.v, s.k0 + c0, rows, p.vs[0], p.vs[1], kv, p.D);
-  float ak[4][DP / 16], av[4][DP / 16];
+  uint64_t ak[4][DP / 32], av[4][DP / 32];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) ak[i][c] = av[i][c] = 0.f;
+    for (int c = 0; c < DP / 32; ++c) ak[i][c] = av[i][c] = 0;
   const float c2 = p.scale * kLog2e;
   for (int head = kv * group; head < (kv + 1) * group; ++head)
     for (int r0 = first; r0 < s.lq; r0 += BT) {
@@ -265,6 +286,7 @@ __global__ void __launch_bounds__(NT) plain_dkv_kernel(const PackedParams p) {
         const int64_t at = head * p.total_q + s.q0 + r0 + r;
         st[threadIdx.x] = threadIdx.x < BT ? (live ? p.lse[at] : -INFINITY) : (live ? p.delta[at] : 0.f);
       }
+      tiles_here();
       __syncthreads();
       float sc[4][4], dp[4][4];
       dot_tile<DP, 4>(sc, kt, qt, ty, tx);
@@ -281,14 +303,14 @@ __global__ void __launch_bounds__(NT) plain_dkv_kernel(const PackedParams p) {
           w[(ty * 4 + i) * WP + r] = sc[i][j];
         }
       }
-      __syncthreads();
+      __syncwarp();  // a row's weights are written and read by one warp
       accumulate<DP, 4>(av, w, dt, ty, tx);
-      __syncthreads();
+      __syncwarp();
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[(ty * 4 + i) * WP + tx + 16 * j] = dp[i][j];
-      __syncthreads();
+      __syncwarp();
       accumulate<DP, 4>(ak, w, qt, ty, tx);
     }
   const float mul[4] = {p.scale, p.scale, p.scale, p.scale}, one[4] = {1.f, 1.f, 1.f, 1.f};
@@ -315,15 +337,18 @@ __global__ void __launch_bounds__(NT) plain_split_kernel(const PackedParams p, c
     qt[r * (DP + 4) + c] =
         r < rows && c < p.D ? static_cast<const float*>(p.q)[(s.q0 + r / group) * p.qs[0] + (kv * group + r % group) * p.qs[1] + c] : 0.f;
   }
+  let_dependents_launch();
   const int limit = ty < rows ? (p.causal ? min(to, ty / group + s.lk - s.lq + 1) : to) : 0;  // keys this row sees
   const float c2 = p.scale * kLog2e;
-  float m = -INFINITY, l = 0.f, acc[1][DP / 16];
+  float m = -INFINITY, l = 0.f;
+  uint64_t acc[1][DP / 32];
 #pragma unroll
-  for (int c = 0; c < DP / 16; ++c) acc[0][c] = 0.f;
+  for (int c = 0; c < DP / 32; ++c) acc[0][c] = 0;
   for (int k0 = from; k0 < to; k0 += BT) {
     __syncthreads();
     load_tile<DP>(kt, p.k, s.k0 + k0, to - k0, p.ks[0], p.ks[1], kv, p.D);
     load_tile<DP>(vt, p.v, s.k0 + k0, to - k0, p.vs[0], p.vs[1], kv, p.D);
+    tiles_here();
     __syncthreads();
     float sc[1][4];
     dot_tile<DP, 1>(sc, qt, kt, ty, tx);
@@ -345,16 +370,16 @@ __global__ void __launch_bounds__(NT) plain_split_kernel(const PackedParams p, c
     l = l * shrink + reduce16_sum(sum);
     m = top;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) acc[0][c] *= shrink;
+    for (int c = 0; c < DP / 32; ++c) acc[0][c] = mul_f2(acc[0][c], pack_f2(shrink, shrink));
     __syncwarp();  // a row's weights are written and read by one warp
     accumulate<DP, 1>(acc, w, vt, ty, tx);
   }
   if (ty >= rows) return;
   const int64_t at = (slot * p.Hk + kv) * 16 + ty;
 #pragma unroll
-  for (int c = 0; c < DP / 16; ++c) {
-    const int col = tx * 4 + 16 * (c & ~3) + (c & 3);
-    if (col < p.D) part_o[at * p.D + col] = acc[0][c];
+  for (int c = 0; c < DP / 32; c += 2) {
+    const int col = tx * 4 + 32 * c;
+    if (col < p.D) *reinterpret_cast<ulonglong2*>(part_o + at * p.D + col) = make_ulonglong2(acc[0][c], acc[0][c + 1]);
   }
   if (tx == 0) {
     part_ml[at * 2] = m;
@@ -370,9 +395,9 @@ int launch_fwd(const PackedParams& p, cudaStream_t st) {
   int dev = 0;
   GW_CUDA_TRY(cudaGetDevice(&dev));
   static OncePerDevice once;
-  const int rc = ensure_dynamic_smem(plain_fwd_kernel<DP>, tiles_bytes<DP>(2), once, dev);
+  const int rc = ensure_dynamic_smem(plain_fwd_kernel<DP>, tiles_bytes<DP>(3), once, dev);
   if (rc != GW_OK) return rc;
-  plain_fwd_kernel<DP><<<dim3(static_cast<unsigned>(packed_tile_bound(p.total_q, BT, p.nseq)), p.H), NT, tiles_bytes<DP>(2), st>>>(p);
+  plain_fwd_kernel<DP><<<dim3(static_cast<unsigned>(packed_tile_bound(p.total_q, BT, p.nseq)), p.H), NT, tiles_bytes<DP>(3), st>>>(p);
   GW_LAUNCH_CHECK();
   return GW_OK;
 }

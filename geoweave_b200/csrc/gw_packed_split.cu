@@ -4,12 +4,9 @@
 // one chunk of one sequence's keys for one key head and keeps a running maximum, sum and output per row; a second kernel joins
 // the chunks: with (m_i, l_i, o_i) of each, m = max m_i, l = sum l_i 2^(m_i - m), o = sum o_i 2^(m_i - m) / l.
 //
-// 16-bit operands: each warp walks the keys in steps of 32 (16 for wide heads) with m16n8k16 products.  Every lane copies the 16-byte
-// pieces that its own fragments need into a ring of its own in shared memory, three steps deep (about 190 KB in flight an
-// SM), and nothing is synchronised or exchanged: a contraction may run over the columns in any order as
-// long as both operands agree, so a lane's piece of a K row is its B fragment as it stands, and Q is gathered to match; for P V
-// a lane reads the same eight columns of two neighbouring keys and interleaves them.  The tensor cores are idle most of
-// the time here (16 rows against 128 lanes would leave tcgen05 waiting for a layout it needs in shared memory).
+// 16-bit operands: each warp walks its share of the keys in steps of 32 (16 for wide heads) with m16n8k16 products; K and V come by
+// TMA into a ring of its own, three steps deep (192 KB in flight an SM), so the warps never wait for one another.  The tensor cores
+// are idle most of the time (16 rows against 128 lanes would leave tcgen05 nothing to win).
 #include "gw_packed_mma.cuh"
 
 namespace gw {
@@ -18,26 +15,25 @@ namespace {
 constexpr int kRows = 16;        // rows of one key head
 constexpr int kSplitThreads = 128;
 
-// 16 bytes global -> shared, asynchronously; zeros where there is nothing to read
-__device__ __forceinline__ void copy16(uint4* dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {  // all but the last N groups of this thread have arrived
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-// A warp's step: 32 keys (16 for wide heads), K and V pieces of every lane, 8 KB; a ring of three for each of four warps
+// A warp's step: 32 keys (16 for wide heads) of K and V, 8 KB; each of the four warps has a ring of three
 template <int DP>
 struct SplitShape {
-  static constexpr int NT = DP == 64 ? 4 : 2;  // n8 tiles of keys a step
-  static constexpr int KP = DP / 32;           // 16-byte pieces of a K row in one lane
-  static constexpr int CG = DP / 64;           // 16-byte pieces of a V row in one lane
-  static constexpr int kPieces = NT * KP + NT * 2 * CG;
+  static constexpr int NT = DP == 64 ? 4 : 2;      // n8 tiles of keys a step
+  static constexpr int kKeys = 8 * NT;
+  static constexpr int kBoxes = DP / 64;           // boxes of 64 columns
+  static constexpr int kBox = kKeys * 128;         // bytes
+  static constexpr int kStep = 2 * kBoxes * kBox;  // K and V
   static constexpr int kStages = 3;
-  static constexpr size_t kRing = static_cast<size_t>(kSplitThreads) * kPieces * kStages * 16;
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kSplitThreads / 32) * kStages * kStep;
 };
+
+// four 8 x 8 matrices of 16-bit values from shared memory, one row address a lane; `trans`: transposed on the way
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void load_matrices_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
 
 struct SplitParams {
   PackedParams p;
@@ -65,104 +61,90 @@ __device__ __forceinline__ int row_limit(const PackedParams& p, const PackedSeq&
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kSplitThreads, 2) split_mma_kernel(const SplitParams sp) {
+__global__ void __launch_bounds__(kSplitThreads, 2)
+split_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const SplitParams sp) {
   using Shape = SplitShape<DP>;
-  constexpr int NT = Shape::NT, KP = Shape::KP, CG = Shape::CG, ST = Shape::kStages;
+  constexpr int NT = Shape::NT, NB = Shape::kBoxes, ST = Shape::kStages, STEP = Shape::kKeys, STRIDE = STEP * (kSplitThreads / 32);
   const PackedParams& p = sp.p;
-  extern __shared__ uint4 ring[];  // [stage][piece][thread]; every lane reads what it copied itself, so nothing is synchronised
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ float red_ml[kSplitThreads / 32][kRows][2];
-  float(*red_o)[kRows][DP] = reinterpret_cast<float(*)[kRows][DP]>(ring);  // behind the last step
+  __shared__ uint64_t full[kSplitThreads / 32][ST];
+  float(*red_o)[kRows][DP] = reinterpret_cast<float(*)[kRows][DP]>(smem);  // behind the last step
+  static_assert(sizeof(float) * (kSplitThreads / 32) * kRows * DP <= Shape::kSmem - 1024, "the join fits the rings");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
   // the key heads of one chunk side by side: a token's heads are neighbours in memory, and are read at about the same time
   const int kv = blockIdx.x % p.Hk, group = p.H / p.Hk;
   const int64_t slot = blockIdx.x / p.Hk;
+  let_dependents_launch();
+  if (lane == 0) {
+    for (int i = 0; i < ST; ++i) mbar_init(&full[warp][i], 1);
+    mbar_fence_init();
+    fence_proxy_async_smem();
+  }
+  __syncwarp();
   PackedSeq s;
   int64_t tiles, end;
   if (!packed_find(p, true, sp.chunk, slot, &s, &tiles, &end)) return;
   const int rows = min(kRows, s.lq * group);
   if (rows == 0) return;
-  const int k_from = s.tile * sp.chunk, k_to = min(s.lk, k_from + sp.chunk);
-
-  // Q fragments; lane (g, quad) holds columns 32 i + 8 quad .. + 7 of rows g and g + 8
-  uint32_t qa[KP][2][4];
-#pragma unroll
-  for (int i = 0; i < KP; ++i) {
-    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-    const int col = 32 * i + 8 * quad;
-    if (col < p.D) {
-      if (g < rows)
-        lo = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (s.q0 + g / group) * p.qs[0] + (kv * group + g % group) * p.qs[1] + col);
-      if (g + 8 < rows)
-        hi = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (s.q0 + (g + 8) / group) * p.qs[0] +
-                                             (kv * group + (g + 8) % group) * p.qs[1] + col);
+  const int k_from = s.tile * sp.chunk + warp * STEP, k_to = min(s.lk, (s.tile + 1) * sp.chunk);
+  unsigned char* ring = smem + warp * ST * Shape::kStep;
+  const int steps = k_from < k_to ? (k_to - k_from + STRIDE - 1) / STRIDE : 0;
+  auto fetch = [&](int i) {  // step i of this warp
+    if (i < steps && elect_one()) {
+      unsigned char* at = ring + i % ST * Shape::kStep;
+      mbar_arrive_expect_tx(&full[warp][i % ST], Shape::kStep);
+      load_rows<DP, STEP>(at, &tmK, kv, s.k0 + k_from + i * STRIDE, &full[warp][i % ST]);
+      load_rows<DP, STEP>(at + NB * Shape::kBox, &tmV, kv, s.k0 + k_from + i * STRIDE, &full[warp][i % ST]);
     }
-    qa[i][0][0] = lo.x; qa[i][0][1] = hi.x; qa[i][0][2] = lo.y; qa[i][0][3] = hi.y;
-    qa[i][1][0] = lo.z; qa[i][1][1] = hi.z; qa[i][1][2] = lo.w; qa[i][1][3] = hi.w;
-  }
-  const int lim0 = row_limit(p, s, g, group, rows), lim1 = row_limit(p, s, g + 8, group, rows);
-  const T* kb = static_cast<const T*>(p.k) + static_cast<int64_t>(s.k0) * p.ks[0] + kv * p.ks[1];
-  const T* vb = static_cast<const T*>(p.v) + static_cast<int64_t>(s.k0) * p.vs[0] + kv * p.vs[1];
-
-  float o[CG * 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-#pragma unroll
-  for (int i = 0; i < CG * 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  const float c = p.scale * kLog2e;
-  constexpr int STEP = 8 * NT, STRIDE = STEP * (kSplitThreads / 32);
-
-  auto fetch = [&](int k0, int stage) {
-    uint4* at = ring + stage * Shape::kPieces * kSplitThreads + threadIdx.x;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < KP; ++i) {
-        const int key = k0 + 8 * t + g, col = 32 * i + 8 * quad;
-        const bool there = key < k_to && col < p.D;
-        copy16(at + (t * KP + i) * kSplitThreads, there ? kb + key * p.ks[0] + col : kb, there);
-      }
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int i = 0; i < CG; ++i) {
-          const int key = k0 + 8 * t + 2 * quad + e, col = 64 * i + 8 * g;
-          const bool there = key < k_to && col < p.D;
-          copy16(at + (NT * KP + (t * 2 + e) * CG + i) * kSplitThreads, there ? vb + key * p.vs[0] + col : vb, there);
-        }
   };
-  int ahead = k_from + warp * STEP, stage = 0;
 #pragma unroll
-  for (int i = 0; i < ST - 1; ++i, ahead += STRIDE) {
-    if (ahead < k_to) fetch(ahead, i);
-    copies_commit();
-  }
-  for (int k0 = k_from + warp * STEP; k0 < k_to; k0 += STRIDE, ahead += STRIDE) {
-    copies_wait<ST - 2>();
-    uint4 kf[NT][KP], vf[NT][2][CG];
-    {
-      const uint4* at = ring + stage * Shape::kPieces * kSplitThreads + threadIdx.x;
+  for (int i = 0; i < ST; ++i) fetch(i);
+
+  // Q fragments: rows g and g + 8, columns 16 i + 2 quad, + 1 and + 8, + 9
+  uint32_t qa[DP / 16][4];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
+  for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
-        for (int i = 0; i < KP; ++i) kf[t][i] = at[(t * KP + i) * kSplitThreads];
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int i = 0; i < CG; ++i) vf[t][e][i] = at[(NT * KP + (t * 2 + e) * CG + i) * kSplitThreads];
-      }
+    for (int e = 0; e < 4; ++e) {
+      const int r = g + 8 * (e & 1), col = 16 * i + 8 * (e >> 1) + 2 * quad;
+      qa[i][e] = 0;
+      if (r < rows && col < p.D)
+        qa[i][e] = *reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.q) + (s.q0 + r / group) * p.qs[0] +
+                                                      (kv * group + r % group) * p.qs[1] + col);
     }
-    // the stage that the step before this one has used
-    if (ahead < k_to) fetch(ahead, stage == 0 ? ST - 1 : stage - 1);
-    copies_commit();
-    stage = stage == ST - 1 ? 0 : stage + 1;
+  const int lim0 = row_limit(p, s, g, group, rows), lim1 = row_limit(p, s, g + 8, group, rows);
+  float o[DP / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  const float c = p.scale * kLog2e;
+  bool ok = true;
+
+  for (int it = 0; it < steps; ++it) {
+    const int k0 = k_from + it * STRIDE;
+    unsigned char* at = ring + it % ST * Shape::kStep;
+    const uint32_t kt = smem_u32(at), vt = kt + NB * Shape::kBox;
+    ok = mbar_wait_bounded(&full[warp][it % ST], (it / ST) & 1);
+    if (!__all_sync(0xffffffffu, ok)) break;
+    if (k0 + STEP > k_to) {  // the last step: V rows behind the chunk may hold anything, and meet weights of zero
+#pragma unroll 1
+      for (int b = 0; b < NB; ++b)
+        for (int i = (k_to - k0) * 8 + lane; i < STEP * 8; i += 32) *reinterpret_cast<uint4*>(at + (NB + b) * Shape::kBox + i * 16) = make_uint4(0, 0, 0, 0);
+      __syncwarp();
+    }
     float sc[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+      const int row = 8 * t + (lane & 7);
 #pragma unroll
-      for (int i = 0; i < KP; ++i) {
-        mma_16816(sc[t], qa[i][0], kf[t][i].x, kf[t][i].y, T{});
-        mma_16816(sc[t], qa[i][1], kf[t][i].z, kf[t][i].w, T{});
+      for (int i = 0; i < DP / 32; ++i) {  // 32 columns: the four matrices are their 8-column chunks
+        uint32_t kf[4];
+        const int chunk = (i & 1) * 4 + (lane >> 3);
+        load_matrices(kf, kt + (i >> 1) * Shape::kBox + row * 128 + ((chunk ^ (row & 7)) << 4));
+        mma_16816(sc[t], qa[2 * i], kf[0], kf[1], T{});
+        mma_16816(sc[t], qa[2 * i + 1], kf[2], kf[3], T{});
       }
     }
     float t0 = -INFINITY, t1 = -INFINITY;
@@ -199,7 +181,7 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_mma_kernel(const Split
       pa[t][1] = pack_half2<T>(d, e);
     }
 #pragma unroll
-    for (int i = 0; i < CG * 8; ++i) {
+    for (int i = 0; i < DP / 8; ++i) {
       o[i][0] *= f0;
       o[i][1] *= f0;
       o[i][2] *= f1;
@@ -208,28 +190,31 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_mma_kernel(const Split
 #pragma unroll
     for (int t = 0; t < NT; t += 2) {
       const uint32_t a[4] = {pa[t][0], pa[t][1], pa[t + 1][0], pa[t + 1][1]};
+      const int row = 8 * t + (lane & 15);  // matrices: keys 0-7 and 8-15 of this pair of tiles, two 8-column chunks
 #pragma unroll
-      for (int i = 0; i < CG; ++i) {
-        const uint32_t x[2][4] = {{vf[t][0][i].x, vf[t][0][i].y, vf[t][0][i].z, vf[t][0][i].w}, {vf[t][1][i].x, vf[t][1][i].y, vf[t][1][i].z, vf[t][1][i].w}};
-        const uint32_t y[2][4] = {{vf[t + 1][0][i].x, vf[t + 1][0][i].y, vf[t + 1][0][i].z, vf[t + 1][0][i].w},
-                                  {vf[t + 1][1][i].x, vf[t + 1][1][i].y, vf[t + 1][1][i].z, vf[t + 1][1][i].w}};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {  // columns 64 i + 8 g + 2 w and + 1: n8 tiles 8 i + 2 w and + 1
-          mma_16816(o[8 * i + 2 * w], a, __byte_perm(x[0][w], x[1][w], 0x5410), __byte_perm(y[0][w], y[1][w], 0x5410), T{});
-          mma_16816(o[8 * i + 2 * w + 1], a, __byte_perm(x[0][w], x[1][w], 0x7632), __byte_perm(y[0][w], y[1][w], 0x7632), T{});
-        }
+      for (int i = 0; i < DP / 16; ++i) {
+        uint32_t vf[4];
+        const int chunk = (i & 3) * 2 + (lane >> 4);
+        load_matrices_trans(vf, vt + (i >> 2) * Shape::kBox + row * 128 + ((chunk ^ (row & 7)) << 4));
+        mma_16816(o[2 * i], a, vf[0], vf[1], T{});
+        mma_16816(o[2 * i + 1], a, vf[2], vf[3], T{});
       }
     }
+    __syncwarp();  // every lane has read the step
+    fetch(it + ST);
+  }
+  if (!ok) {  // let the copies in flight land before the shared memory is given up
+    if (lane == 0)
+      for (int i = 0; i < ST; ++i) mbar_wait_limit(&full[warp][i], 0, kDrainLimitNs);
+    report_status(p.status, GW_ERR_TIMEOUT);
   }
 #pragma unroll
   for (int d = 1; d < 4; d <<= 1) {
     l0 += __shfl_xor_sync(0xffffffffu, l0, d);
     l1 += __shfl_xor_sync(0xffffffffu, l1, d);
   }
-  copies_wait<0>();
-  __syncthreads();  // the ring is free
-  // join the four warps.  The accumulator of n8 tile 8 i + j holds, in lane (g, quad), rows g and g + 8 of the tile's columns
-  // 2 quad and 2 quad + 1, and the tile's column n stands for column 64 i + 8 n + j of the head
+  __syncthreads();  // the rings are free
+  // join the four warps: lane (g, quad) holds rows g and g + 8 of columns 8 i + 2 quad and + 1
   if (quad == 0) {
     red_ml[warp][g][0] = m0;
     red_ml[warp][g][1] = l0;
@@ -237,14 +222,12 @@ __global__ void __launch_bounds__(kSplitThreads, 2) split_mma_kernel(const Split
     red_ml[warp][g + 8][1] = l1;
   }
 #pragma unroll
-  for (int i = 0; i < CG; ++i)
+  for (int i = 0; i < DP / 8; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        red_o[warp][g][64 * i + 8 * (2 * quad + e) + j] = o[8 * i + j][e];
-        red_o[warp][g + 8][64 * i + 8 * (2 * quad + e) + j] = o[8 * i + j][2 + e];
-      }
+    for (int e = 0; e < 2; ++e) {
+      red_o[warp][g][8 * i + 2 * quad + e] = o[i][e];
+      red_o[warp][g + 8][8 * i + 2 * quad + e] = o[i][2 + e];
+    }
   __syncthreads();
   const int64_t at = (slot * p.Hk + kv) * kRows;
   for (int i = threadIdx.x; i < rows * p.D; i += kSplitThreads) {
@@ -298,6 +281,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_join_kernel(const SplitPa
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
+  wait_for_predecessor();
   const int64_t left = sp.slots - before;
   const int chunks = static_cast<int>(min(static_cast<int64_t>((lk + sp.chunk - 1) / sp.chunk), left < 0 ? 0 : left));
   const int64_t row0 = (before * p.Hk + kv) * kRows + r, step = static_cast<int64_t>(p.Hk) * kRows;  // partial rows of the chunks
@@ -351,34 +335,50 @@ __global__ void __launch_bounds__(kSplitThreads) split_join_kernel(const SplitPa
 }
 
 template <typename T, int DP>
-int launch_split_mma(const SplitParams& sp, dim3 grid, int dev, cudaStream_t st) {
+int launch_split_mma(const SplitParams& sp, int dtype, dim3 grid, int dev, cudaStream_t st) {
+  const PackedParams& p = sp.p;
+  CUtensorMap mk, mv;
+  GW_CUDA_TRY(cudaSetDevice(dev));  // a thread that has launched nothing yet has no context to encode tensor maps in
+  int rc = make_token_map(&mk, p.k, dtype, p.total_k, p.Hk, p.D, p.ks[0], p.ks[1], SplitShape<DP>::kKeys);
+  if (rc == GW_OK) rc = make_token_map(&mv, p.v, dtype, p.total_k, p.Hk, p.D, p.vs[0], p.vs[1], SplitShape<DP>::kKeys);
   static OncePerDevice once;
-  const int rc = ensure_dynamic_smem(split_mma_kernel<T, DP>, SplitShape<DP>::kRing, once, dev);
+  if (rc == GW_OK) rc = ensure_dynamic_smem(split_mma_kernel<T, DP>, SplitShape<DP>::kSmem, once, dev);
   if (rc != GW_OK) return rc;
-  split_mma_kernel<T, DP><<<grid, kSplitThreads, SplitShape<DP>::kRing, st>>>(sp);
+  split_mma_kernel<T, DP><<<grid, kSplitThreads, SplitShape<DP>::kSmem, st>>>(mk, mv, sp);
   return GW_OK;
 }
 
 template <typename T>
-int launch_split(const SplitParams& sp, int max_q, int dev, cudaStream_t st) {
+int launch_split(const SplitParams& sp, int max_q, int dtype, int dev, cudaStream_t st) {
   if (sp.slots * sp.p.Hk > 0x7fffffff) return GW_ERR_UNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(sp.slots * sp.p.Hk));
   int rc;
   if constexpr (sizeof(T) == 2)
-    rc = sp.p.D <= 64 ? launch_split_mma<T, 64>(sp, grid, dev, st) : launch_split_mma<T, 128>(sp, grid, dev, st);
+    rc = sp.p.D <= 64 ? launch_split_mma<T, 64>(sp, dtype, grid, dev, st) : launch_split_mma<T, 128>(sp, dtype, grid, dev, st);
   else
     rc = packed_plain_split(sp.p, sp.chunk, sp.slots, sp.part_o, sp.part_ml, st);
   if (rc != GW_OK) return rc;
   GW_LAUNCH_CHECK();
-  split_join_kernel<T><<<dim3(sp.p.nseq + 1, sp.p.Hk, max_q * (sp.p.H / sp.p.Hk)), kSplitThreads, 0, st>>>(sp, max_q);
+  // the join may be launched while the last chunks still run: it reads the borders, then waits for them
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(sp.p.nseq + 1, sp.p.Hk, max_q * (sp.p.H / sp.p.Hk));
+  cfg.blockDim = dim3(kSplitThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  GW_CUDA_TRY(cudaLaunchKernelEx(&cfg, split_join_kernel<T>, sp, max_q));
   GW_LAUNCH_CHECK();
   return GW_OK;
 }
 
-// Chunks of a size that gives every SM about eight blocks, but no shorter than four steps of a block's warps: below that
-// the fixed cost of a block and of the join outweighs what more blocks bring.
+// Chunks of a size that gives every SM about four blocks, two at a time: with eight the fixed cost of a block shows (24 caches of 129 to
+// 33 312 keys, 4 key heads: 52 us against 48; one cache of 33 312 keys, 16 key heads: 50 against 44), with two the uneven ends of ragged
+// caches do (16 key heads: 130 against 125).  No shorter than two steps of a block's warps.
 int chunk_keys(int64_t total_k, int Hk, int sms) {
-  const int64_t want = total_k * Hk / (8 * static_cast<int64_t>(sms));
+  const int64_t want = total_k * Hk / (4 * static_cast<int64_t>(sms));
   const int64_t c = (want + 127) / 128 * 128;
   return static_cast<int>(c < 256 ? 256 : c > (1 << 20) ? (1 << 20) : c);
 }
@@ -403,9 +403,9 @@ int packed_split_fwd(const PackedParams& p, int dtype, int64_t max_q, int dev, i
   sp.part_o = static_cast<float*>(workspace);
   sp.part_ml = sp.part_o + sp.slots * p.Hk * kRows * p.D;
   const int most = static_cast<int>(max_q);
-  if (dtype == GW_F32) return launch_split<float>(sp, most, dev, st);
-  if (dtype == GW_BF16) return launch_split<__nv_bfloat16>(sp, most, dev, st);
-  return launch_split<__half>(sp, most, dev, st);
+  if (dtype == GW_F32) return launch_split<float>(sp, most, dtype, dev, st);
+  if (dtype == GW_BF16) return launch_split<__nv_bfloat16>(sp, most, dtype, dev, st);
+  return launch_split<__half>(sp, most, dtype, dev, st);
 }
 
 }  // namespace gw
