@@ -34,7 +34,7 @@ struct BwdShape {
 };
 
 struct BwdShared {
-  uint64_t own_full, s_full, dp_full, loaded, p_full, ds_full, ds_done, all_done;
+  uint64_t own_full, s_full, dp_full, s_read, dp_read, p_full, ds_full, ds_done, all_done;
   uint64_t a_full[4], a_empty[4], b_full[4], b_empty[4], st_full[4];
   PackedSeq seq;
   int64_t tiles, end;
@@ -58,7 +58,7 @@ __device__ __forceinline__ uint32_t bwd_setup(BwdShared* sh, const PackedParams&
       sh->end = end;
       sh->found = found;
       for (uint64_t* b : {&sh->own_full, &sh->s_full, &sh->dp_full, &sh->ds_done, &sh->all_done}) mbar_init(b, 1);
-      for (uint64_t* b : {&sh->loaded, &sh->p_full, &sh->ds_full}) mbar_init(b, Shape::kLoad);
+      for (uint64_t* b : {&sh->s_read, &sh->dp_read, &sh->p_full, &sh->ds_full}) mbar_init(b, Shape::kLoad);
       for (int i = 0; i < 4; ++i) {
         mbar_init(&sh->a_full[i], 1);
         mbar_init(&sh->a_empty[i], 1);
@@ -162,17 +162,22 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const uint64_t kd = make_smem_desc(smem_u32(k_smem)), vd = make_smem_desc(smem_u32(v_smem));
       const uint64_t kd_mn = make_smem_desc_mn(smem_u32(k_smem));
       bool ok = n == 0 || mbar_wait_bounded(&sh->own_full, 0);
-      auto products = [&](int j) {  // S and dP of key tile j
+      auto products = [&](int j) {  // S and dP of key tile j, each as soon as the one before it has been read
         const int st = j % ST;
         ok = mbar_wait_bounded(&sh->a_full[st], (j / ST) & 1) && mbar_wait_bounded(&sh->b_full[st], (j / ST) & 1);
         if (!ok) return;
         if ((j + 1) * W > s.lk) zero_rows_from<DP, W>(k_smem + st * WB, s.lk - j * W);  // K is also dq's operand
-        if (j > 0) ok = mbar_wait_bounded(&sh->loaded, (j - 1) & 1);
+        if (j > 0) ok = mbar_wait_bounded(&sh->s_read, (j - 1) & 1);
         if (!ok) return;
         tc_fence_after();
         if (elect_one()) {
           mma_rows<DP>(tmem + kS, qd, kd + st * (WB >> 4), idesc_s);
           tc_commit(&sh->s_full);
+        }
+        if (j > 0) ok = mbar_wait_bounded(&sh->dp_read, (j - 1) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        if (elect_one()) {
           mma_rows<DP>(tmem + kDp, gd, vd + st * (WB >> 4), idesc_s);
           tc_commit(&sh->dp_full);
           tc_commit(&sh->b_empty[st]);
@@ -238,6 +243,9 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         tmem_load32(tmem + lanes + kS + half * 64, x);
         tmem_load32(tmem + lanes + kS + half * 64 + 32, x + 32);
         tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->s_read);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           float a, b;
@@ -253,7 +261,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->loaded);
+        if (lane == 0) mbar_arrive(&sh->dp_read);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           const uint64_t d = mul_f2(pack_f2(x[2 * i], x[2 * i + 1]), add_f2(pack_f2(y[2 * i], y[2 * i + 1]), nd2));
