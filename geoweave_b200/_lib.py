@@ -88,10 +88,10 @@ SIGNATURES = {
                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "gw_packed_attn_fwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int64, c_int64, c_int, c_int, c_int, c_int64]),
     "gw_packed_attn_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_int,
-                                   _I64x2, _I64x2, _I64x2, c_float, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p,
+                                   _I64x2, _I64x2, _I64x2, c_float, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p,
                                    c_void_p]),
     "gw_packed_attn_bwd_workspace_bytes": (c_size_t, [c_int64, c_int]),
-    "gw_packed_attn_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64,
+    "gw_packed_attn_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64,
                                    c_int64, c_int, c_int, c_int, _I64x2, _I64x2, _I64x2, _I64x2, c_float, c_int, c_void_p, c_void_p,
                                    c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "gw_rotary_axes": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int64, c_int, c_int, c_int, _I64x3, _I64x3, c_void_p, c_int, c_int,

@@ -23,11 +23,12 @@ struct PackedParams {
   float scale;
   int causal;
   void* o;        // [total_q, H, D] contiguous
+  void* o_low;    // like o: what rounding o to 16 bits took off, for the backward pass; nullable
   float* lse;     // [H, total_q] natural logarithm, nullable in the forward pass
   // backward
   const void* d_o;
   int64_t dos[2];
-  float* delta;   // [H, total_q]: rowsum(d_o * o)
+  float* delta;   // [H, total_q]: rowsum(d_o * (o + o_low))
   void *dq, *dk, *dv;  // contiguous
   int* status;
 };

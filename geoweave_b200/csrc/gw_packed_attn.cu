@@ -13,7 +13,7 @@ int check_packed(const PackedParams& p, int dtype, int* dev, DeviceFacts* facts)
   if (p.D > 128 || p.D % 8 != 0 || p.H > 65535 || p.total_q > 0x7fffff00 || p.total_k > 0x7fffff00 || p.nseq > 0xffffff)
     return GW_ERR_UNSUPPORTED;
   const int64_t es = static_cast<int64_t>(dtype_size(dtype));
-  for (const void* t : {p.q, p.k, p.v, static_cast<const void*>(p.o)})
+  for (const void* t : {p.q, p.k, p.v, static_cast<const void*>(p.o), static_cast<const void*>(p.o_low)})
     if (!aligned16(t)) return GW_ERR_INVALID_ARG;
   for (const int64_t s : {p.qs[0], p.qs[1], p.ks[0], p.ks[1], p.vs[0], p.vs[1]})
     if (s <= 0 || s * es % 16 != 0) return GW_ERR_INVALID_ARG;
@@ -54,9 +54,10 @@ extern "C" size_t gw_packed_attn_fwd_workspace_bytes(int dtype, int nseq, int64_
 extern "C" int gw_packed_attn_fwd(const void* q, const void* k, const void* v, int dtype, const int32_t* cu_q, const int32_t* cu_k, int nseq,
                                   int64_t total_q, int64_t total_k, int H, int Hk, int D, const int64_t* q_strides,
                                   const int64_t* k_strides, const int64_t* v_strides, float scale, int causal, int64_t max_q, void* out,
-                                  float* lse, void* workspace, size_t workspace_bytes, int* status_dev, gw_stream_t stream) {
+                                  void* out_low, float* lse, void* workspace, size_t workspace_bytes, int* status_dev, gw_stream_t stream) {
   PackedParams p = make_params(q, k, v, cu_q, cu_k, nseq, total_q, total_k, H, Hk, D, q_strides, k_strides, v_strides, scale, causal, status_dev);
   p.o = out;
+  p.o_low = dtype == GW_F32 ? nullptr : out_low;
   p.lse = lse;
   if (!out || max_q < 0) return GW_ERR_INVALID_ARG;
   int dev = 0;
@@ -76,7 +77,8 @@ extern "C" size_t gw_packed_attn_bwd_workspace_bytes(int64_t total_q, int H) {
   return total_q > 0 && H > 0 ? static_cast<size_t>(total_q) * H * 4 : 0;
 }
 
-extern "C" int gw_packed_attn_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* d_out, int dtype,
+extern "C" int gw_packed_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_low, const float* lse, const void* d_out,
+                                  int dtype,
                                   const int32_t* cu_q, const int32_t* cu_k, int nseq, int64_t total_q, int64_t total_k, int H, int Hk,
                                   int D, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
                                   const int64_t* d_out_strides, float scale, int causal, void* dq, void* dk, void* dv, void* workspace,
@@ -84,6 +86,7 @@ extern "C" int gw_packed_attn_bwd(const void* q, const void* k, const void* v, c
   PackedParams p = make_params(q, k, v, cu_q, cu_k, nseq, total_q, total_k, H, Hk, D, q_strides, k_strides, v_strides, scale, causal, status_dev);
   if (!out || !lse || !d_out || !d_out_strides || !dq || !dk || !dv) return GW_ERR_INVALID_ARG;
   p.o = const_cast<void*>(out);
+  p.o_low = dtype == GW_F32 ? nullptr : const_cast<void*>(out_low);
   p.lse = const_cast<float*>(lse);
   p.d_o = d_out;
   p.dq = dq; p.dk = dk; p.dv = dv;

@@ -208,21 +208,25 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const bool live = row < s.lq;
       const int64_t token = s.q0 + row;
-      // D of this row, from the saved output
+      // D of this row, from the saved output.  D's error is shared by the whole row of dS, where the errors of the 16-bit dS largely
+      // cancel: with o as rounded it is up to half of the gradients' error over few keys, hence o_low.
       float delta = 0.f, neg_lse = -INFINITY;
       if (live) {
         const T* o = static_cast<const T*>(p.o) + (token * p.H + head) * p.D;
+        const T* low = p.o_low != nullptr ? static_cast<const T*>(p.o_low) + (token * p.H + head) * p.D : nullptr;
         const T* g = static_cast<const T*>(p.d_o) + token * p.dos[0] + head * p.dos[1];
         for (int i = 0; i < p.D; i += 8) {
           const uint4 ow = *reinterpret_cast<const uint4*>(o + i), gw = *reinterpret_cast<const uint4*>(g + i);
-          const uint32_t oe[4] = {ow.x, ow.y, ow.z, ow.w}, ge[4] = {gw.x, gw.y, gw.z, gw.w};
+          const uint4 lw = low != nullptr ? *reinterpret_cast<const uint4*>(low + i) : make_uint4(0, 0, 0, 0);
+          const uint32_t oe[4] = {ow.x, ow.y, ow.z, ow.w}, ge[4] = {gw.x, gw.y, gw.z, gw.w}, le[4] = {lw.x, lw.y, lw.z, lw.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            float a, b, c, d;
+            float a, b, c, d, e, f;
             unpack2<T>(oe[k], a, b);
             unpack2<T>(ge[k], c, d);
-            delta = fmaf(a, c, delta);
-            delta = fmaf(b, d, delta);
+            unpack2<T>(le[k], e, f);
+            delta = fmaf(a + e, c, delta);
+            delta = fmaf(b + f, d, delta);
           }
         }
         const int64_t at = static_cast<int64_t>(head) * p.total_q + token;

@@ -425,7 +425,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->item_empty[i & 1]);
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      T* dst = static_cast<T*>(p.o) + (token * p.H + head) * p.D;
+      const int64_t at = (token * p.H + head) * p.D;
+      T *dst = static_cast<T*>(p.o) + at, *low = p.o_low != nullptr ? static_cast<T*>(p.o_low) + at : nullptr;
 #pragma unroll 1
       for (int b = 0; b < DP / 32; ++b) {
         if (32 * b >= p.D) break;
@@ -438,7 +439,18 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           uint32_t* e = reinterpret_cast<uint32_t*>(&out);
 #pragma unroll
           for (int h = 0; h < 4; ++h) e[h] = l == 0.f ? 0u : pack_half2<T>(o[8 * k + 2 * h] * inv, o[8 * k + 2 * h + 1] * inv);
-          if (live && 32 * b + 8 * k < p.D) *reinterpret_cast<uint4*>(dst + 32 * b + 8 * k) = out;
+          if (live && 32 * b + 8 * k < p.D) {
+            *reinterpret_cast<uint4*>(dst + 32 * b + 8 * k) = out;
+            if (low != nullptr) {
+#pragma unroll
+              for (int h = 0; h < 4; ++h) {
+                float u, v;
+                unpack2<T>(e[h], u, v);
+                e[h] = l == 0.f ? 0u : pack_half2<T>(fmaf(o[8 * k + 2 * h], inv, -u), fmaf(o[8 * k + 2 * h + 1], inv, -v));
+              }
+              *reinterpret_cast<uint4*>(low + 32 * b + 8 * k) = out;
+            }
+          }
         }
       }
       tc_fence_before();  // O may be written again once this item's successor has its first P

@@ -327,10 +327,15 @@ __global__ void __launch_bounds__(kSplitThreads) split_join_kernel(const SplitPa
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int64_t token = q0 + r / group;
   const int head = kv * group + r % group;
-  T* dst = static_cast<T*>(p.o) + (token * p.H + head) * p.D + 4 * col;
+  const int64_t at = (token * p.H + head) * p.D + 4 * col;
   const float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) dst[i] = from_float<T>(l == 0.f ? 0.f : v[i]);
+  for (int i = 0; i < 4; ++i) {
+    const float x = l == 0.f ? 0.f : v[i];
+    const T rounded = from_float<T>(x);
+    static_cast<T*>(p.o)[at + i] = rounded;
+    if (p.o_low != nullptr) static_cast<T*>(p.o_low)[at + i] = from_float<T>(x - to_float(rounded));
+  }
   if (col == 0 && p.lse != nullptr) p.lse[head * p.total_q + token] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 

@@ -82,12 +82,15 @@ def _checked(q, k, v, cu_seqlens_q, cu_seqlens_k):
 
 
 def packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=False, softmax_scale=None, max_seqlen_q=None,
-                             return_lse=False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """Shared implementation: ``(o [tokens, heads, head_dim], lse fp32 [heads, tokens] or None)``."""
+                             return_lse=False, o_low: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Shared implementation: ``(o [tokens, heads, head_dim], lse fp32 [heads, tokens] or None)``.  ``o_low``, contiguous and like
+    ``o``, receives what rounding ``o`` to 16 bits took off (the backward pass wants it; not used for fp32)."""
     scale = _scale(softmax_scale, q.shape[-1])
     if max_seqlen_q is not None and int(max_seqlen_q) < 0:
         raise ValueError(f"max_seqlen_q must not be negative, got {max_seqlen_q}")
     dev, T, S, H, Hk, D, cu_q, cu_k = _checked(q, k, v, cu_seqlens_q, cu_seqlens_k)
+    if o_low is not None and (o_low.shape != q.shape or o_low.dtype != q.dtype or o_low.device != dev or not o_low.is_contiguous()):
+        raise ValueError("o_low must be a contiguous tensor like o")
     o = torch.empty((T, H, D), device=dev, dtype=q.dtype)
     lse = torch.empty((H, T), device=dev, dtype=torch.float32) if return_lse else None
     if T == 0:
@@ -95,6 +98,8 @@ def packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=Fa
     if S == 0:
         if lse is not None:
             lse.fill_(float("-inf"))
+        if o_low is not None:
+            o_low.zero_()
         return o.zero_(), lse
     (q, qs), (k, ks), (v, vs) = _prepared(q), _prepared(k), _prepared(v)
     nseq, code = cu_q.shape[0] - 1, _lib.dtype_code(q)
@@ -104,7 +109,7 @@ def packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=Fa
         nbytes = lib.gw_packed_attn_fwd_workspace_bytes(code, nseq, T, S, H, Hk, D, most)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         rc = lib.gw_packed_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), code, cu_q.data_ptr(), cu_k.data_ptr(), nseq, T, S, H, Hk, D,
-                                    qs, ks, vs, scale, int(bool(causal)), most, o.data_ptr(), _lib.ptr(lse),
+                                    qs, ks, vs, scale, int(bool(causal)), most, o.data_ptr(), _lib.ptr(o_low), _lib.ptr(lse),
                                     _lib.ptr(ws), nbytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "gw_packed_attn_fwd")
     if _lib.debug_enabled():
@@ -112,7 +117,7 @@ def packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=Fa
     return o, lse
 
 
-def packed_attention_backward(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, d_out, causal=False, softmax_scale=None):
+def packed_attention_backward(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, d_out, causal=False, softmax_scale=None, o_low=None):
     """Gradients ``(dq, dk, dv)`` of the forward, contiguous and of the inputs' dtype.  The sums run in a fixed order
     (one kernel owns query rows, another key rows; no atomics), so results are reproducible."""
     scale = _scale(softmax_scale, q.shape[-1])
@@ -128,14 +133,17 @@ def packed_attention_backward(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, d_out
         return dq.zero_(), dk.zero_(), dv.zero_()
     (q, qs), (k, ks), (v, vs), (d_out, ds) = _prepared(q), _prepared(k), _prepared(v), _prepared(d_out.to(q.dtype))
     o, lse = _prepared(o.contiguous())[0], lse.contiguous()
+    if o_low is not None and (o_low.shape != o.shape or o_low.dtype != o.dtype or not o_low.is_contiguous()):
+        raise ValueError("o_low must be the forward's")
     nseq = cu_q.numel() - 1
     lib = _lib.load()
     nbytes = lib.gw_packed_attn_bwd_workspace_bytes(T, H)
     with _lib.on_device(dev):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        rc = lib.gw_packed_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), d_out.data_ptr(),
+        rc = lib.gw_packed_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.ptr(o_low), lse.data_ptr(), d_out.data_ptr(),
                                     _lib.dtype_code(q), cu_q.data_ptr(), cu_k.data_ptr(), nseq, T, S, H, Hk, D, qs, ks, vs, ds,
-                                    scale, int(bool(causal)), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nbytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
+                                    scale, int(bool(causal)), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nbytes,
+                                    _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "gw_packed_attn_bwd")
     if _lib.debug_enabled():
         _lib.check_status(dev)
@@ -145,16 +153,17 @@ def packed_attention_backward(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, d_out
 class _PackedFlashAttn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens_q, cu_seqlens_k, causal, softmax_scale, max_seqlen_q):
-        o, lse = packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, causal, softmax_scale, max_seqlen_q, True)
-        ctx.save_for_backward(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse)
+        o_low = None if q.dtype is torch.float32 else torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        o, lse = packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, causal, softmax_scale, max_seqlen_q, True, o_low)
+        ctx.save_for_backward(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, o_low)
         ctx.causal, ctx.softmax_scale = causal, softmax_scale
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        q, k, v, cu_q, cu_k, o, lse = ctx.saved_tensors
-        dq, dk, dv = packed_attention_backward(q, k, v, cu_q, cu_k, o, lse, d_out, ctx.causal, ctx.softmax_scale)
+        q, k, v, cu_q, cu_k, o, lse, o_low = ctx.saved_tensors
+        dq, dk, dv = packed_attention_backward(q, k, v, cu_q, cu_k, o, lse, d_out, ctx.causal, ctx.softmax_scale, o_low)
         return dq, dk, dv, None, None, None, None, None
 
 

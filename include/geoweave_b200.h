@@ -309,7 +309,8 @@ int gw_project_fused(const void* x, const void* weight, const void* bias, int dt
  * contiguous D; query head h reads key head h / (H / Hk).  Sequence b holds the rows cu_q[b] .. cu_q[b+1] of q and
  * cu_k[b] .. cu_k[b+1] of k and v (int32 [nseq + 1] on the device, starting at 0, not decreasing, within the totals; anything
  * else sets the status word, and no access leaves the tensors).  causal: query i of lq sees the keys 0 .. i + lk - lq of lk.
- * out [total_q, H, D] contiguous; lse fp32 [H, total_q], nullable.  A row without an allowed key gets out = 0 and
+ * out [total_q, H, D] contiguous; lse fp32 [H, total_q], nullable; out_low like out, nullable: what rounding out to 16 bits took
+ * off, for the backward pass (unused with GW_F32).  A row without an allowed key gets out = 0 and
  * lse = -inf, as do the rows behind the last sequence.  Non-finite values of k and v stay within their own sequence.
  * max_q: no sequence has more query rows (0: unknown).  It may only choose the kernel: a longer sequence sets the status
  * word and its rows further on are not written.
@@ -320,18 +321,18 @@ int gw_project_fused(const void* x, const void* weight, const void* bias, int dt
 size_t gw_packed_attn_fwd_workspace_bytes(int dtype, int nseq, int64_t total_q, int64_t total_k, int H, int Hk, int D, int64_t max_q);
 int gw_packed_attn_fwd(const void* q, const void* k, const void* v, int dtype, const int32_t* cu_q, const int32_t* cu_k, int nseq,
                        int64_t total_q, int64_t total_k, int H, int Hk, int D, const int64_t* q_strides, const int64_t* k_strides,
-                       const int64_t* v_strides, float scale, int causal, int64_t max_q, void* out, float* lse, void* workspace,
-                       size_t workspace_bytes, int* status_dev, gw_stream_t stream);
+                       const int64_t* v_strides, float scale, int causal, int64_t max_q, void* out, void* out_low, float* lse,
+                       void* workspace, size_t workspace_bytes, int* status_dev, gw_stream_t stream);
 
-/* Its backward pass.  out and lse are the forward's results, d_out [total_q, H, D] the gradient (strides as q's); dq, dk, dv
+/* Its backward pass.  out, out_low (nullable) and lse are the forward's results, d_out [total_q, H, D] the gradient (strides as q's); dq, dk, dv
  * are contiguous and like q, k, v:
- *   D = rowsum(d_out * out),  dS = P * (d_out v^T - D) * scale,  dq = dS k,  dk = sum over the key head's query heads dS^T q,
+ *   D = rowsum(d_out * (out + out_low)),  dS = P * (d_out v^T - D) * scale,  dq = dS k,  dk = sum over the key head's query heads dS^T q,
  *   dv = the same sum of P^T d_out.
  * P is made again from q, k and lse.  No atomics: the results do not depend on timing.  workspace holds D:
  * gw_packed_attn_bwd_workspace_bytes(total_q, H) bytes.  Everything else as gw_packed_attn_fwd. */
 size_t gw_packed_attn_bwd_workspace_bytes(int64_t total_q, int H);
-int gw_packed_attn_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* d_out, int dtype,
-                       const int32_t* cu_q, const int32_t* cu_k, int nseq, int64_t total_q, int64_t total_k, int H, int Hk, int D,
+int gw_packed_attn_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_low, const float* lse,
+                       const void* d_out, int dtype, const int32_t* cu_q, const int32_t* cu_k, int nseq, int64_t total_q, int64_t total_k, int H, int Hk, int D,
                        const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides, const int64_t* d_out_strides,
                        float scale, int causal, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                        int* status_dev, gw_stream_t stream);

@@ -58,13 +58,13 @@ def test_entry_points_refuse_bad_arguments_before_any_launch(lib):
     p, two, three = 4096, _lib.i64x2([64, 64]), _lib.i64x3([64, 64, 64])  # an aligned address that is never followed
     wide = (ctypes.c_int * 2)(32, 32)
     fwd = lambda q=p, dt=_lib.GW_BF16, nseq=1, tq=8, tk=8, H=1, Hk=1, D=64, st=two, scale=1.0, o=p: lib.gw_packed_attn_fwd(
-        q, p, p, dt, p, p, nseq, tq, tk, H, Hk, D, st, two, two, scale, 0, 0, o, None, None, 0, None, None)
+        q, p, p, dt, p, p, nseq, tq, tk, H, Hk, D, st, two, two, scale, 0, 0, o, None, None, None, 0, None, None)
     assert fwd(q=None) == fwd(o=None) == fwd(nseq=-1) == fwd(tq=-1) == fwd(H=3, Hk=2) == fwd(H=0) == -1
     assert fwd(q=4097) == fwd(st=_lib.i64x2([60, 64])) == fwd(st=_lib.i64x2([0, 64])) == -1
     assert fwd(scale=0.0) == fwd(scale=-1.0) == fwd(scale=float("nan")) == fwd(scale=float("inf")) == -1
     assert fwd(dt=7) == fwd(D=136) == fwd(D=60) == fwd(H=70000, Hk=70000) == fwd(tq=1 << 31) == -2
     bwd = lambda q=p, lse=p, ws=p, n=1 << 20, st=two, dq=p: lib.gw_packed_attn_bwd(
-        q, p, p, p, lse, p, _lib.GW_F16, p, p, 1, 8, 8, 1, 1, 64, two, two, two, st, 1.0, 0, dq, p, p, ws, n, None, None)
+        q, p, p, p, None, lse, p, _lib.GW_F16, p, p, 1, 8, 8, 1, 1, 64, two, two, two, st, 1.0, 0, dq, p, p, ws, n, None, None)
     assert bwd(q=None) == bwd(lse=None) == bwd(dq=None) == -1
     rot = lambda q=p, pos=p, widths=wide, axes=2, D=64, rows=4, H=1, dt=_lib.GW_F32: lib.gw_rotary_axes(
         q, None, dt, 1, 4, H, 0, D, three, None, pos, 1, axes, widths, p, p, rows, 0, p, None, None, None)
