@@ -17,6 +17,17 @@
 namespace gw {
 namespace {
 
+struct BwdShared {
+  uint64_t own_full, s_full, dp_full, s_read, dp_read, p_full, ds_full, ds_done, all_done;
+  uint64_t a_full[4], a_empty[4], b_full[4], b_empty[4], st_full[4];
+  PackedSeq seq;
+  int64_t tiles, end;
+  int found;
+  float part[2][kTile];  // the two halves' sums of d_o * o
+  uint32_t tmem_base;
+  volatile int abort_flag;
+};
+
 // A block owns 128 rows and walks the other side in tiles of kWalk rows.  Narrow heads: 64, so that the accumulators need half of the
 // tensor memory and two blocks share an SM; one's softmax, loads and output then run under the other's products.  Wide heads:
 // 128, one block an SM.  Four warps for each 64 columns make P and dS, then one warp loads and one issues products.
@@ -30,19 +41,8 @@ struct BwdShape {
   static constexpr int kStages = DP == 64 ? 4 : 2;
   static constexpr int kOwnBytes = DP / 64 * kBoxBytes, kWalkBytes = kWalk * DP * 2;
   static constexpr uint32_t kColumns = DP == 64 ? 256 : 512;
-  static constexpr size_t kSmem = 1024 + 2 * kOwnBytes + static_cast<size_t>(2 * kStages) * kWalkBytes + 512 + kStages * 2 * kWalk * 4;
+  static constexpr size_t kSmem = 1024 + 2 * kOwnBytes + static_cast<size_t>(2 * kStages) * kWalkBytes + sizeof(BwdShared) + kStages * 2 * kWalk * 4;
 };
-
-struct BwdShared {
-  uint64_t own_full, s_full, dp_full, s_read, dp_read, p_full, ds_full, ds_done, all_done;
-  uint64_t a_full[4], a_empty[4], b_full[4], b_empty[4], st_full[4];
-  PackedSeq seq;
-  int64_t tiles, end;
-  int found;
-  uint32_t tmem_base;
-  volatile int abort_flag;
-};
-static_assert(sizeof(BwdShared) <= 512, "shared bookkeeping");
 
 // Barriers, the block's tile and tensor memory; the same in both kernels.
 template <int DP>
@@ -211,14 +211,32 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       // D of this row, from the saved output.  D's error is shared by the whole row of dS, where the errors of the 16-bit dS largely
       // cancel: with o as rounded it is up to half of the gradients' error over few keys, hence o_low.
       float delta = 0.f, neg_lse = -INFINITY;
-      if (live) {
+      bool ok = true;
+      const int64_t at = static_cast<int64_t>(head) * p.total_q + token;
+      if (n > 0) {
+        // 64 columns a thread (the other half's warps take the rest of a wide head); d_o is in shared memory
         const T* o = static_cast<const T*>(p.o) + (token * p.H + head) * p.D;
-        const T* low = p.o_low != nullptr ? static_cast<const T*>(p.o_low) + (token * p.H + head) * p.D : nullptr;
-        const T* g = static_cast<const T*>(p.d_o) + token * p.dos[0] + head * p.dos[1];
-        for (int i = 0; i < p.D; i += 8) {
-          const uint4 ow = *reinterpret_cast<const uint4*>(o + i), gw = *reinterpret_cast<const uint4*>(g + i);
-          const uint4 lw = low != nullptr ? *reinterpret_cast<const uint4*>(low + i) : make_uint4(0, 0, 0, 0);
-          const uint32_t oe[4] = {ow.x, ow.y, ow.z, ow.w}, ge[4] = {gw.x, gw.y, gw.z, gw.w}, le[4] = {lw.x, lw.y, lw.z, lw.w};
+        const T* low = static_cast<const T*>(p.o_low) + (token * p.H + head) * p.D;
+        uint4 ow[8], lw[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int col = half * 64 + i * 8;
+          const bool there = live && col < p.D;
+          ow[i] = there ? *reinterpret_cast<const uint4*>(o + col) : make_uint4(0, 0, 0, 0);
+          lw[i] = there && p.o_low != nullptr ? *reinterpret_cast<const uint4*>(low + col) : make_uint4(0, 0, 0, 0);
+        }
+        if (live) {
+          const float lse = p.lse[at];
+          neg_lse = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
+        }
+        ok = mbar_wait_bounded(&sh->own_full, 0);
+        const int r = (warp & 3) * 32 + lane;
+        const unsigned char* g = g_smem + half * kBoxBytes + r * 128;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint4 gw = *reinterpret_cast<const uint4*>(g + ((i ^ (r & 7)) << 4));
+          const uint32_t oe[4] = {ow[i].x, ow[i].y, ow[i].z, ow[i].w}, ge[4] = {gw.x, gw.y, gw.z, gw.w};
+          const uint32_t le[4] = {lw[i].x, lw[i].y, lw[i].z, lw[i].w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             float a, b, c, d, e, f;
@@ -229,18 +247,20 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             delta = fmaf(b + f, d, delta);
           }
         }
-        const int64_t at = static_cast<int64_t>(head) * p.total_q + token;
-        const float lse = p.lse[at];
-        neg_lse = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
-        if (half == 0) p.delta[at] = delta;
+        if (!live) delta = 0.f;  // behind the sequence d_o is its neighbour's
+        if (Shape::kHalves == 2) {
+          sh->part[half][r] = delta;
+          named_bar_sync(1, 256);
+          delta = sh->part[0][r] + sh->part[1][r];
+        }
       }
+      if (live && half == 0) p.delta[at] = delta;
       const float c = p.scale * kLog2e;
       const uint64_t c2 = pack_f2(c, c), l2 = pack_f2(neg_lse, neg_lse), nd2 = pack_f2(-delta, -delta);
       const int limit = (p.causal ? min(s.lk, row + off + 1) : s.lk) - half * 64;
       const int open = p.causal ? min(s.lk, r0 + off + 1) : s.lk;
-      bool ok = true;
       for (int j = 0; j < n; ++j) {
-        ok = mbar_wait_bounded(&sh->s_full, j & 1);
+        ok = ok && mbar_wait_bounded(&sh->s_full, j & 1);
         if (!ok || sh->abort_flag) break;
         tc_fence_after();
         float x[64], y[64];
