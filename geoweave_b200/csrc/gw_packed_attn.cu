@@ -48,7 +48,7 @@ extern "C" size_t gw_packed_attn_fwd_workspace_bytes(int dtype, int nseq, int64_
   int dev = 0;
   DeviceFacts facts;
   if (!packed_split_fits(p, max_q) || device_facts(&dev, &facts) != GW_OK) return 0;
-  return packed_split_bytes(p, facts.sms);
+  return packed_split_bytes(p, max_q, facts.sms);
 }
 
 extern "C" int gw_packed_attn_fwd(const void* q, const void* k, const void* v, int dtype, const int32_t* cu_q, const int32_t* cu_k, int nseq,
@@ -67,7 +67,7 @@ extern "C" int gw_packed_attn_fwd(const void* q, const void* k, const void* v, i
   if (total_q == 0) return GW_OK;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (packed_split_fits(p, max_q)) {
-    if (!workspace || !aligned16(workspace) || workspace_bytes < packed_split_bytes(p, facts.sms)) return GW_ERR_WORKSPACE;
+    if (!workspace || !aligned16(workspace) || workspace_bytes < packed_split_bytes(p, max_q, facts.sms)) return GW_ERR_WORKSPACE;
     return packed_split_fwd(p, dtype, max_q, dev, facts.sms, workspace, st);
   }
   return dtype == GW_F32 ? packed_plain_fwd(p, st) : packed_mma_fwd(p, dtype, dev, facts.sms, st);

@@ -80,6 +80,14 @@ struct FwdShared {
 };
 static_assert(sizeof(FwdShared) <= 512, "shared bookkeeping");
 
+// The next item is there when the loads of the one before it have all been issued: for warps whose tile has no rows in that one
+// its whole length away, so the limit is long; it ends with anyone's failure.
+__device__ __forceinline__ bool wait_item(FwdShared* sh, int i) {
+  for (int tries = 0; tries < 60 && !sh->abort_flag; ++tries)
+    if (mbar_wait_bounded(&sh->item_full[i & 1], (i >> 1) & 1)) return true;
+  return false;
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(FwdShape<DP>::kThreads, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -211,7 +219,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint64_t vd = make_smem_desc_mn(smem_u32(v_smem));
     uint32_t ring = 0, done[kTiles] = {}, q_use[kTiles] = {};  // key tiles in the ring before this item; of each tile; query tiles
     for (int i = 0; ok && !sh->abort_flag; ++i) {
-      ok = mbar_wait_bounded(&sh->item_full[i & 1], (i >> 1) & 1);
+      ok = wait_item(sh, i);
       if (!ok) break;
       const FwdItem* item = &sh->item[i & 1];
       const int kind = uniform(item->kind), most = uniform(item->most), lk = uniform(item->lk);
@@ -318,7 +326,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const float c = p.scale * kLog2e;
     uint32_t done = 0;  // key tiles of this tile so far
     for (int i = 0; ok && !sh->abort_flag; ++i) {
-      ok = mbar_wait_bounded(&sh->item_full[i & 1], (i >> 1) & 1);
+      ok = wait_item(sh, i);
       if (!ok) break;
       const FwdItem* item = &sh->item[i & 1];  // given back behind the output
       const int kind = item->kind;

@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(NT) plain_dkv_kernel(const PackedParams p) {
 // The forward for at most 16 rows of one key head and one chunk of keys (see gw_packed_split.cu): a thread holds one row.
 // The rows come first in the tile's 64 x (DP + 4) place; partial results are joined by the caller.
 template <int DP>
-__global__ void __launch_bounds__(NT) plain_split_kernel(const PackedParams p, const int chunk, float* part_o, float* part_ml) {
+__global__ void __launch_bounds__(NT) plain_split_kernel(const PackedParams p, const int chunk, const int max_rows, float* part_o, float* part_ml) {
   extern __shared__ float smem[];
   float *qt = smem, *kt = qt + 16 * (DP + 4), *vt = kt + BT * (DP + 4), *w = vt + BT * (DP + 4);
   const int kv = blockIdx.x % p.Hk, group = p.H / p.Hk, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(NT) plain_split_kernel(const PackedParams p, c
   PackedSeq s;
   int64_t tiles, end;
   if (!packed_find(p, true, chunk, slot, &s, &tiles, &end)) return;
-  const int rows = min(16, s.lq * group);
+  const int rows = min(max_rows, s.lq * group);
   if (rows == 0) return;
   const int from = s.tile * chunk, to = min(s.lk, from + chunk);
   for (int i = threadIdx.x; i < 16 * DP; i += NT) {
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(NT) plain_split_kernel(const PackedParams p, c
     accumulate<DP, 1>(acc, w, vt, ty, tx);
   }
   if (ty >= rows) return;
-  const int64_t at = (slot * p.Hk + kv) * 16 + ty;
+  const int64_t at = (slot * p.Hk + kv) * max_rows + ty;
 #pragma unroll
   for (int c = 0; c < DP / 32; c += 2) {
     const int col = tx * 4 + 32 * c;
@@ -419,13 +419,13 @@ int launch_bwd(const PackedParams& p, cudaStream_t st) {
 }
 
 template <int DP>
-int launch_split(const PackedParams& p, int chunk, int64_t slots, float* part_o, float* part_ml, cudaStream_t st) {
+int launch_split(const PackedParams& p, int chunk, int max_rows, int64_t slots, float* part_o, float* part_ml, cudaStream_t st) {
   int dev = 0;
   GW_CUDA_TRY(cudaGetDevice(&dev));
   static OncePerDevice once;
   const int rc = ensure_dynamic_smem(plain_split_kernel<DP>, tiles_bytes<DP>(3), once, dev);
   if (rc != GW_OK) return rc;
-  plain_split_kernel<DP><<<static_cast<unsigned>(slots * p.Hk), NT, tiles_bytes<DP>(3), st>>>(p, chunk, part_o, part_ml);
+  plain_split_kernel<DP><<<static_cast<unsigned>(slots * p.Hk), NT, tiles_bytes<DP>(3), st>>>(p, chunk, max_rows, part_o, part_ml);
   GW_LAUNCH_CHECK();
   return GW_OK;
 }
@@ -434,8 +434,8 @@ int launch_split(const PackedParams& p, int chunk, int64_t slots, float* part_o,
 
 int packed_plain_fwd(const PackedParams& p, cudaStream_t st) { return p.D <= 64 ? launch_fwd<64>(p, st) : launch_fwd<128>(p, st); }
 int packed_plain_bwd(const PackedParams& p, cudaStream_t st) { return p.D <= 64 ? launch_bwd<64>(p, st) : launch_bwd<128>(p, st); }
-int packed_plain_split(const PackedParams& p, int chunk, int64_t slots, float* part_o, float* part_ml, cudaStream_t st) {
-  return p.D <= 64 ? launch_split<64>(p, chunk, slots, part_o, part_ml, st) : launch_split<128>(p, chunk, slots, part_o, part_ml, st);
+int packed_plain_split(const PackedParams& p, int chunk, int max_rows, int64_t slots, float* part_o, float* part_ml, cudaStream_t st) {
+  return p.D <= 64 ? launch_split<64>(p, chunk, max_rows, slots, part_o, part_ml, st) : launch_split<128>(p, chunk, max_rows, slots, part_o, part_ml, st);
 }
 
 }  // namespace gw

@@ -38,9 +38,10 @@ __device__ __forceinline__ void load_matrices_trans(uint32_t (&r)[4], uint32_t a
 struct SplitParams {
   PackedParams p;
   int chunk;       // keys per block
+  int rows;        // rows of a key head that the caller promises: queries x heads of a group
   int64_t slots;   // chunk slots in the workspace
-  float* part_o;   // [slots, Hk, 16, D]
-  float* part_ml;  // [slots, Hk, 16, 2]: maximum of scale log2 e S, sum
+  float* part_o;   // [slots, Hk, rows, D]
+  float* part_ml;  // [slots, Hk, rows, 2]: maximum of scale log2 e S, sum
 };
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
@@ -86,7 +87,7 @@ split_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
   PackedSeq s;
   int64_t tiles, end;
   if (!packed_find(p, true, sp.chunk, slot, &s, &tiles, &end)) return;
-  const int rows = min(kRows, s.lq * group);
+  const int rows = min(sp.rows, s.lq * group);
   if (rows == 0) return;
   const int k_from = s.tile * sp.chunk + warp * STEP, k_to = min(s.lk, (s.tile + 1) * sp.chunk);
   unsigned char* ring = smem + warp * ST * Shape::kStep;
@@ -229,7 +230,7 @@ split_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
       red_o[warp][g + 8][8 * i + 2 * quad + e] = o[i][2 + e];
     }
   __syncthreads();
-  const int64_t at = (slot * p.Hk + kv) * kRows;
+  const int64_t at = (slot * p.Hk + kv) * sp.rows;
   for (int i = threadIdx.x; i < rows * p.D; i += kSplitThreads) {
     const int r = i / p.D, col = i % p.D;
     float m = red_ml[0][r][0];
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_join_kernel(const SplitPa
   wait_for_predecessor();
   const int64_t left = sp.slots - before;
   const int chunks = static_cast<int>(min(static_cast<int64_t>((lk + sp.chunk - 1) / sp.chunk), left < 0 ? 0 : left));
-  const int64_t row0 = (before * p.Hk + kv) * kRows + r, step = static_cast<int64_t>(p.Hk) * kRows;  // partial rows of the chunks
+  const int64_t row0 = (before * p.Hk + kv) * sp.rows + r, step = static_cast<int64_t>(p.Hk) * sp.rows;  // partial rows of the chunks
 
   float m = -INFINITY;
   for (int n = threadIdx.x; n < chunks; n += kSplitThreads) m = fmaxf(m, sp.part_ml[(row0 + n * step) * 2]);
@@ -361,12 +362,12 @@ int launch_split(const SplitParams& sp, int max_q, int dtype, int dev, cudaStrea
   if constexpr (sizeof(T) == 2)
     rc = sp.p.D <= 64 ? launch_split_mma<T, 64>(sp, dtype, grid, dev, st) : launch_split_mma<T, 128>(sp, dtype, grid, dev, st);
   else
-    rc = packed_plain_split(sp.p, sp.chunk, sp.slots, sp.part_o, sp.part_ml, st);
+    rc = packed_plain_split(sp.p, sp.chunk, sp.rows, sp.slots, sp.part_o, sp.part_ml, st);
   if (rc != GW_OK) return rc;
   GW_LAUNCH_CHECK();
   // the join may be launched while the last chunks still run: it reads the borders, then waits for them
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(sp.p.nseq + 1, sp.p.Hk, max_q * (sp.p.H / sp.p.Hk));
+  cfg.gridDim = dim3(sp.p.nseq + 1, sp.p.Hk, sp.rows);
   cfg.blockDim = dim3(kSplitThreads);
   cfg.stream = st;
   cudaLaunchAttribute early = {};
@@ -396,17 +397,18 @@ bool packed_split_fits(const PackedParams& p, int64_t max_q) {
   return max_q > 0 && max_q * (p.H / p.Hk) <= kRows && p.Hk <= 65535;
 }
 
-size_t packed_split_bytes(const PackedParams& p, int sms) {
-  return static_cast<size_t>(split_slots(p, chunk_keys(p.total_k, p.Hk, sms))) * p.Hk * kRows * (p.D + 2) * 4;
+size_t packed_split_bytes(const PackedParams& p, int64_t max_q, int sms) {
+  return static_cast<size_t>(split_slots(p, chunk_keys(p.total_k, p.Hk, sms))) * p.H * max_q * (p.D + 2) * 4;
 }
 
 int packed_split_fwd(const PackedParams& p, int dtype, int64_t max_q, int dev, int sms, void* workspace, cudaStream_t st) {
   SplitParams sp;
   sp.p = p;
   sp.chunk = chunk_keys(p.total_k, p.Hk, sms);
+  sp.rows = static_cast<int>(max_q) * (p.H / p.Hk);
   sp.slots = split_slots(p, sp.chunk);
   sp.part_o = static_cast<float*>(workspace);
-  sp.part_ml = sp.part_o + sp.slots * p.Hk * kRows * p.D;
+  sp.part_ml = sp.part_o + sp.slots * p.Hk * sp.rows * p.D;
   const int most = static_cast<int>(max_q);
   if (dtype == GW_F32) return launch_split<float>(sp, most, dtype, dev, st);
   if (dtype == GW_BF16) return launch_split<__nv_bfloat16>(sp, most, dtype, dev, st);

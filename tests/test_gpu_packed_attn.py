@@ -269,6 +269,83 @@ def test_single_tokens_non_finite_neighbours():
         assert_within("o", o[b:b + 1], tuple(x[b:b + 1] for x in ref["o"]))
 
 
+def test_a_bound_on_the_queries_that_is_too_small_is_reported():
+    import geoweave_b200
+    from geoweave_b200.custom_flash_attn import packed_flash_attn_inference_func
+
+    q, k, v, _ = _inputs([1, 3, 1], [50, 60, 70], 4, 4, 64, torch.bfloat16, 19)
+    ref = packed_reference(q, k, v, [1, 3, 1], [50, 60, 70], False, 0.125)
+    o, _ = packed_flash_attn_inference_func(q, k, v, borders([1, 3, 1], q.device), borders([50, 60, 70], q.device), max_seqlen_q=1)
+    with pytest.raises(geoweave_b200.GeoWeaveError):
+        geoweave_b200.check_status()
+    for row in (0, 4):  # the sequences that keep to it
+        assert_within("o", o[row:row + 1], tuple(x[row:row + 1] for x in ref["o"]))
+    _check([1, 3, 1], [50, 60, 70], 4, 4, 64, torch.bfloat16, False, train=False, max_q=3)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_single_tokens_and_training_captured_and_replayed(dtype):
+    """Through the public entry points, autograd included: what a captured program does must follow its inputs."""
+    from geoweave_b200 import check_status
+    from geoweave_b200.custom_flash_attn import packed_flash_attn_func, packed_flash_attn_inference_func
+
+    lens_k = [700, 33, 1500]
+    q1, k, v, _ = _inputs([1] * 3, lens_k, 8, 2, 64, dtype, 22)
+    qs, ks, vs, g = _inputs([200, 90], [200, 90], 4, 2, 64, dtype, 23)
+    cu1, cuk, cus = borders([1] * 3, q1.device), borders(lens_k, q1.device), borders([200, 90], q1.device)
+
+    def step():
+        token, _ = packed_flash_attn_inference_func(q1, k, v, cu1, cuk, True, max_seqlen_q=1)
+        leaves = [x.detach().requires_grad_() for x in (qs, ks, vs)]
+        o = packed_flash_attn_func(*leaves, cus, None, True)
+        return (token, o.detach(), *torch.autograd.grad(o, leaves, g))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in (24, 25):
+        for old, new in zip((q1, k, v), _inputs([1] * 3, lens_k, 8, 2, 64, dtype, seed)):
+            old.copy_(new)
+        for old, new in zip((qs, ks, vs, g), _inputs([200, 90], [200, 90], 4, 2, 64, dtype, seed + 10)):
+            old.copy_(new)
+        for _ in range(3):
+            graph.replay()
+        for a, b in zip(step(), captured):
+            assert torch.equal(a, b)
+    check_status()
+
+
+def test_offsets_beyond_32_bits():
+    """A key sequence of more than 4 GiB a tensor: its last keys count as its first do.  The scores are set up so that a few far keys
+    carry all the weight, which makes the result known without touching the rest."""
+    from geoweave_b200 import check_status
+    from geoweave_b200.custom_flash_attn import packed_flash_attn_inference_func
+    from tests.gpu_util import dev
+
+    n, D = (1 << 24) + 77, 128
+    k = torch.zeros(n, 1, D, dtype=torch.bfloat16, device=dev())
+    v = torch.zeros(n, 1, D, dtype=torch.bfloat16, device=dev())
+    far = torch.tensor([5, n // 2 + 3, n - 2, n - 1], device=dev())
+    k[far] = 4.0
+    v[far] = torch.arange(1, 5, device=dev(), dtype=torch.bfloat16)[:, None, None]
+    q = torch.full((300, 1, D), 1.0, dtype=torch.bfloat16, device=dev())
+    cu_k = borders([n], dev())
+    # scores 512 / sqrt(128) = 45.25 for the four, 0 for the rest, whose share is n e^-45 < 1e-12: the mean of 1, 2, 3, 4
+    for rows, most in ((1, 1), (16, 16), (300, None)):
+        o, lse = packed_flash_attn_inference_func(q[:rows], k, v, borders([rows], dev()), cu_k, max_seqlen_q=most, return_lse=True)
+        assert (o.float() - 2.5).abs().max() <= 2.5 * 2.0 ** -8
+        assert (lse - (512 / math.sqrt(128) + math.log(4))).abs().max() <= 1e-4
+    # causal: the row before the last does not see the last key
+    o, _ = packed_flash_attn_inference_func(q[:2], k, v, borders([2], dev()), cu_k, True, max_seqlen_q=2)
+    assert (o[0].float() - 2.0).abs().max() <= 2.0 ** -7 and (o[1].float() - 2.5).abs().max() <= 2.5 * 2.0 ** -8
+    check_status()
+
+
 def test_bad_borders_are_reported_and_nothing_is_lost():
     import geoweave_b200
     from geoweave_b200.custom_flash_attn import packed_flash_attn_func, packed_flash_attn_inference_func
