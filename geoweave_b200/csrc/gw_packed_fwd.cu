@@ -1,6 +1,7 @@
 // Attention over packed sequences on the tcgen05 tensor cores, forward, 16-bit operands, head dim up to 128.
 //
-// One block owns 256 query rows of one head (two tiles of 128) and walks the keys in tiles of 128.  For each pair of tiles
+// One block owns 256 query rows of one head (two tiles of 128; one tile where the rows are few) and walks the keys in tiles of
+// 128.  For each pair of tiles
 //   S = Q K^T          both operands in shared memory (TMA, 128-byte swizzle), S in tensor memory, fp32
 //   P = 2^(c S - c m)  one thread owns one row: 128 values of its TMEM lane, no shuffles; c = scale log2 e
 //   O += P V           P goes back to tensor memory as the 16-bit A operand, O stays in tensor memory
@@ -8,7 +9,7 @@
 // 2^8 (P then lies within 2^8, where both 16-bit types keep their full precision, and l in fp32), which after the first tiles
 // hardly ever happens, so the rescaling pass over O is off the critical path.
 //
-// A persistent block takes its items (256 rows of a head) from a list in falling order of work, one in every gridDim: the loads of
+// A persistent block takes its items (the rows of a head) from a list in falling order of work, one in every gridDim: the loads of
 // the next item run under the last products and the output of this one.  Warps 0-3 and 4-7 are the softmax of the two tiles,
 // warp 8 makes the work list and loads, the rest issue products.  While one tile is in its softmax the tensor cores make the
 // other's S and O, and its own next S where P has room beside S (head dims up to 64: one issuing warp for each tile, so
@@ -48,23 +49,23 @@ int make_token_map(CUtensorMap* map, const void* base, int dtype, int64_t tokens
 namespace {
 
 constexpr float kLag = 8.f;  // a maximum may grow by this much (as a power of two) before O is rescaled
-constexpr int kTiles = 2;    // query tiles of a block
-constexpr int kWarps = 4 * kTiles;
-constexpr int kLoad = kWarps, kIssue = kWarps + 1;  // warps: softmax first, then one that loads, then those that issue products
+constexpr int kTiles = 2;    // most query tiles of a block
 
-template <int DP>
+// TILES: query tiles of a block, two where there are enough of them to occupy the SMs
+template <int DP, int TILES>
 struct FwdShape {
-  static constexpr int kIssuers = DP == 64 ? 2 : 1;
+  static constexpr int kWarps = 4 * TILES, kLoad = kWarps, kIssue = kWarps + 1;  // softmax first, then one that loads, then issuers
+  static constexpr int kIssuers = DP == 64 ? TILES : 1;
   static constexpr int kThreads = (kIssue + kIssuers) * 32;
   static constexpr int kStages = DP == 64 ? 3 : 2;  // K and V rings
   static constexpr int kTileBytes = DP / 64 * kBoxBytes;
   // tensor memory: S of both tiles, then P where it has room of its own (it takes S's place for wide heads), then O
   static constexpr uint32_t kS = 0, kP = DP == 64 ? 256 : 0, kPStride = DP == 64 ? 64 : 128, kO = DP == 64 ? 384 : 256;
-  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kTiles + 2 * kStages) * kTileBytes + 512;
+  static constexpr size_t kSmem = 1024 + static_cast<size_t>(TILES + 2 * kStages) * kTileBytes + 512;
 };
 
 enum { kItemRows, kItemTail, kItemEnd };
-struct FwdItem {  // 256 rows of a head; or some rows behind the last sequence; or the end of the list
+struct FwdItem {  // the rows of a block, of one head; or some rows behind the last sequence; or the end of the list
   int kind, head, q0, lq, k0, lk, r0;
   int keys[kTiles], n[kTiles], most;  // keys that any row of each tile sees; key tiles of each, of both
   int64_t part, parts, end;
@@ -81,22 +82,21 @@ struct FwdShared {
 static_assert(sizeof(FwdShared) <= 512, "shared bookkeeping");
 
 // The next item is there when the loads of the one before it have all been issued: for warps whose tile has no rows in that one
-// its whole length away, so the limit is long; it ends with anyone's failure.
+// its whole length away, so the limit is long.  After a failure the loading warp ends the list at once.
 __device__ __forceinline__ bool wait_item(FwdShared* sh, int i) {
-  for (int tries = 0; tries < 60 && !sh->abort_flag; ++tries)
-    if (mbar_wait_bounded(&sh->item_full[i & 1], (i >> 1) & 1)) return true;
-  return false;
+  return mbar_wait_limit(&sh->item_full[i & 1], (i >> 1) & 1, 60 * kWaitLimitNs);
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(FwdShape<DP>::kThreads, 1)
+template <typename T, int DP, int TILES>
+__global__ void __launch_bounds__(FwdShape<DP, TILES>::kThreads, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const PackedParams p, const int64_t slots, const int ab_format) {
-  using Shape = FwdShape<DP>;
+  using Shape = FwdShape<DP, TILES>;
   constexpr int ST = Shape::kStages, TB = Shape::kTileBytes, NI = Shape::kIssuers;
+  constexpr int kWarps = Shape::kWarps, kLoad = Shape::kLoad, kIssue = Shape::kIssue;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* q_smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  unsigned char* k_smem = q_smem + kTiles * TB;
+  unsigned char* k_smem = q_smem + TILES * TB;
   unsigned char* v_smem = k_smem + ST * TB;
   FwdShared* sh = reinterpret_cast<FwdShared*>(v_smem + ST * TB);
 
@@ -104,7 +104,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const int lane = threadIdx.x & 31;
 
   if (warp == kLoad && lane == 0) {
-    for (int i = 0; i < kTiles; ++i) {
+    for (int i = 0; i < TILES; ++i) {
       mbar_init(&sh->q_full[i], 1);
       mbar_init(&sh->q_empty[i], 1);
       mbar_init(&sh->s_full[i], 1);
@@ -136,7 +136,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   if (warp == kLoad) {
     // ------------------------------ work list and loads ------------------------------
     uint32_t ring = 0, q_use[kTiles] = {};  // key tiles and query tiles loaded so far
-    int i = 0;
+    int i = 0, told = 0;                    // items, and those of them that the others have been told of
     for (int64_t at = blockIdx.x; ok && !sh->abort_flag; at += gridDim.x, ++i) {
       FwdItem w{};
       w.head = static_cast<int>(at % p.H);
@@ -145,15 +145,15 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       int64_t tiles = 0;
       if (rank >= slots) {
         w.kind = kItemEnd;
-      } else if (packed_find_sorted(p, false, kTiles * kTile, rank, &seq, &tiles, &w.end)) {
+      } else if (packed_find_sorted(p, false, TILES * kTile, rank, &seq, &tiles, &w.end)) {
         w.kind = kItemRows;
         w.q0 = seq.q0;
         w.lq = seq.lq;
         w.k0 = seq.k0;
         w.lk = seq.lk;
-        w.r0 = seq.tile * kTiles * kTile;
+        w.r0 = seq.tile * TILES * kTile;
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
+        for (int t = 0; t < TILES; ++t) {
           const int last = min(w.r0 + (t + 1) * kTile, w.lq);
           w.keys[t] = last <= w.r0 + t * kTile ? 0 : p.causal ? max(0, min(w.lk, last + w.lk - w.lq)) : w.lk;
           w.n[t] = (w.keys[t] + kTile - 1) / kTile;
@@ -170,6 +170,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         sh->item[i & 1] = w;
         mbar_arrive(&sh->item_full[i & 1]);
       }
+      ++told;
       if (w.kind == kItemEnd) break;
       if (w.kind == kItemTail) continue;
       const int kv = w.head / (p.H / p.Hk);
@@ -192,7 +193,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           mbar_arrive_expect_tx(&sh->k_full[st], TB);
           load_rows<DP>(k_smem + st * TB, &tmK, kv, w.k0 + j * kTile, &sh->k_full[st]);
         }
-        if (j == 0 && w.n[1] > 0) load_q(1);
+        if (TILES == 2 && j == 0 && w.n[1] > 0) load_q(1);
         ok = ok && mbar_wait_bounded(&sh->v_empty[st], par);
         if (lane == 0) {  // also after a wait that ran out, so that the drain below finds both copies of the stage
           mbar_arrive_expect_tx(&sh->v_full[st], TB);
@@ -201,8 +202,11 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
     }
     if (!ok) sh->abort_flag = 1;
-    if (sh->abort_flag && lane == 0) {  // let the copies in flight land before the shared memory is given up
-      for (int t = 0; t < kTiles; ++t)
+    if (sh->abort_flag && lane == 0) {
+      sh->item[told & 1].kind = kItemEnd;
+      mbar_arrive(&sh->item_full[told & 1]);
+      // let the copies in flight land before the shared memory is given up
+      for (int t = 0; t < TILES; ++t)
         if (q_use[t] > 0) mbar_wait_limit(&sh->q_full[t], (q_use[t] - 1) & 1, kDrainLimitNs);
       for (uint32_t u = ring > ST ? ring - ST : 0u; u <= ring; ++u) {
         mbar_wait_limit(&sh->k_full[u % ST], (u / ST) & 1u, kDrainLimitNs);
@@ -225,7 +229,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const int kind = uniform(item->kind), most = uniform(item->most), lk = uniform(item->lk);
       int n[kTiles], keys[kTiles];
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
+      for (int t = 0; t < TILES; ++t) {
         n[t] = uniform(item->n[t]);
         keys[t] = uniform(item->keys[t]);
       }
@@ -248,7 +252,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       };
       int mine = 0;
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
+      for (int t = 0; t < TILES; ++t) {
         if (t % NI != w0 || n[t] == 0) continue;
         mine = max(mine, n[t]);
         scores(t, 0);
@@ -268,7 +272,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint32_t st = (ring + j) % ST, st_next = (ring + j + 1) % ST;
         bool v_here = false;
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
+        for (int t = 0; t < TILES; ++t) {
           if (t % NI != w0 || j >= n[t]) continue;
           const uint32_t c = done[t] + j;
           if (DP == 64 && j + 1 < n[t]) scores(t, j + 1);  // P has its own place: ahead of this tile's softmax
@@ -308,7 +312,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       ring += most;
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
+      for (int t = 0; t < TILES; ++t) {
         done[t] += n[t];
         q_use[t] += n[t] > 0 ? 1 : 0;
       }
@@ -477,28 +481,38 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   if (warp == kIssue) tmem_dealloc(tmem, 512);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int TILES>
 int launch_fwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
   GW_CUDA_TRY(cudaSetDevice(dev));  // a thread that has launched nothing yet has no context to encode tensor maps in
   int rc = make_token_map(&mq, p.q, dtype, p.total_q, p.H, p.D, p.qs[0], p.qs[1], kTile);
   if (rc == GW_OK) rc = make_token_map(&mk, p.k, dtype, p.total_k, p.Hk, p.D, p.ks[0], p.ks[1], kTile);
   if (rc == GW_OK) rc = make_token_map(&mv, p.v, dtype, p.total_k, p.Hk, p.D, p.vs[0], p.vs[1], kTile);
+  using Shape = FwdShape<DP, TILES>;
   static OncePerDevice once;
-  if (rc == GW_OK) rc = ensure_dynamic_smem(packed_fwd_kernel<T, DP>, FwdShape<DP>::kSmem, once, dev);
+  if (rc == GW_OK) rc = ensure_dynamic_smem(packed_fwd_kernel<T, DP, TILES>, Shape::kSmem, once, dev);
   if (rc != GW_OK) return rc;
-  const int64_t slots = packed_tile_bound(p.total_q, kTiles * kTile, p.nseq), items = slots * p.H;
-  packed_fwd_kernel<T, DP><<<static_cast<unsigned>(items < sms ? items : sms), FwdShape<DP>::kThreads, FwdShape<DP>::kSmem, st>>>(
+  const int64_t slots = packed_tile_bound(p.total_q, TILES * kTile, p.nseq), items = slots * p.H;
+  packed_fwd_kernel<T, DP, TILES><<<static_cast<unsigned>(items < sms ? items : sms), Shape::kThreads, Shape::kSmem, st>>>(
       mq, mk, mv, p, slots, dtype == GW_BF16 ? 1 : 0);
   GW_LAUNCH_CHECK();
   return GW_OK;
 }
 
+template <typename T>
+int choose_fwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t st) {
+  // Rows for fewer blocks of two tiles than there are SMs: one tile a block, twice the blocks (one view of 1041 tokens, 16 heads: 20.5 us
+  // against 26.6; 1041 rows against 33 312 keys: 274 against 379).  With three views the two are equal, with 32 two tiles
+  // win, 269 us against 340, since both share every key tile.
+  const bool few = (p.total_q + 2 * kTile - 1) / (2 * kTile) * p.H < sms;
+  if (p.D <= 64) return few ? launch_fwd<T, 64, 1>(p, dtype, dev, sms, st) : launch_fwd<T, 64, 2>(p, dtype, dev, sms, st);
+  return few ? launch_fwd<T, 128, 1>(p, dtype, dev, sms, st) : launch_fwd<T, 128, 2>(p, dtype, dev, sms, st);
+}
+
 }  // namespace
 
 int packed_mma_fwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t st) {
-  if (dtype == GW_BF16) return p.D <= 64 ? launch_fwd<__nv_bfloat16, 64>(p, dtype, dev, sms, st) : launch_fwd<__nv_bfloat16, 128>(p, dtype, dev, sms, st);
-  return p.D <= 64 ? launch_fwd<__half, 64>(p, dtype, dev, sms, st) : launch_fwd<__half, 128>(p, dtype, dev, sms, st);
+  return dtype == GW_BF16 ? choose_fwd<__nv_bfloat16>(p, dtype, dev, sms, st) : choose_fwd<__half>(p, dtype, dev, sms, st);
 }
 
 }  // namespace gw

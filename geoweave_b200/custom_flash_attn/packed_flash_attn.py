@@ -192,5 +192,5 @@ def packed_flash_attn_inference_func(q, k, v, cu_seqlens_q, cu_seqlens_k=None, c
                                      return_lse: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """As ``packed_flash_attn_func`` without gradients: ``(o, lse | None)``, ``lse`` fp32 ``[H, total_q]`` (natural logarithm,
     ``-inf`` for rows without an allowed key)."""
-    return packed_attention_forward(q.detach(), k.detach(), v.detach(), cu_seqlens_q, cu_seqlens_k, causal, softmax_scale, max_seqlen_q,
-                                    return_lse)
+    with torch.no_grad():
+        return packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, causal, softmax_scale, max_seqlen_q, return_lse)
