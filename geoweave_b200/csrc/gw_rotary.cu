@@ -22,7 +22,11 @@ namespace {
 
 constexpr int kAxes = 4;
 constexpr int kThreads = 256;
-constexpr int kBlocksPerSm = 6;
+// Blocks an SM, and so registers a thread: with whole 16-byte pieces the compiler needs more (fp32, 33 312 tokens: 94 us with four
+// against 103 with six; bf16 heads of 128: 41 against 47), with 8-byte ones more threads are better (bf16, 12-column halves: 61
+// with six against 72 with four).
+template <typename T, int V>
+constexpr int kBlocksPerSm = sizeof(T) * V >= 16 ? 4 : 6;
 
 struct RotaryParams {
   const void *q, *k;
@@ -47,19 +51,13 @@ struct alignas(sizeof(T) * V) Piece {
 };
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) rotary_axes_kernel(const RotaryParams p) {
+__global__ void __launch_bounds__(kThreads, (kBlocksPerSm<T, V>)) rotary_axes_kernel(const RotaryParams p) {
   const int pairs = p.turned / 2 / V, units = pairs + (p.D - p.turned + V - 1) / V;
   const int per_token = units * p.head_lanes;
   const int slot = threadIdx.x / per_token;
   if (slot >= p.tokens_per_block) return;
   const int unit = (threadIdx.x % per_token) % units, lane = (threadIdx.x % per_token) / units;
   using P = Piece<T, V>;
-  const bool turns = unit < pairs;
-  int a = 0, before = 0;  // the axis of this piece, and the angles of the axes in front of it
-  while (turns && unit * V >= before + p.half[a]) before += p.half[a++];
-  // the pair's two pieces; a piece behind the axes is copied
-  const int lo = turns ? unit * V + before : p.turned + (unit - pairs) * V, hi = turns ? lo + p.half[a] : lo;
-
   const int64_t stride = static_cast<int64_t>(gridDim.x) * p.tokens_per_block;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * p.tokens_per_block + slot; t < p.tokens; t += stride) {
     const int64_t b = t / p.per_batch, n = t % p.per_batch;
@@ -67,16 +65,22 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) rotary_axes_kernel(con
     const T* k = static_cast<const T*>(p.k) + b * p.ks[0] + n * p.ks[1];
     T* qo = static_cast<T*>(p.q_out) + t * p.H * p.D;
     T* ko = static_cast<T*>(p.k_out) + t * p.Hk * p.D;
-    if (!turns) {
+
+    if (unit >= pairs) {  // a piece behind the axes
+      const int c = p.turned + (unit - pairs) * V;
 #pragma unroll 4
       for (int h = lane; h < p.H + p.Hk; h += p.head_lanes) {
         const bool is_q = h < p.H;
         const T* src = is_q ? q + h * p.qs[2] : k + (h - p.H) * p.ks[2];
         T* dst = is_q ? qo + h * p.D : ko + (h - p.H) * p.D;
-        *reinterpret_cast<P*>(dst + lo) = *reinterpret_cast<const P*>(src + lo);
+        *reinterpret_cast<P*>(dst + c) = *reinterpret_cast<const P*>(src + c);
       }
       continue;
     }
+
+    int a = 0, before = 0;  // the axis of this piece, and the angles of the axes in front of it
+    while (unit * V >= before + p.half[a]) before += p.half[a++];
+    const int lo = unit * V + before, hi = lo + p.half[a];
     const int64_t at = t * p.axes + a;
     int64_t pos = p.pos64 ? static_cast<const int64_t*>(p.pos)[at] : static_cast<const int32_t*>(p.pos)[at];
     if (pos < 0 || pos >= p.table_rows) {  // outside the tables: say so and carry on
@@ -112,7 +116,7 @@ int launch(RotaryParams p, int sms, cudaStream_t st) {
   p.head_lanes = (heads + 3) / 4;  // four heads a thread keep eight loads in flight
   if (p.head_lanes * units > kThreads) p.head_lanes = kThreads / units;
   p.tokens_per_block = kThreads / (units * p.head_lanes);
-  const int64_t need = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block, most = static_cast<int64_t>(sms) * kBlocksPerSm;
+  const int64_t need = (p.tokens + p.tokens_per_block - 1) / p.tokens_per_block, most = static_cast<int64_t>(sms) * kBlocksPerSm<T, V>;
   const int64_t grid = need < most ? need : most;
   rotary_axes_kernel<T, V><<<static_cast<unsigned>(grid), kThreads, 0, st>>>(p);
   GW_LAUNCH_CHECK();
