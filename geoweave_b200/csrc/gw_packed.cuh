@@ -44,14 +44,24 @@ __device__ __forceinline__ int packed_border(const int32_t* cu, int i, int64_t t
   return c < 0 ? 0 : (c > total ? static_cast<int>(total) : c);
 }
 
+// Warp-wide: reports border arrays that do not start at zero, decrease or pass the totals.  One warp of a call does it, behind
+// its other work.
+__device__ __forceinline__ void packed_check(const PackedParams& p) {
+  bool bad = false;
+  for (int b = threadIdx.x & 31; b < p.nseq; b += 32) {
+    const int q0 = p.cu_q[b], q1 = p.cu_q[b + 1], k0 = p.cu_k[b], k1 = p.cu_k[b + 1];
+    bad |= q0 < 0 || q1 < q0 || q1 > p.total_q || k0 < 0 || k1 < k0 || k1 > p.total_k || (b == 0 && (q0 != 0 || k0 != 0));
+  }
+  if (__any_sync(0xffffffffu, bad) && (threadIdx.x & 31) == 0) report_status(p.status, GW_ERR_INVALID_ARG);
+}
+
 // Warp-wide: tile `slot` of the list of all sequences' tiles (tile_rows rows each, along the q or the k side).  True
-// when there is such a tile.  Otherwise *tiles is the number of tiles, *end the row behind the last sequence, and border
-// arrays that do not start at zero, decrease or pass the totals are reported.  All lanes get the same answers.
+// when there is such a tile.  Otherwise *tiles is the number of tiles and *end the row behind the last sequence.  All lanes get
+// the same answers.
 __device__ __forceinline__ bool packed_find(const PackedParams& p, bool key_side, int tile_rows, int64_t slot, PackedSeq* out,
                                             int64_t* tiles, int64_t* end) {
   const int lane = threadIdx.x & 31;
   int64_t base = 0;
-  bool bad = false;
   for (int b0 = 0; b0 < p.nseq; b0 += 32) {
     const int b = b0 + lane;
     int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
@@ -60,12 +70,10 @@ __device__ __forceinline__ bool packed_find(const PackedParams& p, bool key_side
       q1 = packed_border(p.cu_q, b + 1, p.total_q);
       k0 = packed_border(p.cu_k, b, p.total_k);
       k1 = packed_border(p.cu_k, b + 1, p.total_k);
-      bad |= q0 != p.cu_q[b] || q1 != p.cu_q[b + 1] || k0 != p.cu_k[b] || k1 != p.cu_k[b + 1] || q1 < q0 || k1 < k0;
-      bad |= b == 0 && (q0 != 0 || k0 != 0);
       q1 = max(q0, q1);
       k1 = max(k0, k1);
     }
-    const int n = key_side ? (k1 - k0 + tile_rows - 1) / tile_rows : (q1 - q0 + tile_rows - 1) / tile_rows;
+    const int n = static_cast<int>((static_cast<int64_t>(key_side ? k1 - k0 : q1 - q0) + tile_rows - 1) / tile_rows);
     int64_t incl = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -86,7 +94,6 @@ __device__ __forceinline__ bool packed_find(const PackedParams& p, bool key_side
   }
   *tiles = base;
   *end = p.nseq > 0 ? packed_border(key_side ? p.cu_k : p.cu_q, p.nseq, key_side ? p.total_k : p.total_q) : 0;
-  if (__any_sync(0xffffffffu, bad) && lane == 0) report_status(p.status, GW_ERR_INVALID_ARG);
   return false;
 }
 

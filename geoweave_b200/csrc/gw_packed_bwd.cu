@@ -320,6 +320,10 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                    live, n > 0);
     }
   }
+  if (blockIdx.x == 0 && warp == Shape::kLoad) {
+    __syncwarp();
+    packed_check(p);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

@@ -201,6 +201,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
     }
+    if (blockIdx.x == 0) packed_check(p);
     if (!ok) sh->abort_flag = 1;
     if (sh->abort_flag && lane == 0) {
       sh->item[told & 1].kind = kItemEnd;

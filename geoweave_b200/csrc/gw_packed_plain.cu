@@ -124,6 +124,7 @@ __device__ __forceinline__ float reduce16_sum(float x) {
 // The block's work; false when it has none (then the rows behind the last sequence have been dealt with).
 __device__ __forceinline__ bool block_tile(const PackedParams& p, bool key_side, int head, PackedSeq* s, void* out, void* out2, float* lse) {
   int64_t tiles, end;
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0 && threadIdx.x < 32) packed_check(p);
   if (packed_find(p, key_side, BT, blockIdx.x, s, &tiles, &end)) return true;
   const int64_t total = key_side ? p.total_k : p.total_q, parts = gridDim.x - tiles, part = blockIdx.x - tiles;
   const int heads = key_side ? p.Hk : p.H;
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(NT) plain_split_kernel(const PackedParams p, c
   if (!packed_find(p, true, chunk, slot, &s, &tiles, &end)) return;
   const int rows = min(max_rows, s.lq * group);
   if (rows == 0) return;
-  const int from = s.tile * chunk, to = min(s.lk, from + chunk);
+  const int from = s.tile * chunk, to = from + min(chunk, s.lk - from);
   for (int i = threadIdx.x; i < 16 * DP; i += NT) {
     const int r = i / DP, c = i % DP;
     qt[r * (DP + 4) + c] =

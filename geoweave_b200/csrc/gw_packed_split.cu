@@ -89,7 +89,7 @@ split_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
   if (!packed_find(p, true, sp.chunk, slot, &s, &tiles, &end)) return;
   const int rows = min(sp.rows, s.lq * group);
   if (rows == 0) return;
-  const int k_from = s.tile * sp.chunk + warp * STEP, k_to = min(s.lk, (s.tile + 1) * sp.chunk);
+  const int k_chunk = s.tile * sp.chunk, k_to = k_chunk + min(sp.chunk, s.lk - k_chunk), k_from = k_chunk + warp * STEP;
   unsigned char* ring = smem + warp * ST * Shape::kStep;
   const int steps = k_from < k_to ? (k_to - k_from + STRIDE - 1) / STRIDE : 0;
   auto fetch = [&](int i) {  // step i of this warp
@@ -260,7 +260,9 @@ __global__ void __launch_bounds__(kSplitThreads) split_join_kernel(const SplitPa
   const PackedParams& p = sp.p;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kv = blockIdx.y, group = p.H / p.Hk, b = blockIdx.x, r = blockIdx.z;
   if (b == p.nseq) {
+    wait_for_predecessor();  // every block: the kernel must not end before the chunks do
     if (r > 0) return;
+    if (kv == 0 && warp == 0) packed_check(p);
     PackedSeq s;
     int64_t tiles, end;
     packed_find(p, false, 1, static_cast<int64_t>(0x7fffffffffffffff), &s, &tiles, &end);
@@ -274,17 +276,20 @@ __global__ void __launch_bounds__(kSplitThreads) split_join_kernel(const SplitPa
   const int k0 = packed_border(p.cu_k, b, p.total_k), k1 = packed_border(p.cu_k, b + 1, p.total_k);
   const int lq = max(0, q1 - q0), lk = max(0, k1 - k0);
   if (lq > max_q && threadIdx.x == 0) report_status(p.status, GW_ERR_INVALID_ARG);
-  if (r >= min(lq, max_q) * group) return;
+  if (r >= min(lq, max_q) * group) {
+    wait_for_predecessor();
+    return;
+  }
   int64_t before = 0;  // chunks in front of this sequence
   for (int i = lane; i < b; i += 32) {
     const int c0 = packed_border(p.cu_k, i, p.total_k), c1 = packed_border(p.cu_k, i + 1, p.total_k);
-    before += (max(0, c1 - c0) + sp.chunk - 1) / sp.chunk;
+    before += (static_cast<int64_t>(max(0, c1 - c0)) + sp.chunk - 1) / sp.chunk;
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
   wait_for_predecessor();
   const int64_t left = sp.slots - before;
-  const int chunks = static_cast<int>(min(static_cast<int64_t>((lk + sp.chunk - 1) / sp.chunk), left < 0 ? 0 : left));
+  const int chunks = static_cast<int>(min((static_cast<int64_t>(lk) + sp.chunk - 1) / sp.chunk, left < 0 ? 0 : left));
   const int64_t row0 = (before * p.Hk + kv) * sp.rows + r, step = static_cast<int64_t>(p.Hk) * sp.rows;  // partial rows of the chunks
 
   float m = -INFINITY;

@@ -118,13 +118,13 @@ class _RotaryAxesFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, pos, axes):
         ctx.axes = axes
-        ctx.save_for_backward(pos)
+        ctx.save_for_backward(pos, axes.cos, axes.sin)  # the tables too, so that a change in between is noticed
         return _rotate(q, k, pos, axes, False)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
-        (pos,) = ctx.saved_tensors
+        pos, _, _ = ctx.saved_tensors
         return (*_rotate(dq, dk, pos, ctx.axes, True), None, None)
 
 
@@ -145,11 +145,11 @@ class _RotaryQOnly(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, pos, axes):
         ctx.axes = axes
-        ctx.save_for_backward(pos)
+        ctx.save_for_backward(pos, axes.cos, axes.sin)  # the tables too, so that a change in between is noticed
         return _rotate(q, None, pos, axes, False)[0]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq):
-        (pos,) = ctx.saved_tensors
+        pos, _, _ = ctx.saved_tensors
         return _rotate(dq, None, pos, ctx.axes, True)[0], None, None

@@ -365,6 +365,46 @@ def test_bad_borders_are_reported_and_nothing_is_lost():
     _check([100], [100], 2, 2, 64, torch.bfloat16, False)  # the next call is right again
 
 
+def test_borders_that_name_more_tiles_than_there_are_rows_are_reported():
+    """Overlapping sequences leave no spare block, which is where the rows behind the last sequence are dealt with."""
+    import geoweave_b200
+    from geoweave_b200.custom_flash_attn import packed_flash_attn_func, packed_flash_attn_inference_func
+
+    for dtype in DTYPES:
+        q, k, v, g = _inputs([2000], [2000], 2, 2, 64, dtype, 40)
+        cu = torch.tensor([0, 2000] * 8, dtype=torch.int32, device=q.device)
+        for most in (None, 1):
+            packed_flash_attn_inference_func(q, k, v, cu, None, False, None, most)
+            with pytest.raises(geoweave_b200.GeoWeaveError):
+                geoweave_b200.check_status()
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        torch.autograd.grad(packed_flash_attn_func(*leaves, cu), leaves, g)
+        with pytest.raises(geoweave_b200.GeoWeaveError):
+            geoweave_b200.check_status()
+
+
+def test_changes_between_forward_and_backward_are_noticed():
+    from geoweave_b200.custom_flash_attn import packed_flash_attn_func
+    from geoweave_b200.rotary import apply_rotary_axes, rotary_axes
+
+    q, k, v, g = _inputs([50], [50], 2, 2, 64, torch.bfloat16, 41)
+    cu = borders([50], q.device)
+    leaf = q.clone().requires_grad_()
+    o = packed_flash_attn_func(leaf, k, v, cu)
+    k.add_(1)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(o, leaf, g)
+    axes = rotary_axes((32, 32), 8, q.device)
+    out, _ = apply_rotary_axes(leaf, None, torch.zeros(50, 2, dtype=torch.int64, device=q.device), axes)
+    axes.cos.add_(1)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, leaf, g)
+    o = packed_flash_attn_func(leaf, k, v, cu)
+    (first,) = torch.autograd.grad(o, leaf, g, create_graph=True)
+    with pytest.raises(RuntimeError):  # no second derivative, and no silent zero in its place
+        torch.autograd.grad(first.sum(), leaf)
+
+
 def test_refusals():
     from geoweave_b200.custom_flash_attn import packed_flash_attn_func as f
 
