@@ -78,25 +78,20 @@ __device__ __forceinline__ uint32_t bwd_setup(BwdShared* sh, const PackedParams&
   return __shfl_sync(0xffffffffu, sh->tmem_base, 0);
 }
 
-// columns [from, to) of one row of an accumulator in this thread's TMEM lane, times mul, as 16-bit values (zeros if !any)
+// columns [from, to) of one row of an accumulator in this thread's TMEM lane, times mul, as 16-bit values (zeros if !any); `base` is
+// the tensor that the row `dst` belongs to
 template <typename T>
-__device__ __forceinline__ void store_acc(T* dst, uint32_t addr, int from, int to, int D, float mul, bool live, bool any) {
+__device__ __forceinline__ void store_acc(const void* base, T* dst, uint32_t addr, int from, int to, int D, float mul, bool live, bool any) {
 #pragma unroll 1
   for (int b = from; b < to; b += 32) {
     if (b >= D) break;
     float o[32];
-    if (any) {
-      tmem_load32(addr + b, o);
-      tmem_wait_ld();
-    }
+    tmem_load32(addr + b, o);  // without a product: whatever is there, and unused
+    tmem_wait_ld();
+    uint32_t e[16];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint4 w;
-      uint32_t* e = reinterpret_cast<uint32_t*>(&w);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) e[k] = any ? pack_half2<T>(o[8 * i + 2 * k] * mul, o[8 * i + 2 * k + 1] * mul) : 0u;
-      if (live && b + 8 * i < D) *reinterpret_cast<uint4*>(dst + b + 8 * i) = w;
-    }
+    for (int k = 0; k < 16; ++k) e[k] = any ? pack_half2<T>(o[2 * k] * mul, o[2 * k + 1] * mul) : 0u;
+    if (live) store_row32(dst + b, e, D - b, row_sectors(base, D));
   }
 }
 
@@ -316,7 +311,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         report_status(p.status, GW_ERR_TIMEOUT);
       }
       tc_fence_after();
-      store_acc<T>(static_cast<T*>(p.dq) + (token * p.H + head) * p.D, tmem + lanes + kDq, half * (DP / Shape::kHalves), (half + 1) * (DP / Shape::kHalves), p.D, p.scale,
+      store_acc<T>(p.dq, static_cast<T*>(p.dq) + (token * p.H + head) * p.D, tmem + lanes + kDq, half * (DP / Shape::kHalves), (half + 1) * (DP / Shape::kHalves), p.D, p.scale,
                    live, n > 0);
     }
   }
@@ -543,9 +538,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       tc_fence_after();
       const int64_t at = (static_cast<int64_t>(s.k0 + row) * p.Hk + kv) * p.D;
-      if (half == 0) store_acc<T>(static_cast<T*>(p.dv) + at, tmem + lanes + kDv, 0, DP, p.D, kLower, live, n > 0);
+      if (half == 0) store_acc<T>(p.dv, static_cast<T*>(p.dv) + at, tmem + lanes + kDv, 0, DP, p.D, kLower, live, n > 0);
       if (half == Shape::kHalves - 1)
-        store_acc<T>(static_cast<T*>(p.dk) + at, tmem + lanes + kDk, 0, DP, p.D, p.scale, live, n > 0);
+        store_acc<T>(p.dk, static_cast<T*>(p.dk) + at, tmem + lanes + kDk, 0, DP, p.D, p.scale, live, n > 0);
     }
   }
   tc_fence_before();

@@ -446,24 +446,18 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         float o[32];
         tmem_load32(o_addr + 32 * b, o);  // without a key: whatever is there, and unused
         tmem_wait_ld();
+        uint32_t e[16];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint4 out;
-          uint32_t* e = reinterpret_cast<uint32_t*>(&out);
+        for (int k = 0; k < 16; ++k) e[k] = l == 0.f ? 0u : pack_half2<T>(o[2 * k] * inv, o[2 * k + 1] * inv);
+        if (live) store_row32(dst + 32 * b, e, p.D - 32 * b, row_sectors(p.o, p.D));
+        if (low != nullptr) {
 #pragma unroll
-          for (int h = 0; h < 4; ++h) e[h] = l == 0.f ? 0u : pack_half2<T>(o[8 * k + 2 * h] * inv, o[8 * k + 2 * h + 1] * inv);
-          if (live && 32 * b + 8 * k < p.D) {
-            *reinterpret_cast<uint4*>(dst + 32 * b + 8 * k) = out;
-            if (low != nullptr) {
-#pragma unroll
-              for (int h = 0; h < 4; ++h) {
-                float u, v;
-                unpack2<T>(e[h], u, v);
-                e[h] = l == 0.f ? 0u : pack_half2<T>(fmaf(o[8 * k + 2 * h], inv, -u), fmaf(o[8 * k + 2 * h + 1], inv, -v));
-              }
-              *reinterpret_cast<uint4*>(low + 32 * b + 8 * k) = out;
-            }
+          for (int k = 0; k < 16; ++k) {
+            float u, v;
+            unpack2<T>(e[k], u, v);
+            e[k] = l == 0.f ? 0u : pack_half2<T>(fmaf(o[2 * k], inv, -u), fmaf(o[2 * k + 1], inv, -v));
           }
+          if (live) store_row32(low + 32 * b, e, p.D - 32 * b, row_sectors(p.o_low, p.D));
         }
       }
       tc_fence_before();  // O may be written again once this item's successor has its first P

@@ -135,6 +135,24 @@ __device__ __forceinline__ bool elect_one() {
 // a value read from memory that is the same in all lanes, made known as such to the compiler
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
+// 32 16-bit values of one row, as many of them as lie below `left`: whole 32-byte sectors where the row allows it
+__device__ __forceinline__ void store_row32(void* dst, const uint32_t (&e)[16], int left, bool sectors) {
+  if (sectors) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (16 * i < left)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(static_cast<char*>(dst) + 32 * i), "r"(e[8 * i]),
+                     "r"(e[8 * i + 1]), "r"(e[8 * i + 2]), "r"(e[8 * i + 3]), "r"(e[8 * i + 4]), "r"(e[8 * i + 5]), "r"(e[8 * i + 6]),
+                     "r"(e[8 * i + 7])
+                     : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (8 * i < left) reinterpret_cast<uint4*>(dst)[i] = make_uint4(e[4 * i], e[4 * i + 1], e[4 * i + 2], e[4 * i + 3]);
+  }
+}
+__device__ __forceinline__ bool row_sectors(const void* base, int D) { return D % 16 == 0 && (reinterpret_cast<uintptr_t>(base) & 31) == 0; }
+
 // Rows from `from` on of an operand tile become zero (whole warp): the rows behind a sequence's end belong to its
 // neighbour or to nobody, and zero times whatever stands there need not be zero.
 template <int DP, int ROWS = kTile>
