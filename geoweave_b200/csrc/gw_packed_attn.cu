@@ -103,5 +103,5 @@ extern "C" int gw_packed_attn_bwd(const void* q, const void* k, const void* v, c
   if (total_q > 0 && (!workspace || workspace_bytes < gw_packed_attn_bwd_workspace_bytes(total_q, H))) return GW_ERR_WORKSPACE;
   p.delta = static_cast<float*>(workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == GW_F32 ? packed_plain_bwd(p, st) : packed_mma_bwd(p, dtype, dev, st);
+  return dtype == GW_F32 ? packed_plain_bwd(p, st) : packed_mma_bwd(p, dtype, dev, facts.sms, st);
 }

@@ -46,12 +46,12 @@ struct BwdShape {
 
 // Barriers, the block's tile and tensor memory; the same in both kernels.
 template <int DP>
-__device__ __forceinline__ uint32_t bwd_setup(BwdShared* sh, const PackedParams& p, bool key_side, int heads, int warp, int lane) {
+__device__ __forceinline__ uint32_t bwd_setup(BwdShared* sh, const PackedParams& p, bool key_side, int64_t rank, int warp, int lane) {
   using Shape = BwdShape<DP>;
   if (warp == Shape::kLoad) {
     PackedSeq s{};
     int64_t tiles = 0, end = 0;
-    const bool found = packed_find_sorted(p, key_side, kTile, blockIdx.x / heads, &s, &tiles, &end);
+    const bool found = packed_find_sorted(p, key_side, kTile, rank, &s, &tiles, &end);
     if (lane == 0) {
       sh->seq = s;
       sh->tiles = tiles;
@@ -79,15 +79,26 @@ __device__ __forceinline__ uint32_t bwd_setup(BwdShared* sh, const PackedParams&
 }
 
 // columns [from, to) of one row of an accumulator in this thread's TMEM lane, times mul, as 16-bit values (zeros if !any); `base` is
-// the tensor that the row `dst` belongs to
+// the tensor that the row `dst` belongs to; `more`, if any: values to be added, four columns every kTile
 template <typename T>
-__device__ __forceinline__ void store_acc(const void* base, T* dst, uint32_t addr, int from, int to, int D, float mul, bool live, bool any) {
+__device__ __forceinline__ void store_acc(const void* base, T* dst, uint32_t addr, int from, int to, int D, float mul, bool live, bool any,
+                                          const float4* more = nullptr) {
 #pragma unroll 1
   for (int b = from; b < to; b += 32) {
     if (b >= D) break;
     float o[32];
     tmem_load32(addr + b, o);  // without a product: whatever is there, and unused
     tmem_wait_ld();
+    if (more != nullptr) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float4 m = more[(b / 4 + c) * kTile];
+        o[4 * c] += m.x;
+        o[4 * c + 1] += m.y;
+        o[4 * c + 2] += m.z;
+        o[4 * c + 3] += m.w;
+      }
+    }
     uint32_t e[16];
 #pragma unroll
     for (int k = 0; k < 16; ++k) e[k] = any ? pack_half2<T>(o[2 * k] * mul, o[2 * k + 1] * mul) : 0u;
@@ -112,7 +123,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
   const int head = blockIdx.x % p.H, kv = head / (p.H / p.Hk);
-  const uint32_t tmem = bwd_setup<DP>(sh, p, false, p.H, warp, lane);
+  const uint32_t tmem = bwd_setup<DP>(sh, p, false, blockIdx.x / p.H, warp, lane);
   if (!sh->found) {
     packed_zero_rows<T>(p.dq, nullptr, sh->end, p.total_q, p.H, head, p.D, blockIdx.x / p.H - sh->tiles, gridDim.x / p.H - sh->tiles,
                         blockDim.x);
@@ -325,7 +336,15 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   if (warp == Shape::kIssue) tmem_dealloc(tmem, Shape::kColumns);
 }
 
-template <typename T, int DP>
+// The whole cluster meets, and what its blocks wrote before is there behind it.
+__device__ __forceinline__ void cluster_meet() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// BLOCKS blocks share the query tiles of one key tile: with two, a cluster, the second adds its sums to the first's at the end
+// through the first's shared memory (the first's part, then the second's: a fixed order).
+template <typename T, int DP, int BLOCKS>
 __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kBlocks)
 packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const __grid_constant__ CUtensorMap tmG, const PackedParams p, const int ab_format) {
@@ -346,10 +365,11 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
-  const int kv = blockIdx.x % p.Hk, group = p.H / p.Hk;
-  const uint32_t tmem = bwd_setup<DP>(sh, p, true, p.Hk, warp, lane);
+  const int64_t item = blockIdx.x / BLOCKS;
+  const int share = blockIdx.x % BLOCKS, kv = static_cast<int>(item % p.Hk), group = p.H / p.Hk;
+  const uint32_t tmem = bwd_setup<DP>(sh, p, true, item / p.Hk, warp, lane);
   if (!sh->found) {
-    const int64_t part = blockIdx.x / p.Hk - sh->tiles, parts = gridDim.x / p.Hk - sh->tiles;
+    const int64_t part = (item / p.Hk - sh->tiles) * BLOCKS + share, parts = (gridDim.x / BLOCKS / p.Hk - sh->tiles) * BLOCKS;
     packed_zero_rows<T>(p.dk, nullptr, sh->end, p.total_k, p.Hk, kv, p.D, part, parts, blockDim.x);
     packed_zero_rows<T>(p.dv, nullptr, sh->end, p.total_k, p.Hk, kv, p.D, part, parts, blockDim.x);
   } else {
@@ -359,7 +379,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int q_tiles = (s.lq + W - 1) / W;
     const int first = p.causal ? max(0, c0 - off) / W : 0;  // the first query tile that sees one of these keys
     const int per_head = max(0, q_tiles - first);
-    const int n = per_head * group;
+    const int all = per_head * group;                        // pairs of tiles
+    const int begin = share == 0 ? 0 : (all + 1) / BLOCKS;   // this block's: the first half, rounded up, or the rest
+    const int n = BLOCKS == 1 ? all : share == 0 ? (all + 1) / 2 : all / 2;
 
     if (warp == Shape::kLoad) {
       bool ok = true;
@@ -370,7 +392,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         load_rows<DP>(v_smem, &tmV, kv, s.k0 + c0, &sh->own_full);
       }
       for (; i < n; ++i) {
-        const int st = i % ST, head = kv * group + i / per_head, r0 = (first + i % per_head) * W;
+        const int st = i % ST, at = begin + i, head = kv * group + at / per_head, r0 = (first + at % per_head) * W;
         ok = mbar_wait_bounded(&sh->a_empty[st], ((i / ST) & 1u) ^ 1u);
         if (!ok || sh->abort_flag) break;
         if (lane == 0) {
@@ -414,7 +436,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       bool ok = n == 0 || mbar_wait_bounded(&sh->own_full, 0);
       // S^T = K Q^T / dP^T = V d_o^T of query tile i; rows behind the sequence's end become zeros first
       auto product = [&](int i, uint64_t* full, unsigned char* tiles, uint64_t a, uint64_t b, uint32_t d, uint64_t* done) {
-        const int st = i % ST, left = s.lq - (first + i % per_head) * W;
+        const int st = i % ST, left = s.lq - (first + (begin + i) % per_head) * W;
         ok = mbar_wait_bounded(&full[st], (i / ST) & 1);
         if (!ok) return;
         if (left < W) zero_rows_from<DP, W>(tiles + st * WB, left);
@@ -460,12 +482,11 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const int row = c0 + (warp & 3) * 32 + lane;
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t s_addr = tmem + lanes + kS + half * 64, d_addr = tmem + lanes + kDp + half * 64;
-      const bool live = row < s.lk;
       const float c = p.scale * kLog2e;
       const uint64_t c2 = pack_f2(c, c), lower2 = pack_f2(kLower, kLower);
       bool ok = true;
       for (int i = 0; i < n; ++i) {
-        const int st = i % ST, r0 = (first + i % per_head) * W;
+        const int st = i % ST, r0 = (first + (begin + i) % per_head) * W;
         const ulonglong2* l2 = reinterpret_cast<const ulonglong2*>(stats + st * 2 * W + half * 64);
         const ulonglong2* d2 = reinterpret_cast<const ulonglong2*>(stats + st * 2 * W + W + half * 64);
         const bool edge = p.causal && c0 + kTile - 1 > r0 + off;  // some pair of the tiles is masked
@@ -537,10 +558,43 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         report_status(p.status, GW_ERR_TIMEOUT);
       }
       tc_fence_after();
+    }
+
+    // ------------------------------ output: dv by the first four warps, dk by the last four ------------------------------
+    const int half = warp >> 2, r = (warp & 3) * 32 + lane, row = c0 + r;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    // the other block's sums, [dv, dk][DP / 4][128 rows], where the operand tiles were
+    float4* sums = reinterpret_cast<float4*>(k_smem);
+    if (BLOCKS == 2) {
+      cluster_meet();  // the first block's tiles have been used
+      if (share == 1 && warp < Shape::kLoad && n > 0) {
+        uint32_t remote;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(remote) : "r"(smem_u32(sums)));
+        for (int which = 0; which < 2; ++which) {
+          if (half != (which == 0 ? 0 : Shape::kHalves - 1)) continue;
+#pragma unroll 1
+          for (int b = 0; b < DP; b += 32) {
+            float o[32];
+            tmem_load32(tmem + lanes + (which == 0 ? kDv : kDk) + b, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote + (((which * (DP / 4) + b / 4 + c) * kTile + r) << 4)),
+                           "f"(o[4 * c]), "f"(o[4 * c + 1]), "f"(o[4 * c + 2]), "f"(o[4 * c + 3])
+                           : "memory");
+          }
+        }
+      }
+      cluster_meet();
+    }
+    if (share == 0 && warp < Shape::kLoad) {
+      const bool live = row < s.lk;
       const int64_t at = (static_cast<int64_t>(s.k0 + row) * p.Hk + kv) * p.D;
-      if (half == 0) store_acc<T>(p.dv, static_cast<T*>(p.dv) + at, tmem + lanes + kDv, 0, DP, p.D, kLower, live, n > 0);
+      const float4* more = BLOCKS == 2 && all > 1 ? sums + r : nullptr;
+      if (half == 0) store_acc<T>(p.dv, static_cast<T*>(p.dv) + at, tmem + lanes + kDv, 0, DP, p.D, kLower, live, all > 0, more);
       if (half == Shape::kHalves - 1)
-        store_acc<T>(p.dk, static_cast<T*>(p.dk) + at, tmem + lanes + kDk, 0, DP, p.D, p.scale, live, n > 0);
+        store_acc<T>(p.dk, static_cast<T*>(p.dk) + at, tmem + lanes + kDk, 0, DP, p.D, p.scale, live, all > 0,
+                     more != nullptr ? more + DP / 4 * kTile : nullptr);
     }
   }
   tc_fence_before();
@@ -550,7 +604,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 }
 
 template <typename T, int DP>
-int launch_bwd(const PackedParams& p, int dtype, int dev, cudaStream_t st) {
+int launch_bwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t st) {
   CUtensorMap mq, mk, mv, mg;
   GW_CUDA_TRY(cudaSetDevice(dev));  // a thread that has launched nothing yet has no context to encode tensor maps in
   // each tensor once as the side that a block owns and once as the side that it walks
@@ -564,27 +618,49 @@ int launch_bwd(const PackedParams& p, int dtype, int dev, cudaStream_t st) {
   };
   constexpr int W = BwdShape<DP>::kWalk, kThreads = BwdShape<DP>::kThreads;
   maps(kTile, W);
-  static OncePerDevice once_q, once_k;
+  static OncePerDevice once_q, once_k, once_k2;
   constexpr size_t smem = BwdShape<DP>::kSmem;
   if (rc == GW_OK) rc = ensure_dynamic_smem(packed_dq_kernel<T, DP>, smem, once_q, dev);
-  if (rc == GW_OK) rc = ensure_dynamic_smem(packed_dkv_kernel<T, DP>, smem, once_k, dev);
+  if (rc == GW_OK) rc = ensure_dynamic_smem(packed_dkv_kernel<T, DP, 1>, smem, once_k, dev);
+  if (rc == GW_OK) rc = ensure_dynamic_smem(packed_dkv_kernel<T, DP, 2>, smem, once_k2, dev);
   if (rc != GW_OK) return rc;
   const int format = dtype == GW_BF16 ? 1 : 0;
   const int64_t q_items = packed_tile_bound(p.total_q, kTile, p.nseq) * p.H, k_items = packed_tile_bound(p.total_k, kTile, p.nseq) * p.Hk;
-  if (q_items > 0x7fffffff || k_items > 0x7fffffff) return GW_ERR_UNSUPPORTED;
+  if (q_items > 0x7fffffff || k_items > 0x3fffffff) return GW_ERR_UNSUPPORTED;
   packed_dq_kernel<T, DP><<<static_cast<unsigned>(q_items), kThreads, smem, st>>>(mq, mk, mv, mg, p, format);
   GW_LAUNCH_CHECK();
   if (W != kTile && maps(W, kTile) != GW_OK) return rc;
-  packed_dkv_kernel<T, DP><<<static_cast<unsigned>(k_items), kThreads, smem, st>>>(mq, mk, mv, mg, p, format);
-  GW_LAUNCH_CHECK();
+  // Few and long blocks -- grouped heads, whose key tiles walk every head of the group -- leave SMs idle at the end: two share a key
+  // tile.  One sequence of 4099 tokens, 2 key heads of 64 under 16: 436 us against 676 for the whole training step; ragged
+  // prompts, 4 key heads of 128: 556 against 594.  Not for more than two and a half rounds of blocks (8328 tokens, 16 heads: 1590
+  // against 1563) nor for less than 24 pairs of tiles a block (views of 1041 tokens, 16 heads: 190 against 167).
+  const int64_t items = (p.total_k + kTile - 1) / kTile * p.Hk, at_once = static_cast<int64_t>(sms) * BwdShape<DP>::kBlocks;
+  const bool share = 2 * items < 5 * at_once && p.total_q * (p.H / p.Hk) >= 24 * static_cast<int64_t>(W) * p.nseq;
+  if (!share) {
+    packed_dkv_kernel<T, DP, 1><<<static_cast<unsigned>(k_items), kThreads, smem, st>>>(mq, mk, mv, mg, p, format);
+    GW_LAUNCH_CHECK();
+    return GW_OK;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * k_items));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute cluster = {};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = 2;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = 1;
+  GW_CUDA_TRY(cudaLaunchKernelEx(&cfg, packed_dkv_kernel<T, DP, 2>, mq, mk, mv, mg, p, format));
   return GW_OK;
 }
 
 }  // namespace
 
-int packed_mma_bwd(const PackedParams& p, int dtype, int dev, cudaStream_t st) {
-  if (dtype == GW_BF16) return p.D <= 64 ? launch_bwd<__nv_bfloat16, 64>(p, dtype, dev, st) : launch_bwd<__nv_bfloat16, 128>(p, dtype, dev, st);
-  return p.D <= 64 ? launch_bwd<__half, 64>(p, dtype, dev, st) : launch_bwd<__half, 128>(p, dtype, dev, st);
+int packed_mma_bwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t st) {
+  if (dtype == GW_BF16) return p.D <= 64 ? launch_bwd<__nv_bfloat16, 64>(p, dtype, dev, sms, st) : launch_bwd<__nv_bfloat16, 128>(p, dtype, dev, sms, st);
+  return p.D <= 64 ? launch_bwd<__half, 64>(p, dtype, dev, sms, st) : launch_bwd<__half, 128>(p, dtype, dev, sms, st);
 }
 
 }  // namespace gw

@@ -182,6 +182,16 @@ def test_gradients_against_differences():
         assert (along[0] - along[1]).abs() <= 2e-3 * (along[1].abs() + size * math.sqrt(d.numel()) * 0.5)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_rows_of_grouped_heads(D, causal):
+    """Few key tiles with many query tiles each, which two blocks share: even and odd numbers of pairs, one pair, none."""
+    _check([1600], [200], 8, 1, D, torch.bfloat16, causal, seed=50)
+    _check([1700, 1], [130, 300], 6, 2, D, torch.float16, causal, seed=51)
+    _check([2900, 64], [1, 700], 4, 2, D, torch.bfloat16, causal, seed=52)
+    _check([0, 3000], [90, 129], 4, 2, D, torch.float16, causal, seed=53, tail_k=300)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_runs_are_reproducible_and_a_graph_replays_with_other_borders(dtype):
     from geoweave_b200 import check_status
