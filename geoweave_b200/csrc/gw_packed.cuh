@@ -205,7 +205,8 @@ int packed_plain_fwd(const PackedParams& p, cudaStream_t st);
 int packed_plain_bwd(const PackedParams& p, cudaStream_t st);
 int packed_plain_split(const PackedParams& p, int chunk, int max_rows, int64_t slots, float* part_o, float* part_ml, cudaStream_t st);
 // 16-bit tensors (gw_packed_fwd.cu, gw_packed_bwd.cu)
-int packed_mma_fwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t st);
+size_t packed_mma_fwd_bytes(const PackedParams& p, int sms);
+int packed_mma_fwd(const PackedParams& p, int dtype, int dev, int sms, void* workspace, cudaStream_t st);
 int packed_mma_bwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t st);
 // few query rows, divided along the keys (gw_packed_split.cu)
 bool packed_split_fits(const PackedParams& p, int64_t max_q);

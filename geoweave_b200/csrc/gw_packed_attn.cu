@@ -38,17 +38,25 @@ PackedParams make_params(const void* q, const void* k, const void* v, const int3
 
 }  // namespace
 
-// Up to 16 rows (query rows x heads of a group) of a key head: the kernel that divides the keys, and its workspace.
+namespace {
+
+// Up to 16 rows (query rows x heads of a group) of a key head: the kernel for single tokens.  16-bit tensors of few rows: the keys
+// divided among blocks.  Both leave partial results (fp32) in the workspace.
+size_t fwd_bytes(const PackedParams& p, int dtype, int64_t max_q, int sms) {
+  if (packed_split_fits(p, max_q)) return packed_split_bytes(p, max_q, sms);
+  return dtype == GW_F32 ? 0 : packed_mma_fwd_bytes(p, sms);
+}
+
+}  // namespace
+
 extern "C" size_t gw_packed_attn_fwd_workspace_bytes(int dtype, int nseq, int64_t total_q, int64_t total_k, int H, int Hk, int D,
                                                      int64_t max_q) {
   if (nseq < 0 || total_q <= 0 || total_k < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || D <= 0 || D > 128) return 0;
-  (void)dtype;  // partial results are fp32 whatever the type
   PackedParams p{};
-  p.nseq = nseq; p.total_k = total_k; p.H = H; p.Hk = Hk; p.D = D;
+  p.nseq = nseq; p.total_q = total_q; p.total_k = total_k; p.H = H; p.Hk = Hk; p.D = D;
   int dev = 0;
   DeviceFacts facts;
-  if (!packed_split_fits(p, max_q) || device_facts(&dev, &facts) != GW_OK) return 0;
-  return packed_split_bytes(p, max_q, facts.sms);
+  return device_facts(&dev, &facts) == GW_OK ? fwd_bytes(p, dtype, max_q, facts.sms) : 0;
 }
 
 extern "C" int gw_packed_attn_fwd(const void* q, const void* k, const void* v, int dtype, const int32_t* cu_q, const int32_t* cu_k, int nseq,
@@ -66,11 +74,10 @@ extern "C" int gw_packed_attn_fwd(const void* q, const void* k, const void* v, i
   if (rc != GW_OK) return rc;
   if (total_q == 0) return GW_OK;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (packed_split_fits(p, max_q)) {
-    if (!workspace || !aligned16(workspace) || workspace_bytes < packed_split_bytes(p, max_q, facts.sms)) return GW_ERR_WORKSPACE;
-    return packed_split_fwd(p, dtype, max_q, dev, facts.sms, workspace, st);
-  }
-  return dtype == GW_F32 ? packed_plain_fwd(p, st) : packed_mma_fwd(p, dtype, dev, facts.sms, st);
+  const size_t need = fwd_bytes(p, dtype, max_q, facts.sms);
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return GW_ERR_WORKSPACE;
+  if (packed_split_fits(p, max_q)) return packed_split_fwd(p, dtype, max_q, dev, facts.sms, workspace, st);
+  return dtype == GW_F32 ? packed_plain_fwd(p, st) : packed_mma_fwd(p, dtype, dev, facts.sms, workspace, st);
 }
 
 extern "C" size_t gw_packed_attn_bwd_workspace_bytes(int64_t total_q, int H) {

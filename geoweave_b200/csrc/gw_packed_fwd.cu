@@ -66,9 +66,9 @@ struct FwdShape {
 
 enum { kItemRows, kItemTail, kItemEnd };
 struct FwdItem {  // the rows of a block, of one head; or some rows behind the last sequence; or the end of the list
-  int kind, head, q0, lq, k0, lk, r0;
+  int kind, head, part, q0, lq, k0, lk, off, r0;  // k0, lk: the keys that this item walks; query i sees those up to i + off
   int keys[kTiles], n[kTiles], most;  // keys that any row of each tile sees; key tiles of each, of both
-  int64_t part, parts, end;
+  int64_t slot, slots, end;
 };
 
 struct FwdShared {
@@ -87,10 +87,17 @@ __device__ __forceinline__ bool wait_item(FwdShared* sh, int i) {
   return mbar_wait_limit(&sh->item_full[i & 1], (i >> 1) & 1, 60 * kWaitLimitNs);
 }
 
+// Few rows against many keys: the key tiles of a row tile are divided among `count` items, which leave their unnormalised sums
+struct FwdParts {
+  int count;   // 1: not divided
+  float* o;    // [H, count, total_q, D]
+  float2* ml;  // [H, count, total_q]: maximum of scale log2 e S, sum
+};
+
 template <typename T, int DP, int TILES>
 __global__ void __launch_bounds__(FwdShape<DP, TILES>::kThreads, 1)
 packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                  const PackedParams p, const int64_t slots, const int ab_format) {
+                  const PackedParams p, const int64_t slots, const FwdParts fp, const int ab_format) {
   using Shape = FwdShape<DP, TILES>;
   constexpr int ST = Shape::kStages, TB = Shape::kTileBytes, NI = Shape::kIssuers;
   constexpr int kWarps = Shape::kWarps, kLoad = Shape::kLoad, kIssue = Shape::kIssue;
@@ -139,8 +146,10 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     int i = 0, told = 0;                    // items, and those of them that the others have been told of
     for (int64_t at = blockIdx.x; ok && !sh->abort_flag; at += gridDim.x, ++i) {
       FwdItem w{};
-      w.head = static_cast<int>(at % p.H);
-      const int64_t rank = at / p.H;
+      const int parts = TILES == 1 ? fp.count : 1;
+      w.part = static_cast<int>(at % parts);
+      w.head = static_cast<int>(at / parts % p.H);
+      const int64_t rank = at / parts / p.H;
       PackedSeq seq{};
       int64_t tiles = 0;
       if (rank >= slots) {
@@ -151,18 +160,27 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         w.lq = seq.lq;
         w.k0 = seq.k0;
         w.lk = seq.lk;
+        w.off = seq.lk - seq.lq;
         w.r0 = seq.tile * TILES * kTile;
+        if (parts > 1) {  // this part's run of key tiles, out of those that the tile's last row sees
+          const int last = min(w.r0 + kTile, w.lq), seen = p.causal ? max(0, min(w.lk, last + w.off)) : w.lk;
+          const int each = ((seen + kTile - 1) / kTile + parts - 1) / parts;
+          const int from = static_cast<int>(min(static_cast<int64_t>(w.part) * each * kTile, static_cast<int64_t>(seen)));
+          w.k0 += from;
+          w.lk = static_cast<int>(min(static_cast<int64_t>(each) * kTile, static_cast<int64_t>(seen - from)));
+          w.off -= from;
+        }
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
           const int last = min(w.r0 + (t + 1) * kTile, w.lq);
-          w.keys[t] = last <= w.r0 + t * kTile ? 0 : p.causal ? max(0, min(w.lk, last + w.lk - w.lq)) : w.lk;
+          w.keys[t] = last <= w.r0 + t * kTile ? 0 : p.causal ? max(0, min(w.lk, last + w.off)) : w.lk;
           w.n[t] = (w.keys[t] + kTile - 1) / kTile;
           w.most = max(w.most, w.n[t]);
         }
       } else {
         w.kind = kItemTail;
-        w.part = rank - tiles;
-        w.parts = slots - tiles;
+        w.slot = (rank - tiles) * parts + w.part;
+        w.slots = (slots - tiles) * parts;
       }
       ok = mbar_wait_bounded(&sh->item_empty[i & 1], ((i >> 1) & 1) ^ 1);
       if (!ok) break;
@@ -337,12 +355,12 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const int kind = item->kind;
       if (kind == kItemEnd) break;
       if (kind == kItemTail) {
-        packed_zero_rows<T>(p.o, p.lse, item->end, p.total_q, p.H, item->head, p.D, item->part, item->parts, kWarps * 32);
+        packed_zero_rows<T>(p.o, p.lse, item->end, p.total_q, p.H, item->head, p.D, item->slot, item->slots, kWarps * 32);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->item_empty[i & 1]);
         continue;
       }
-      const int lk = item->lk, off = lk - item->lq, first = item->r0 + t * kTile, row = first + (warp & 3) * 32 + lane;
+      const int lk = item->lk, off = item->off, first = item->r0 + t * kTile, row = first + (warp & 3) * 32 + lane;
       const int limit = p.causal ? min(lk, row + off + 1) : lk;   // keys this row sees
       const int open = p.causal ? min(lk, first + off + 1) : lk;  // keys that every row of the tile sees
       const int tiles = item->n[t];
@@ -435,6 +453,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const bool live = row < item->lq;
       const int64_t token = item->q0 + row;
       const int head = item->head;
+      const int64_t part_row = TILES == 1 ? (static_cast<int64_t>(head) * fp.count + item->part) * p.total_q + token : 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->item_empty[i & 1]);
       const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -446,6 +465,15 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         float o[32];
         tmem_load32(o_addr + 32 * b, o);  // without a key: whatever is there, and unused
         tmem_wait_ld();
+        if (TILES == 1 && fp.count > 1) {
+          if (live) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (32 * b + 4 * k < p.D)
+                reinterpret_cast<float4*>(fp.o + part_row * p.D)[8 * b + k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          }
+          continue;
+        }
         uint32_t e[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) e[k] = l == 0.f ? 0u : pack_half2<T>(o[2 * k] * inv, o[2 * k + 1] * inv);
@@ -461,6 +489,10 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
       }
       tc_fence_before();  // O may be written again once this item's successor has its first P
+      if (TILES == 1 && fp.count > 1) {
+        if (live) fp.ml[part_row] = make_float2(m * c, l);
+        continue;
+      }
       if (live && p.lse != nullptr)
         p.lse[head * p.total_q + token] = l == 0.f ? -INFINITY : fmaf(m, p.scale, log2f(l) * kLn2);
     }
@@ -476,8 +508,50 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   if (warp == kIssue) tmem_dealloc(tmem, 512);
 }
 
+// Joins the parts of a row (a warp a row): o = sum o_i 2^(m_i - m) / sum l_i 2^(m_i - m)
+template <typename T>
+__global__ void __launch_bounds__(256) packed_join_kernel(const PackedParams p, const FwdParts fp) {
+  const int lane = threadIdx.x & 31, col = lane * 4;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5), token = row / p.H;
+  const int head = static_cast<int>(row % p.H);
+  // rows behind the last sequence are zeros already
+  if (token >= p.total_q || p.nseq == 0 || token >= packed_border(p.cu_q, p.nseq, p.total_q)) return;
+  const int64_t first = static_cast<int64_t>(head) * fp.count * p.total_q + token;
+  const float2 ml = lane < fp.count ? fp.ml[first + lane * p.total_q] : make_float2(-INFINITY, 0.f);
+  const float m = [&] {
+    float x = ml.y > 0.f || ml.y != ml.y ? ml.x : -INFINITY;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    return x;
+  }();
+  const float weight = ml.y == 0.f ? 0.f : exp2f(ml.x - m);
+  float l = ml.y * weight;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < fp.count; ++i) {
+    const float f = __shfl_sync(0xffffffffu, weight, i);
+    if (f == 0.f || col >= p.D) continue;  // a part without a key left nothing
+    const float4 o = *reinterpret_cast<const float4*>(fp.o + (first + i * p.total_q) * p.D + col);
+    acc[0] = fmaf(o.x, f, acc[0]);
+    acc[1] = fmaf(o.y, f, acc[1]);
+    acc[2] = fmaf(o.z, f, acc[2]);
+    acc[3] = fmaf(o.w, f, acc[3]);
+  }
+  const int64_t at = (token * p.H + head) * p.D + col;
+  if (col < p.D)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = l == 0.f ? 0.f : acc[i] / l;
+      const T rounded = from_float<T>(x);
+      static_cast<T*>(p.o)[at + i] = rounded;
+      if (p.o_low != nullptr) static_cast<T*>(p.o_low)[at + i] = from_float<T>(x - to_float(rounded));
+    }
+  if (lane == 0 && p.lse != nullptr) p.lse[head * p.total_q + token] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
 template <typename T, int DP, int TILES>
-int launch_fwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t st) {
+int launch_fwd(const PackedParams& p, int dtype, int dev, int sms, int parts, void* workspace, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
   GW_CUDA_TRY(cudaSetDevice(dev));  // a thread that has launched nothing yet has no context to encode tensor maps in
   int rc = make_token_map(&mq, p.q, dtype, p.total_q, p.H, p.D, p.qs[0], p.qs[1], kTile);
@@ -487,27 +561,55 @@ int launch_fwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t 
   static OncePerDevice once;
   if (rc == GW_OK) rc = ensure_dynamic_smem(packed_fwd_kernel<T, DP, TILES>, Shape::kSmem, once, dev);
   if (rc != GW_OK) return rc;
-  const int64_t slots = packed_tile_bound(p.total_q, TILES * kTile, p.nseq), items = slots * p.H;
+  const int64_t slots = packed_tile_bound(p.total_q, TILES * kTile, p.nseq), items = slots * p.H * parts;
+  FwdParts fp{parts, static_cast<float*>(workspace), nullptr};
+  fp.ml = reinterpret_cast<float2*>(fp.o + (parts > 1 ? static_cast<int64_t>(p.H) * parts * p.total_q * p.D : 0));
   packed_fwd_kernel<T, DP, TILES><<<static_cast<unsigned>(items < sms ? items : sms), Shape::kThreads, Shape::kSmem, st>>>(
-      mq, mk, mv, p, slots, dtype == GW_BF16 ? 1 : 0);
+      mq, mk, mv, p, slots, fp, dtype == GW_BF16 ? 1 : 0);
   GW_LAUNCH_CHECK();
+  if (parts > 1) {
+    packed_join_kernel<T><<<static_cast<unsigned>((p.total_q * p.H + 7) / 8), 256, 0, st>>>(p, fp);
+    GW_LAUNCH_CHECK();
+  }
   return GW_OK;
 }
 
+// Rows for fewer blocks of two tiles than there are SMs: one tile a block, twice the blocks (one view of 1041 tokens, 16 heads: 20.5 us
+// against 26.6; 1041 rows against 33 312 keys: 274 against 379).  With three views the two are equal, with 32 two tiles
+// win, 269 us against 340, since both share every key tile.
+bool few_rows(const PackedParams& p, int sms) { return (p.total_q + 2 * kTile - 1) / (2 * kTile) * p.H < sms; }
+
+// Fewer row tiles than half the SMs, and keys enough for at least six key tiles a part: the keys are divided too (300 rows, 8 heads
+// against 8328 keys: 30 us against 78; 1041 rows, 4 heads against 33 312: 88 against 274).  With nine key tiles in two parts
+// the second kernel costs what they bring (23.6 against 20.5).
+int key_parts(const PackedParams& p, int sms) {
+  int64_t tiles = (p.total_q + kTile - 1) / kTile;
+  if (tiles < p.nseq) tiles = p.nseq;  // each sequence has a tile of its own
+  if (p.nseq == 0 || tiles * p.H * 2 > sms) return 1;
+  int64_t parts = sms / (tiles * p.H);
+  const int64_t run = p.total_k / p.nseq / (6 * kTile);
+  if (parts > run) parts = run;
+  return static_cast<int>(parts < 2 ? 1 : parts > 16 ? 16 : parts);
+}
+
 template <typename T>
-int choose_fwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t st) {
-  // Rows for fewer blocks of two tiles than there are SMs: one tile a block, twice the blocks (one view of 1041 tokens, 16 heads: 20.5 us
-  // against 26.6; 1041 rows against 33 312 keys: 274 against 379).  With three views the two are equal, with 32 two tiles
-  // win, 269 us against 340, since both share every key tile.
-  const bool few = (p.total_q + 2 * kTile - 1) / (2 * kTile) * p.H < sms;
-  if (p.D <= 64) return few ? launch_fwd<T, 64, 1>(p, dtype, dev, sms, st) : launch_fwd<T, 64, 2>(p, dtype, dev, sms, st);
-  return few ? launch_fwd<T, 128, 1>(p, dtype, dev, sms, st) : launch_fwd<T, 128, 2>(p, dtype, dev, sms, st);
+int choose_fwd(const PackedParams& p, int dtype, int dev, int sms, void* workspace, cudaStream_t st) {
+  const bool few = few_rows(p, sms);
+  const int parts = few ? key_parts(p, sms) : 1;
+  if (p.D <= 64)
+    return few ? launch_fwd<T, 64, 1>(p, dtype, dev, sms, parts, workspace, st) : launch_fwd<T, 64, 2>(p, dtype, dev, sms, 1, nullptr, st);
+  return few ? launch_fwd<T, 128, 1>(p, dtype, dev, sms, parts, workspace, st) : launch_fwd<T, 128, 2>(p, dtype, dev, sms, 1, nullptr, st);
 }
 
 }  // namespace
 
-int packed_mma_fwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t st) {
-  return dtype == GW_BF16 ? choose_fwd<__nv_bfloat16>(p, dtype, dev, sms, st) : choose_fwd<__half>(p, dtype, dev, sms, st);
+size_t packed_mma_fwd_bytes(const PackedParams& p, int sms) {
+  const int parts = few_rows(p, sms) ? key_parts(p, sms) : 1;
+  return parts > 1 ? static_cast<size_t>(p.H) * parts * p.total_q * (p.D + 2) * 4 : 0;
+}
+
+int packed_mma_fwd(const PackedParams& p, int dtype, int dev, int sms, void* workspace, cudaStream_t st) {
+  return dtype == GW_BF16 ? choose_fwd<__nv_bfloat16>(p, dtype, dev, sms, workspace, st) : choose_fwd<__half>(p, dtype, dev, sms, workspace, st);
 }
 
 }  // namespace gw

@@ -183,6 +183,17 @@ def test_gradients_against_differences():
 
 
 @pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float16, 128), (torch.bfloat16, 24), (torch.float32, 64)])
+def test_a_few_hundred_rows_against_long_key_sequences(dtype, D, causal):
+    """The keys of a row tile are divided among blocks: parts that end inside a tile, rows that see only the first parts or none, a
+    sequence that is shorter than its neighbours' parts, rows behind the last sequence."""
+    _check([130], [5003], 4, 2, D, dtype, causal, seed=60, train=True)
+    _check([300, 17], [4100, 9], 2, 1, D, dtype, causal, seed=61, tail_q=200, tail_k=90)
+    _check([700, 40, 1], [600, 2600, 3000], 2, 2, D, dtype, causal, seed=62)
+    _check([20, 0], [0, 6000], 1, 1, D, dtype, causal, seed=63, train=False)
+
+
+@pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("D", [64, 128])
 def test_long_rows_of_grouped_heads(D, causal):
     """Few key tiles with many query tiles each, which two blocks share: even and odd numbers of pairs, one pair, none."""
