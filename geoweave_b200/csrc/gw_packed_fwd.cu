@@ -72,7 +72,7 @@ struct FwdItem {  // the rows of a block, of one head; or some rows behind the l
 };
 
 struct FwdShared {
-  uint64_t q_full[kTiles], q_empty[kTiles], s_full[kTiles], s_read[kTiles], p_full[kTiles], o_done[kTiles];
+  uint64_t q_full[kTiles], q_empty[kTiles], s_full[kTiles], s_read[kTiles], p_half[kTiles], p_full[kTiles], o_done[kTiles];
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
   uint64_t item_full[2], item_empty[2];
   FwdItem item[2];
@@ -116,6 +116,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       mbar_init(&sh->q_empty[i], 1);
       mbar_init(&sh->s_full[i], 1);
       mbar_init(&sh->s_read[i], 4);
+      mbar_init(&sh->p_half[i], 4);
       mbar_init(&sh->p_full[i], 4);
       mbar_init(&sh->o_done[i], 1);
     }
@@ -301,18 +302,35 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             if (ok && (j + 1) * kTile > lk) zero_rows_from<DP>(v_smem + st * TB, lk - j * kTile);
             v_here = true;
           }
+          const int steps = min(kTile, (keys[t] - j * kTile + 15) & ~15) / 16;
+          const uint32_t oa = tmem + Shape::kO + t * DP, pa = tmem + Shape::kP + t * Shape::kPStride;
+          const uint64_t va = vd + st * (TB >> 4);
+          // Wide heads: the product over the first half of P runs while the second is being made (a row's O has been rescaled
+          // before either half): 16 384 tokens, 16 heads 1811 -> 1782 us, two causal sequences of 3000, 100 rows each 33.5 -> 31.8 us.
+          // For narrow heads it is the exponentials that bound the kernel.
+          if (DP != 64) {
+            ok = ok && mbar_wait_bounded(&sh->p_half[t], c & 1);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              if (steps >= 4) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tc_mma_f16_ts(oa, pa + k * 8, va + k * (16 * 128 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+              } else {
+                for (int k = 0; k < steps; ++k) tc_mma_f16_ts(oa, pa + k * 8, va + k * (16 * 128 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+              }
+            }
+          }
           ok = ok && mbar_wait_bounded(&sh->p_full[t], c & 1);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
-            const int steps = min(kTile, (keys[t] - j * kTile + 15) & ~15) / 16;
-            const uint32_t oa = tmem + Shape::kO + t * DP, pa = tmem + Shape::kP + t * Shape::kPStride;
-            const uint64_t va = vd + st * (TB >> 4);
+            constexpr int from = DP != 64 ? 4 : 0;
             if (steps == 8) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k) tc_mma_f16_ts(oa, pa + k * 8, va + k * (16 * 128 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+              for (int k = from; k < 8; ++k) tc_mma_f16_ts(oa, pa + k * 8, va + k * (16 * 128 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
             } else {
-              for (int k = 0; k < steps; ++k) tc_mma_f16_ts(oa, pa + k * 8, va + k * (16 * 128 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+              for (int k = from; k < steps; ++k) tc_mma_f16_ts(oa, pa + k * 8, va + k * (16 * 128 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
             }
             tc_commit(&sh->o_done[t]);
           }
@@ -419,14 +437,27 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const uint64_t c2 = pack_f2(c, c), base2 = pack_f2(base, base);
         uint64_t sum[2] = {0, 0};
         uint32_t pk[64];
+        auto exponentials = [&](int from, int to) {
 #pragma unroll
-        for (int k = 0; k < 64; ++k) {
-          float a, b;
-          unpack_f2(fma_f2(pack_f2(x[2 * k], x[2 * k + 1]), c2, base2), a, b);
-          a = exp2_fast(a);
-          b = exp2_fast(b);
-          sum[k & 1] = add_f2(sum[k & 1], pack_f2(a, b));
-          pk[k] = pack_half2<T>(a, b);
+          for (int k = from; k < to; ++k) {
+            float a, b;
+            unpack_f2(fma_f2(pack_f2(x[2 * k], x[2 * k + 1]), c2, base2), a, b);
+            a = exp2_fast(a);
+            b = exp2_fast(b);
+            sum[k & 1] = add_f2(sum[k & 1], pack_f2(a, b));
+            pk[k] = pack_half2<T>(a, b);
+          }
+        };
+        if (DP != 64) {  // wide heads: the tensor cores may begin with the first half of P
+          exponentials(0, 32);
+          tmem_store32(p_addr, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh->p_half[t]);
+          exponentials(32, 64);
+        } else {
+          exponentials(0, 64);
         }
         float s0, s1, s2, s3;
         unpack_f2(sum[0], s0, s1);
@@ -437,7 +468,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           if (!ok) break;
           tc_fence_after();
         }
-        tmem_store32(p_addr, pk);
+        if (DP == 64) tmem_store32(p_addr, pk);
         tmem_store32(p_addr + 32, pk + 32);
         tmem_wait_st();
         tc_fence_before();
