@@ -39,13 +39,15 @@ struct BwdShape {
   static constexpr int kThreads = (kIssue + 1) * 32;
   static constexpr int kBlocks = DP == 64 ? 2 : 1;
   // Rings of the walked side: kStages in the key-side kernel (q, d_o); in the query-side kernel K stays until dq has used it and V
-  // only until dP is made.  At head dim 128, two stages of each against three and one, a training step: 7 prompts of 45 to 4099
-  // tokens, 4 key heads 558 -> 538 us; 8328 tokens, 16 heads 2558 -> 2397 us.
-  static constexpr int kStages = DP == 64 ? 4 : 2, kStagesK = DP == 64 ? 4 : 3, kStagesV = DP == 64 ? 4 : 1;
-  static_assert(kStagesK + kStagesV == 2 * kStages, "one size for both kernels");
+  // only until dP is made.  At head dim 128, two stages of each against three of K and two of V, a training step: 7 prompts of 45 to
+  // 4099 tokens, 4 key heads 558 -> 515 us; 8328 tokens, 16 heads 2558 -> 2166 us.  (Three and one: 538, 2400.)
+  static constexpr int kStages = DP == 64 ? 4 : 2, kStagesK = DP == 64 ? 4 : 3, kStagesV = DP == 64 ? 4 : 2;
   static constexpr int kOwnBytes = DP / 64 * kBoxBytes, kWalkBytes = kWalk * DP * 2;
   static constexpr uint32_t kColumns = DP == 64 ? 256 : 512;
-  static constexpr size_t kSmem = 1024 + 2 * kOwnBytes + static_cast<size_t>(2 * kStages) * kWalkBytes + sizeof(BwdShared) + kStages * 2 * kWalk * 4;
+  static constexpr size_t kSmemBase = 1024 + 2 * kOwnBytes + sizeof(BwdShared);
+  static constexpr size_t kSmemQ = kSmemBase + static_cast<size_t>(kStagesK + kStagesV) * kWalkBytes;  // query-side kernel
+  static constexpr size_t kSmem = kSmemBase + static_cast<size_t>(2 * kStages) * kWalkBytes + kStages * 2 * kWalk * 4;  // key side: rows' sums
+  static_assert(kSmem <= 232448 && kSmemQ <= 232448, "227 KB");
 };
 
 // Barriers, the block's tile and tensor memory; the same in both kernels.
@@ -115,7 +117,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kBlocks)
 packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                  const __grid_constant__ CUtensorMap tmG, const PackedParams p, const int ab_format) {
   using Shape = BwdShape<DP>;
-  constexpr int SK = Shape::kStagesK, SV = Shape::kStagesV, LEAD = SK > SV ? SK - 1 : 1;  // key tiles by which K runs ahead of V
+  constexpr int SK = Shape::kStagesK, SV = Shape::kStagesV;  // key tiles by which K runs ahead of V
   constexpr int TB = Shape::kOwnBytes, W = Shape::kWalk, WB = Shape::kWalkBytes;
   constexpr uint32_t kS = 0, kDp = W, kDs = 2 * W, kDq = Shape::kColumns - DP;
   extern __shared__ unsigned char smem_raw[];
@@ -143,26 +145,21 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (lane == 0 && n > 0) {
         bool ok = true;
         int jk = 0, jv = 0;  // key tiles whose K and V have been asked for
-        auto load_k = [&]() {
-          const int st = jk % SK;
-          ok = ok && mbar_wait_bounded(&sh->a_empty[st], ((jk / SK) & 1u) ^ 1u);
-          if (!ok || sh->abort_flag) return;
-          mbar_arrive_expect_tx(&sh->a_full[st], WB);
-          load_rows<DP, W>(k_smem + st * WB, &tmK, kv, s.k0 + jk * W, &sh->a_full[st]);
-          ++jk;
-        };
         mbar_arrive_expect_tx(&sh->own_full, 2 * TB);
         load_rows<DP>(q_smem, &tmQ, head, s.q0 + r0, &sh->own_full);
         load_rows<DP>(g_smem, &tmG, head, s.q0 + r0, &sh->own_full);
-        while (jk < n && jk < LEAD && ok && !sh->abort_flag) load_k();
-        while (jv < n && ok && !sh->abort_flag) {
-          const int st = jv % SV;
-          ok = mbar_wait_bounded(&sh->b_empty[st], ((jv / SV) & 1u) ^ 1u);
+        while (jk < n) {  // V first: in the order in which stages come back, dP(j + 1) before dq(j)
+          const int sv = jv % SV, sk = jk % SK;
+          ok = mbar_wait_bounded(&sh->b_empty[sv], ((jv / SV) & 1u) ^ 1u);
           if (!ok || sh->abort_flag) break;
-          mbar_arrive_expect_tx(&sh->b_full[st], WB);
-          load_rows<DP, W>(v_smem + st * WB, &tmV, kv, s.k0 + jv * W, &sh->b_full[st]);
+          mbar_arrive_expect_tx(&sh->b_full[sv], WB);
+          load_rows<DP, W>(v_smem + sv * WB, &tmV, kv, s.k0 + jv * W, &sh->b_full[sv]);
           ++jv;
-          if (jk < n) load_k();
+          ok = mbar_wait_bounded(&sh->a_empty[sk], ((jk / SK) & 1u) ^ 1u);
+          if (!ok || sh->abort_flag) break;
+          mbar_arrive_expect_tx(&sh->a_full[sk], WB);
+          load_rows<DP, W>(k_smem + sk * WB, &tmK, kv, s.k0 + jk * W, &sh->a_full[sk]);
+          ++jk;
         }
         if (!ok) sh->abort_flag = 1;
         if (sh->abort_flag) {  // let the copies in flight land before the shared memory is given up
@@ -631,15 +628,15 @@ int launch_bwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t 
   constexpr int W = BwdShape<DP>::kWalk, kThreads = BwdShape<DP>::kThreads;
   maps(kTile, W);
   static OncePerDevice once_q, once_k, once_k2;
-  constexpr size_t smem = BwdShape<DP>::kSmem;
-  if (rc == GW_OK) rc = ensure_dynamic_smem(packed_dq_kernel<T, DP>, smem, once_q, dev);
+  constexpr size_t smem_q = BwdShape<DP>::kSmemQ, smem = BwdShape<DP>::kSmem;
+  if (rc == GW_OK) rc = ensure_dynamic_smem(packed_dq_kernel<T, DP>, smem_q, once_q, dev);
   if (rc == GW_OK) rc = ensure_dynamic_smem(packed_dkv_kernel<T, DP, 1>, smem, once_k, dev);
   if (rc == GW_OK) rc = ensure_dynamic_smem(packed_dkv_kernel<T, DP, 2>, smem, once_k2, dev);
   if (rc != GW_OK) return rc;
   const int format = dtype == GW_BF16 ? 1 : 0;
   const int64_t q_items = packed_tile_bound(p.total_q, kTile, p.nseq) * p.H, k_items = packed_tile_bound(p.total_k, kTile, p.nseq) * p.Hk;
   if (q_items > 0x7fffffff || k_items > 0x3fffffff) return GW_ERR_UNSUPPORTED;
-  packed_dq_kernel<T, DP><<<static_cast<unsigned>(q_items), kThreads, smem, st>>>(mq, mk, mv, mg, p, format);
+  packed_dq_kernel<T, DP><<<static_cast<unsigned>(q_items), kThreads, smem_q, st>>>(mq, mk, mv, mg, p, format);
   GW_LAUNCH_CHECK();
   if (W != kTile && maps(W, kTile) != GW_OK) return rc;
   // Few and long blocks -- grouped heads, whose key tiles walk every head of the group -- leave SMs idle at the end: two share a key
