@@ -12,6 +12,8 @@
 // make P and dS in registers (a thread owns a row of its 64 columns) and put them back into tensor memory as 16-bit A operands of
 // the accumulating products, whose B operand is the tile that is in shared memory already, read along its rows.  The key-side
 // kernel works on the transposes (rows are keys), so neither P nor dS is ever transposed.
+#include <type_traits>
+
 #include "gw_packed_mma.cuh"
 
 namespace gw {
@@ -20,10 +22,12 @@ namespace {
 struct BwdShared {
   uint64_t own_full, s_full, dp_full, s_read, dp_read, p_full, ds_full, ds_done, all_done;
   uint64_t a_full[4], a_empty[4], b_full[4], b_empty[4], st_full[4];
+  uint64_t top_full[4];  // fp16, wide heads: both warps of a row have left their exponents
   PackedSeq seq;
   int64_t tiles, end;
   int found;
   float part[2][kTile];  // the two halves' sums of d_o * o
+  uint8_t top[2][2][kTile];  // [tile & 1][half][row]: biased exponent of the largest raised |dS|
   uint32_t tmem_base;
   volatile int abort_flag;
 };
@@ -50,6 +54,55 @@ struct BwdShape {
   static_assert(kSmem <= 232448 && kSmemQ <= 232448, "227 KB");
 };
 
+// dS as an fp16 operand.  It is as small as P times the incoming gradient, and fp16 has 15 powers of two below 1 (10 more with
+// ever fewer bits) and 15 above: with d_o of 1e-3 a fifth of 8328 keys' dS became zero (dq off by 0.58 % of its norm, 0.05 % with the
+// result rounded alone), and beyond 65 504 it was infinite.  So each row of the A operand, and with it the row's sums in tensor memory, is
+// raised by a power of two of its own: at first 2^40; whenever a tile's largest value passes 2^15, the row's power falls so that this
+// value lies at 2^7, and the sums so far are lowered to match.  What fp16 then takes off is 2^-11 of a value, or 2^-32 of the row's
+// largest.  A multiplication by a power of two is exact, and so is the way back in fp32 at the end.  bf16 has fp32's range.
+// Cost: the largest of 64 values a thread and tile (wide heads: an exponent shared by the two warps of a row); an fp16 training step of
+// 8328 tokens, 16 heads of 64 1589 -> 1634 us, of 128 2214 -> 2293; ragged prompts, 4 key heads of 128 517 -> 541.
+template <typename T>
+constexpr bool kRaised = std::is_same<T, __half>::value;
+constexpr int kFirstLift = 40, kGoal = 7, kMost = 15;
+
+// Whole warp, behind the tile's masks: 64 of the row's values, raised by 2^lift.  Returns what they and the sums must be multiplied with
+// (1 as a rule), and lowers `lift` to match.
+template <int HALVES>
+__device__ __forceinline__ float lift_row(const float (&x)[64], int& lift, bool live, BwdShared* sh, int half, int row, int tile, bool& ok) {
+  float top[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 64; i += 4)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fabsf(x[i + e]));
+  int exponent = static_cast<int>(__float_as_uint(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))) >> 23);
+  if (HALVES == 2) {
+    sh->top[tile & 1][half][row] = static_cast<uint8_t>(exponent);
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&sh->top_full[row >> 5]);
+    ok = ok && mbar_wait_bounded(&sh->top_full[row >> 5], tile & 1);
+    exponent = max(exponent, static_cast<int>(sh->top[tile & 1][half ^ 1][row]));
+  }
+  // infinite values stay what they are; rows behind the sequence hold its neighbour's and are not stored
+  if (!live || exponent == 255 || exponent < 127 + kMost) return 1.f;
+  lift += 127 + kGoal - exponent;
+  return __int_as_float((127 + 127 + kGoal - exponent) << 23);
+}
+
+// Columns [from, to) of the row's sums in tensor memory times f
+__device__ __forceinline__ void scale_sums(uint32_t addr, int from, int to, float f) {
+#pragma unroll 1
+  for (int b = from; b < to; b += 8) {
+    uint32_t o[8];
+    tmem_ld_x8(addr + b, o);
+    tmem_wait_ld();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+    tmem_store8(addr + b, o);
+  }
+  tmem_wait_st();
+}
+
 // Barriers, the block's tile and tensor memory; the same in both kernels.
 template <int DP>
 __device__ __forceinline__ uint32_t bwd_setup(BwdShared* sh, const PackedParams& p, bool key_side, int64_t rank, int warp, int lane) {
@@ -71,6 +124,7 @@ __device__ __forceinline__ uint32_t bwd_setup(BwdShared* sh, const PackedParams&
         mbar_init(&sh->b_full[i], 1);
         mbar_init(&sh->b_empty[i], 1);
         mbar_init(&sh->st_full[i], 1);
+        mbar_init(&sh->top_full[i], 2);
       }
       sh->abort_flag = 0;
       mbar_fence_init();
@@ -84,17 +138,19 @@ __device__ __forceinline__ uint32_t bwd_setup(BwdShared* sh, const PackedParams&
   return __shfl_sync(0xffffffffu, sh->tmem_base, 0);
 }
 
-// columns [from, to) of one row of an accumulator in this thread's TMEM lane, times mul, as 16-bit values (zeros if !any); `base` is
-// the tensor that the row `dst` belongs to; `more`, if any: values to be added, four columns every kTile
+// columns [from, to) of one row of an accumulator in this thread's TMEM lane, times lower, then times mul, as 16-bit values (zeros if
+// !any); `base` is the tensor that the row `dst` belongs to; `more`, if any: values to be added in between, four columns every kTile
 template <typename T>
-__device__ __forceinline__ void store_acc(const void* base, T* dst, uint32_t addr, int from, int to, int D, float mul, bool live, bool any,
-                                          const float4* more = nullptr) {
+__device__ __forceinline__ void store_acc(const void* base, T* dst, uint32_t addr, int from, int to, int D, float lower, float mul, bool live,
+                                          bool any, const float4* more = nullptr) {
 #pragma unroll 1
   for (int b = from; b < to; b += 32) {
     if (b >= D) break;
     float o[32];
     tmem_load32(addr + b, o);  // without a product: whatever is there, and unused
     tmem_wait_ld();
+#pragma unroll
+    for (int k = 0; k < 32; ++k) o[k] *= lower;
     if (more != nullptr) {
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
@@ -271,7 +327,9 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       if (live && half == 0) p.delta[at] = delta;
       const float c = p.scale * kLog2e;
-      const uint64_t c2 = pack_f2(c, c), l2 = pack_f2(neg_lse, neg_lse), nd2 = pack_f2(-delta, -delta);
+      int lift = kRaised<T> ? kFirstLift : 0;
+      const uint64_t c2 = pack_f2(c, c), nd2 = pack_f2(-delta, -delta);
+      uint64_t l2 = pack_f2(neg_lse + lift, neg_lse + lift);
       const int limit = (p.causal ? min(s.lk, row + off + 1) : s.lk) - half * 64;
       const int open = p.causal ? min(s.lk, r0 + off + 1) : s.lk;
       for (int j = 0; j < n; ++j) {
@@ -311,6 +369,21 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
           for (int i = 0; i < 64; ++i) x[i] = i < valid ? x[i] : 0.f;
         }
+        if constexpr (kRaised<T>) {
+          const float f = lift_row<Shape::kHalves>(x, lift, live, sh, half, (warp & 3) * 32 + lane, j, ok);
+          if (!ok) break;
+          if (__any_sync(0xffffffffu, f != 1.f)) {
+            l2 = pack_f2(neg_lse + lift, neg_lse + lift);
+#pragma unroll
+            for (int i = 0; i < 64; ++i) x[i] *= f;
+            if (j > 0) {
+              ok = mbar_wait_bounded(&sh->ds_done, (j - 1) & 1);
+              if (!ok) break;
+              tc_fence_after();
+              scale_sums(tmem + lanes + kDq, half * (DP / Shape::kHalves), (half + 1) * (DP / Shape::kHalves), f);
+            }
+          }
+        }
         uint32_t w[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) w[i] = pack_half2<T>(x[2 * i], x[2 * i + 1]);
@@ -331,8 +404,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         report_status(p.status, GW_ERR_TIMEOUT);
       }
       tc_fence_after();
-      store_acc<T>(p.dq, static_cast<T*>(p.dq) + (token * p.H + head) * p.D, tmem + lanes + kDq, half * (DP / Shape::kHalves), (half + 1) * (DP / Shape::kHalves), p.D, p.scale,
-                   live, n > 0);
+      store_acc<T>(p.dq, static_cast<T*>(p.dq) + (token * p.H + head) * p.D, tmem + lanes + kDq, half * (DP / Shape::kHalves), (half + 1) * (DP / Shape::kHalves), p.D,
+                   exp2f(static_cast<float>(-lift)), p.scale, live, n > 0);
     }
   }
   if (blockIdx.x == 0 && warp == Shape::kLoad) {
@@ -362,8 +435,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   constexpr uint32_t kS = 0, kDp = W, kDv = 2 * W, kDk = 2 * W + DP;
   // fp16 holds nothing below 2^-24 and few bits below 2^-14, and a P of a long sequence is that small: it is raised by 2^12 (P <= 1)
   // and dv lowered again; bf16 has fp32's range
-  constexpr float kLift = sizeof(T) == 2 && std::is_same<T, __half>::value ? 12.f : 0.f;
-  constexpr float kLower = kLift > 0.f ? 1.f / 4096.f : 1.f;
+  constexpr float kLift = kRaised<T> ? 12.f : 0.f;
+  constexpr float kLower = kRaised<T> ? 1.f / 4096.f : 1.f;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* k_smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char* v_smem = k_smem + TB;
@@ -391,6 +464,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const int all = per_head * group;                        // pairs of tiles
     const int begin = share == 0 ? 0 : (all + 1) / BLOCKS;   // this block's: the first half, rounded up, or the rest
     const int n = BLOCKS == 1 ? all : share == 0 ? (all + 1) / 2 : all / 2;
+    float dk_lower = 1.f;  // of this thread's row
 
     if (warp == Shape::kLoad) {
       bool ok = true;
@@ -492,7 +566,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
       const uint32_t s_addr = tmem + lanes + kS + half * 64, d_addr = tmem + lanes + kDp + half * 64;
       const float c = p.scale * kLog2e;
-      const uint64_t c2 = pack_f2(c, c), lower2 = pack_f2(kLower, kLower);
+      const uint64_t c2 = pack_f2(c, c);
+      int lift = kRaised<T> ? kFirstLift : 0;
+      float raise = exp2f(lift - kLift);  // from the raised P to the raised dS
       bool ok = true;
       for (int i = 0; i < n; ++i) {
         const int st = i % ST, r0 = (first + (begin + i) % per_head) * W;
@@ -542,9 +618,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           const ulonglong2 d = d2[k];
           uint64_t a = mul_f2(pack_f2(x[4 * k], x[4 * k + 1]), add_f2(pack_f2(y[4 * k], y[4 * k + 1]), d.x));
           uint64_t b = mul_f2(pack_f2(x[4 * k + 2], x[4 * k + 3]), add_f2(pack_f2(y[4 * k + 2], y[4 * k + 3]), d.y));
-          if (kLift > 0.f) {
-            a = mul_f2(a, lower2);
-            b = mul_f2(b, lower2);
+          if (kRaised<T>) {
+            a = mul_f2(a, pack_f2(raise, raise));
+            b = mul_f2(b, pack_f2(raise, raise));
           }
           unpack_f2(a, y[4 * k], y[4 * k + 1]);
           unpack_f2(b, y[4 * k + 2], y[4 * k + 3]);
@@ -552,6 +628,17 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (edge) {
 #pragma unroll
           for (int k = 0; k < 64; ++k) y[k] = k >= from ? y[k] : 0.f;
+        }
+        if constexpr (kRaised<T>) {
+          const float f = lift_row<Shape::kHalves>(y, lift, row < s.lk, sh, half, (warp & 3) * 32 + lane, i, ok);
+          if (!ok) break;
+          if (__any_sync(0xffffffffu, f != 1.f)) {
+            raise = exp2f(lift - kLift);
+#pragma unroll
+            for (int k = 0; k < 64; ++k) y[k] *= f;
+            // dP was asked for behind the last product that adds to dk, so that product is done
+            if (i > 0) scale_sums(tmem + lanes + kDk, half * (DP / Shape::kHalves), (half + 1) * (DP / Shape::kHalves), f);
+          }
         }
 #pragma unroll
         for (int k = 0; k < 32; ++k) w[k] = pack_half2<T>(y[2 * k], y[2 * k + 1]);
@@ -566,6 +653,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         sh->abort_flag = 1;
         report_status(p.status, GW_ERR_TIMEOUT);
       }
+      dk_lower = exp2f(static_cast<float>(-lift));
       tc_fence_after();
     }
 
@@ -587,6 +675,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tmem_load32(tmem + lanes + (which == 0 ? kDv : kDk) + b, o);
             tmem_wait_ld();
 #pragma unroll
+            for (int c = 0; c < 32; ++c) o[c] *= which == 0 ? kLower : dk_lower;
+#pragma unroll
             for (int c = 0; c < 8; ++c)
               asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote + (((which * (DP / 4) + b / 4 + c) * kTile + r) << 4)),
                            "f"(o[4 * c]), "f"(o[4 * c + 1]), "f"(o[4 * c + 2]), "f"(o[4 * c + 3])
@@ -600,9 +690,9 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const bool live = row < s.lk;
       const int64_t at = (static_cast<int64_t>(s.k0 + row) * p.Hk + kv) * p.D;
       const float4* more = BLOCKS == 2 && all > 1 ? sums + r : nullptr;
-      if (half == 0) store_acc<T>(p.dv, static_cast<T*>(p.dv) + at, tmem + lanes + kDv, 0, DP, p.D, kLower, live, all > 0, more);
+      if (half == 0) store_acc<T>(p.dv, static_cast<T*>(p.dv) + at, tmem + lanes + kDv, 0, DP, p.D, kLower, 1.f, live, all > 0, more);
       if (half == Shape::kHalves - 1)
-        store_acc<T>(p.dk, static_cast<T*>(p.dk) + at, tmem + lanes + kDk, 0, DP, p.D, p.scale, live, all > 0,
+        store_acc<T>(p.dk, static_cast<T*>(p.dk) + at, tmem + lanes + kDk, 0, DP, p.D, dk_lower, p.scale, live, all > 0,
                      more != nullptr ? more + DP / 4 * kTile : nullptr);
     }
   }
