@@ -178,7 +178,7 @@ extern "C" int gw_rotary_axes(const void* q, const void* k, int dtype, int B, in
   const uintptr_t data = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(q_out) |
                          (Hk > 0 ? reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(k_out) : 0);
   const uintptr_t tabs = reinterpret_cast<uintptr_t>(cos_tab) | reinterpret_cast<uintptr_t>(sin_tab);
-  while (v > 1 && (all % v != 0 || data % (v * es) != 0 || tabs % (v * 4 > 16 ? 16 : v * 4) != 0)) v /= 2;
+  while (v > 1 && (all % v != 0 || data % (v * es) != 0 || tabs % (v * 4) != 0)) v /= 2;  // pieces of the tables: v floats
   int dev = 0;
   DeviceFacts facts;
   const int rc = device_facts(&dev, &facts);

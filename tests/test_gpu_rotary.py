@@ -163,3 +163,23 @@ def test_refusals():
     ]:
         with pytest.raises(error):
             call()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offset", [1, 2, 4, 8, 12])
+def test_tables_inside_a_larger_buffer(offset, dtype):
+    """Tables that start 4 to 48 bytes behind a 256-byte boundary: the widest pieces need 32-byte ones, narrower ones serve as well."""
+    from geoweave_b200.rotary import RotaryAxes, apply_rotary_axes, rotary_axes
+    from tests.gpu_util import dev
+
+    g = torch.Generator().manual_seed(offset)
+    widths, n = (32, 32), 60
+    own = rotary_axes(widths, n, dev())
+    room = torch.empty(2, n * 32 + 16, device=dev())
+    tables = [x[offset:offset + n * 32].view(n, 32).copy_(t) for x, t in zip(room, (own.cos, own.sin))]
+    axes = RotaryAxes(widths, *tables)
+    assert axes.cos.data_ptr() == tables[0].data_ptr() and axes.cos.data_ptr() % 256 == 4 * offset
+    q, k = [torch.randn(77, h, 64, generator=g).to(dtype).to(dev()) for h in (4, 2)]
+    pos = torch.randint(0, n, (77, 2), generator=g).to(dev())
+    for a, b in zip(apply_rotary_axes(q, k, pos, axes), apply_rotary_axes(q, k, pos, own)):
+        assert torch.equal(a, b)
