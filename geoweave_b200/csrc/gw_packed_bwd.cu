@@ -80,7 +80,7 @@ __device__ __forceinline__ float lift_row(const float (&x)[64], int& lift, bool 
     sh->top[tile & 1][half][row] = static_cast<uint8_t>(exponent);
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(&sh->top_full[row >> 5]);
-    ok = ok && mbar_wait_bounded(&sh->top_full[row >> 5], tile & 1);
+    ok = ok && warp_wait(&sh->top_full[row >> 5], tile & 1, &sh->abort_flag);
     exponent = max(exponent, static_cast<int>(sh->top[tile & 1][half ^ 1][row]));
   }
   // infinite values stay what they are; rows behind the sequence hold its neighbour's and are not stored
@@ -231,21 +231,21 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const uint64_t qd = make_smem_desc(smem_u32(q_smem)), gd = make_smem_desc(smem_u32(g_smem));
       const uint64_t kd = make_smem_desc(smem_u32(k_smem)), vd = make_smem_desc(smem_u32(v_smem));
       const uint64_t kd_mn = make_smem_desc_mn(smem_u32(k_smem));
-      bool ok = n == 0 || mbar_wait_bounded(&sh->own_full, 0);
+      bool ok = n == 0 || warp_wait(&sh->own_full, 0, &sh->abort_flag);
       auto products = [&](int j) {  // S and dP of key tile j, each as soon as the one before it has been read
         const int sk = j % SK, sv = j % SV;
-        ok = mbar_wait_bounded(&sh->a_full[sk], (j / SK) & 1);
+        ok = warp_wait(&sh->a_full[sk], (j / SK) & 1, &sh->abort_flag);
         if (!ok) return;
         if ((j + 1) * W > s.lk) zero_rows_from<DP, W>(k_smem + sk * WB, s.lk - j * W);  // K is also dq's operand
-        if (j > 0) ok = mbar_wait_bounded(&sh->s_read, (j - 1) & 1);
+        if (j > 0) ok = warp_wait(&sh->s_read, (j - 1) & 1, &sh->abort_flag);
         if (!ok) return;
         tc_fence_after();
         if (elect_one()) {
           mma_rows<DP>(tmem + kS, qd, kd + sk * (WB >> 4), idesc_s);
           tc_commit(&sh->s_full);
         }
-        ok = mbar_wait_bounded(&sh->b_full[sv], (j / SV) & 1);
-        if (j > 0) ok = ok && mbar_wait_bounded(&sh->dp_read, (j - 1) & 1);
+        ok = warp_wait(&sh->b_full[sv], (j / SV) & 1, &sh->abort_flag);
+        if (j > 0) ok = ok && warp_wait(&sh->dp_read, (j - 1) & 1, &sh->abort_flag);
         if (!ok) return;
         tc_fence_after();
         if (elect_one()) {
@@ -255,10 +255,10 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
       };
       if (n > 0 && ok) products(0);
-      for (int j = 0; j < n && ok && !sh->abort_flag; ++j) {
+      for (int j = 0; j < n && ok; ++j) {
         const int st = j % SK;
         if (j + 1 < n) products(j + 1);
-        ok = ok && mbar_wait_bounded(&sh->ds_full, j & 1);
+        ok = ok && warp_wait(&sh->ds_full, j & 1, &sh->abort_flag);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -300,7 +300,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           const float lse = p.lse[at];
           neg_lse = lse == -INFINITY ? -INFINITY : -lse * kLog2e;
         }
-        ok = mbar_wait_bounded(&sh->own_full, 0);
+        ok = warp_wait(&sh->own_full, 0, &sh->abort_flag);
         const int r = (warp & 3) * 32 + lane;
         const unsigned char* g = g_smem + half * kBoxBytes + r * 128;
 #pragma unroll
@@ -333,8 +333,8 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const int limit = (p.causal ? min(s.lk, row + off + 1) : s.lk) - half * 64;
       const int open = p.causal ? min(s.lk, r0 + off + 1) : s.lk;
       for (int j = 0; j < n; ++j) {
-        ok = ok && mbar_wait_bounded(&sh->s_full, j & 1);
-        if (!ok || sh->abort_flag) break;
+        ok = ok && warp_wait(&sh->s_full, j & 1, &sh->abort_flag);
+        if (!ok) break;
         tc_fence_after();
         float x[64], y[64];
         tmem_load32(tmem + lanes + kS + half * 64, x);
@@ -350,7 +350,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           x[2 * i] = exp2_fast(a);
           x[2 * i + 1] = exp2_fast(b);
         }
-        ok = mbar_wait_bounded(&sh->dp_full, j & 1);
+        ok = warp_wait(&sh->dp_full, j & 1, &sh->abort_flag);
         if (!ok) break;
         tc_fence_after();
         tmem_load32(tmem + lanes + kDp + half * 64, y);
@@ -377,7 +377,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
             for (int i = 0; i < 64; ++i) x[i] *= f;
             if (j > 0) {
-              ok = mbar_wait_bounded(&sh->ds_done, (j - 1) & 1);
+              ok = warp_wait(&sh->ds_done, (j - 1) & 1, &sh->abort_flag);
               if (!ok) break;
               tc_fence_after();
               scale_sums(tmem + lanes + kDq, half * (DP / Shape::kHalves), (half + 1) * (DP / Shape::kHalves), f);
@@ -388,7 +388,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
         for (int i = 0; i < 32; ++i) w[i] = pack_half2<T>(x[2 * i], x[2 * i + 1]);
         if (j > 0) {
-          ok = mbar_wait_bounded(&sh->ds_done, (j - 1) & 1);
+          ok = warp_wait(&sh->ds_done, (j - 1) & 1, &sh->abort_flag);
           if (!ok) break;
           tc_fence_after();
         }
@@ -398,7 +398,7 @@ packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->ds_full);
       }
-      if (n > 0 && ok && !sh->abort_flag) ok = mbar_wait_bounded(&sh->ds_done, (n - 1) & 1);
+      if (n > 0 && ok) ok = warp_wait(&sh->ds_done, (n - 1) & 1, &sh->abort_flag);
       if (!ok) {
         sh->abort_flag = 1;
         report_status(p.status, GW_ERR_TIMEOUT);
@@ -476,8 +476,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       for (; i < n; ++i) {
         const int st = i % ST, at = begin + i, head = kv * group + at / per_head, r0 = (first + at % per_head) * W;
-        ok = mbar_wait_bounded(&sh->a_empty[st], ((i / ST) & 1u) ^ 1u);
-        if (!ok || sh->abort_flag) break;
+        ok = warp_wait(&sh->a_empty[st], ((i / ST) & 1u) ^ 1u, &sh->abort_flag);
+        if (!ok) break;
         if (lane == 0) {
           mbar_arrive_expect_tx(&sh->a_full[st], WB);
           load_rows<DP, W>(q_smem + st * WB, &tmQ, head, s.q0 + r0, &sh->a_full[st]);
@@ -502,7 +502,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (lane == 0) mbar_arrive(&sh->st_full[st]);
       }
       if (!ok) sh->abort_flag = 1;
-      if (sh->abort_flag && lane == 0) {  // let the copies in flight land before the shared memory is given up
+      if (warp_sees(sh->abort_flag) && lane == 0) {  // let the copies in flight land before the shared memory is given up
         if (n > 0) mbar_wait_limit(&sh->own_full, 0, kDrainLimitNs);
         for (int u = max(0, i - ST); u < i; ++u) {
           mbar_wait_limit(&sh->a_full[u % ST], (u / ST) & 1u, kDrainLimitNs);
@@ -516,11 +516,11 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const uint64_t kd = make_smem_desc(smem_u32(k_smem)), vd = make_smem_desc(smem_u32(v_smem));
       const uint64_t qd = make_smem_desc(smem_u32(q_smem)), gd = make_smem_desc(smem_u32(g_smem));
       const uint64_t qd_mn = make_smem_desc_mn(smem_u32(q_smem)), gd_mn = make_smem_desc_mn(smem_u32(g_smem));
-      bool ok = n == 0 || mbar_wait_bounded(&sh->own_full, 0);
+      bool ok = n == 0 || warp_wait(&sh->own_full, 0, &sh->abort_flag);
       // S^T = K Q^T / dP^T = V d_o^T of query tile i; rows behind the sequence's end become zeros first
       auto product = [&](int i, uint64_t* full, unsigned char* tiles, uint64_t a, uint64_t b, uint32_t d, uint64_t* done) {
         const int st = i % ST, left = s.lq - (first + (begin + i) % per_head) * W;
-        ok = mbar_wait_bounded(&full[st], (i / ST) & 1);
+        ok = warp_wait(&full[st], (i / ST) & 1, &sh->abort_flag);
         if (!ok) return;
         if (left < W) zero_rows_from<DP, W>(tiles + st * WB, left);
         tc_fence_after();
@@ -540,13 +540,13 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         product(0, sh->a_full, q_smem, kd, qd, tmem + kS, &sh->s_full);
         if (ok) product(0, sh->b_full, g_smem, vd, gd, tmem + kDp, &sh->dp_full);
       }
-      for (int i = 0; i < n && ok && !sh->abort_flag; ++i) {
-        ok = mbar_wait_bounded(&sh->p_full, i & 1);
+      for (int i = 0; i < n && ok; ++i) {
+        ok = warp_wait(&sh->p_full, i & 1, &sh->abort_flag);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) accumulate(i, tmem + kDv, tmem + kS, gd_mn);
         if (i + 1 < n) product(i + 1, sh->a_full, q_smem, kd, qd, tmem + kS, &sh->s_full);
-        ok = ok && mbar_wait_bounded(&sh->ds_full, i & 1);
+        ok = ok && warp_wait(&sh->ds_full, i & 1, &sh->abort_flag);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -576,8 +576,8 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const ulonglong2* d2 = reinterpret_cast<const ulonglong2*>(stats + st * 2 * W + W + half * 64);
         const bool edge = p.causal && c0 + kTile - 1 > r0 + off;  // some pair of the tiles is masked
         const int from = row - off - r0 - half * 64;              // the first column that sees this key
-        ok = mbar_wait_bounded(&sh->st_full[st], (i / ST) & 1) && mbar_wait_bounded(&sh->s_full, i & 1);
-        if (!ok || sh->abort_flag) break;
+        ok = warp_wait(&sh->st_full[st], (i / ST) & 1, &sh->abort_flag) && warp_wait(&sh->s_full, i & 1, &sh->abort_flag);
+        if (!ok) break;
         tc_fence_after();
         float x[64], y[64];
         uint32_t w[32];
@@ -607,7 +607,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->p_full);
 
-        ok = mbar_wait_bounded(&sh->dp_full, i & 1);
+        ok = warp_wait(&sh->dp_full, i & 1, &sh->abort_flag);
         if (!ok) break;
         tc_fence_after();
         tmem_load32(d_addr, y);
@@ -648,7 +648,7 @@ packed_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->ds_full);
       }
-      if (n > 0 && ok && !sh->abort_flag) ok = mbar_wait_bounded(&sh->all_done, 0);
+      if (n > 0 && ok) ok = warp_wait(&sh->all_done, 0, &sh->abort_flag);
       if (!ok) {
         sh->abort_flag = 1;
         report_status(p.status, GW_ERR_TIMEOUT);

@@ -84,7 +84,7 @@ static_assert(sizeof(FwdShared) <= 512, "shared bookkeeping");
 // The next item is there when the loads of the one before it have all been issued: for warps whose tile has no rows in that one
 // its whole length away, so the limit is long.  After a failure the loading warp ends the list at once.
 __device__ __forceinline__ bool wait_item(FwdShared* sh, int i) {
-  return mbar_wait_limit(&sh->item_full[i & 1], (i >> 1) & 1, 60 * kWaitLimitNs);
+  return warp_wait(&sh->item_full[i & 1], (i >> 1) & 1, &sh->abort_flag, 60 * kWaitLimitNs);
 }
 
 // Few rows against many keys: the key tiles of a row tile are divided among `count` items, which leave their unnormalised sums
@@ -145,7 +145,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     // ------------------------------ work list and loads ------------------------------
     uint32_t ring = 0, q_use[kTiles] = {};  // key tiles and query tiles loaded so far
     int i = 0, told = 0;                    // items, and those of them that the others have been told of
-    for (int64_t at = blockIdx.x; ok && !sh->abort_flag; at += gridDim.x, ++i) {
+    for (int64_t at = blockIdx.x; ok; at += gridDim.x, ++i) {
       FwdItem w{};
       const int parts = TILES == 1 ? fp.count : 1;
       w.part = static_cast<int>(at % parts);
@@ -183,7 +183,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         w.slot = (rank - tiles) * parts + w.part;
         w.slots = (slots - tiles) * parts;
       }
-      ok = mbar_wait_bounded(&sh->item_empty[i & 1], ((i >> 1) & 1) ^ 1);
+      ok = warp_wait(&sh->item_empty[i & 1], ((i >> 1) & 1) ^ 1, &sh->abort_flag);
       if (!ok) break;
       if (lane == 0) {
         sh->item[i & 1] = w;
@@ -194,7 +194,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (w.kind == kItemTail) continue;
       const int kv = w.head / (p.H / p.Hk);
       auto load_q = [&](int t) {
-        ok = ok && mbar_wait_bounded(&sh->q_empty[t], (q_use[t] & 1) ^ 1);
+        ok = ok && warp_wait(&sh->q_empty[t], (q_use[t] & 1) ^ 1, &sh->abort_flag);
         if (!ok) return;
         if (lane == 0) {
           mbar_arrive_expect_tx(&sh->q_full[t], TB);
@@ -202,18 +202,18 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         ++q_use[t];
       };
-      for (int j = 0; j < w.most && ok && !sh->abort_flag; ++j, ++ring) {
+      for (int j = 0; j < w.most && ok; ++j, ++ring) {
         const int st = ring % ST;
         const uint32_t par = ((ring / ST) & 1u) ^ 1u;
         if (j == 0 && w.n[0] > 0) load_q(0);
-        ok = ok && mbar_wait_bounded(&sh->k_empty[st], par);
+        ok = ok && warp_wait(&sh->k_empty[st], par, &sh->abort_flag);
         if (!ok) break;
         if (lane == 0) {
           mbar_arrive_expect_tx(&sh->k_full[st], TB);
           load_rows<DP>(k_smem + st * TB, &tmK, kv, w.k0 + j * kTile, &sh->k_full[st]);
         }
         if (TILES == 2 && j == 0 && w.n[1] > 0) load_q(1);
-        ok = ok && mbar_wait_bounded(&sh->v_empty[st], par);
+        ok = ok && warp_wait(&sh->v_empty[st], par, &sh->abort_flag);
         if (lane == 0) {  // also after a wait that ran out, so that the drain below finds both copies of the stage
           mbar_arrive_expect_tx(&sh->v_full[st], TB);
           load_rows<DP>(v_smem + st * TB, &tmV, kv, w.k0 + j * kTile, &sh->v_full[st]);
@@ -222,7 +222,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     if (blockIdx.x == 0) packed_check(p);
     if (!ok) sh->abort_flag = 1;
-    if (sh->abort_flag && lane == 0) {
+    if (warp_sees(sh->abort_flag) && lane == 0) {
       sh->item[told & 1].kind = kItemEnd;
       mbar_arrive(&sh->item_full[told & 1]);
       // let the copies in flight land before the shared memory is given up
@@ -242,7 +242,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint64_t qd = make_smem_desc(smem_u32(q_smem)), kd = make_smem_desc(smem_u32(k_smem));
     const uint64_t vd = make_smem_desc_mn(smem_u32(v_smem));
     uint32_t ring = 0, done[kTiles] = {}, q_use[kTiles] = {};  // key tiles in the ring before this item; of each tile; query tiles
-    for (int i = 0; ok && !sh->abort_flag; ++i) {
+    for (int i = 0; ok; ++i) {
       ok = wait_item(sh, i);
       if (!ok) break;
       const FwdItem* item = &sh->item[i & 1];
@@ -259,9 +259,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       if (kind == kItemTail) continue;
       auto scores = [&](int t, int j) {  // S of key tile j; S has been read: for wide heads P, which sits on it, has been used
         const uint32_t at = ring + j, c = done[t] + j;
-        if (j == 0) ok = ok && mbar_wait_bounded(&sh->q_full[t], q_use[t] & 1);
-        if (DP == 64 || j == 0) ok = ok && mbar_wait_bounded(&sh->k_full[at % ST], (at / ST) & 1);
-        if (DP == 64 && c > 0) ok = ok && mbar_wait_bounded(&sh->s_read[t], (c - 1) & 1);
+        if (j == 0) ok = ok && warp_wait(&sh->q_full[t], q_use[t] & 1, &sh->abort_flag);
+        if (DP == 64 || j == 0) ok = ok && warp_wait(&sh->k_full[at % ST], (at / ST) & 1, &sh->abort_flag);
+        if (DP == 64 && c > 0) ok = ok && warp_wait(&sh->s_read[t], (c - 1) & 1, &sh->abort_flag);
         if (!ok) return;
         tc_fence_after();
         if (elect_one()) {
@@ -280,7 +280,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       // A stage goes back once for each issuer.  One whose tile does not read it still waits until it is full: running ahead
       // of the loads it would count twice in one phase of the barrier.
       auto pass_on = [&](uint64_t* full, uint64_t* empty, uint32_t at) {
-        ok = ok && mbar_wait_bounded(&full[at % ST], (at / ST) & 1);
+        ok = ok && warp_wait(&full[at % ST], (at / ST) & 1, &sh->abort_flag);
         if (ok && lane == 0) mbar_arrive(&empty[at % ST]);
       };
       if (mine > 0) {
@@ -288,7 +288,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       } else if (most > 0) {
         pass_on(sh->k_full, sh->k_empty, ring);
       }
-      for (int j = 0; j < most && ok && !sh->abort_flag; ++j) {
+      for (int j = 0; j < most && ok; ++j) {
         const uint32_t st = (ring + j) % ST, st_next = (ring + j + 1) % ST;
         bool v_here = false;
 #pragma unroll
@@ -297,8 +297,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           const uint32_t c = done[t] + j;
           if (DP == 64 && j + 1 < n[t]) scores(t, j + 1);  // P has its own place: ahead of this tile's softmax
           if (!v_here) {
-            ok = ok && mbar_wait_bounded(&sh->v_full[st], ((ring + j) / ST) & 1);
-            if (DP != 64 && j + 1 < mine) ok = ok && mbar_wait_bounded(&sh->k_full[st_next], ((ring + j + 1) / ST) & 1);
+            ok = ok && warp_wait(&sh->v_full[st], ((ring + j) / ST) & 1, &sh->abort_flag);
+            if (DP != 64 && j + 1 < mine) ok = ok && warp_wait(&sh->k_full[st_next], ((ring + j + 1) / ST) & 1, &sh->abort_flag);
             if (ok && (j + 1) * kTile > lk) zero_rows_from<DP>(v_smem + st * TB, lk - j * kTile);
             v_here = true;
           }
@@ -309,7 +309,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           // before either half): 16 384 tokens, 16 heads 1811 -> 1782 us, two causal sequences of 3000, 100 rows each 33.5 -> 31.8 us.
           // For narrow heads it is the exponentials that bound the kernel.
           if (DP != 64) {
-            ok = ok && mbar_wait_bounded(&sh->p_half[t], c & 1);
+            ok = ok && warp_wait(&sh->p_half[t], c & 1, &sh->abort_flag);
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
@@ -321,7 +321,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               }
             }
           }
-          ok = ok && mbar_wait_bounded(&sh->p_full[t], c & 1);
+          ok = ok && warp_wait(&sh->p_full[t], c & 1, &sh->abort_flag);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
@@ -366,7 +366,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t o_addr = tmem + lanes + Shape::kO + t * DP;
     const float c = p.scale * kLog2e;
     uint32_t done = 0;  // key tiles of this tile so far
-    for (int i = 0; ok && !sh->abort_flag; ++i) {
+    for (int i = 0; ok; ++i) {
       ok = wait_item(sh, i);
       if (!ok) break;
       const FwdItem* item = &sh->item[i & 1];  // given back behind the output
@@ -384,8 +384,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const int tiles = item->n[t];
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < tiles; ++j, ++done) {
-        ok = mbar_wait_bounded(&sh->s_full[t], done & 1);
-        if (!ok || sh->abort_flag) break;
+        ok = warp_wait(&sh->s_full[t], done & 1, &sh->abort_flag);
+        if (!ok) break;
         tc_fence_after();
         float x[128];
 #pragma unroll
@@ -417,7 +417,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             const float shrink = grown ? exp2_fast((m - mx) * c) : 1.f;
             l *= shrink;
             if (grown) m = mx;
-            ok = mbar_wait_bounded(&sh->o_done[t], (done - 1) & 1);
+            ok = warp_wait(&sh->o_done[t], (done - 1) & 1, &sh->abort_flag);
             if (!ok) break;
             o_ready = true;
             tc_fence_after();
@@ -464,7 +464,7 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         unpack_f2(sum[1], s2, s3);
         l += (s0 + s1) + (s2 + s3);
         if (DP == 64 && j > 0 && !o_ready) {  // the previous product still reads P (for wide heads S, and so P, waited for it)
-          ok = mbar_wait_bounded(&sh->o_done[t], (done - 1) & 1);
+          ok = warp_wait(&sh->o_done[t], (done - 1) & 1, &sh->abort_flag);
           if (!ok) break;
           tc_fence_after();
         }
@@ -475,9 +475,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh->p_full[t]);
       }
-      if (!ok || sh->abort_flag) break;
+      if (!ok) break;
       if (tiles > 0) {
-        ok = mbar_wait_bounded(&sh->o_done[t], (done - 1) & 1);
+        ok = warp_wait(&sh->o_done[t], (done - 1) & 1, &sh->abort_flag);
         if (!ok) break;
         tc_fence_after();
       }

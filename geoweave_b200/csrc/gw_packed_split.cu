@@ -122,12 +122,13 @@ split_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
   const float c = p.scale * kLog2e;
   bool ok = true;
 
-  for (int it = 0; it < steps; ++it) {
+  int it = 0;
+  for (; it < steps; ++it) {
     const int k0 = k_from + it * STRIDE;
     unsigned char* at = ring + it % ST * Shape::kStep;
     const uint32_t kt = smem_u32(at), vt = kt + NB * Shape::kBox;
-    ok = mbar_wait_bounded(&full[warp][it % ST], (it / ST) & 1);
-    if (!__all_sync(0xffffffffu, ok)) break;
+    ok = warp_wait(&full[warp][it % ST], (it / ST) & 1, nullptr);
+    if (!ok) break;
     if (k0 + STEP > k_to) {  // the last step: V rows behind the chunk may hold anything, and meet weights of zero
 #pragma unroll 1
       for (int b = 0; b < NB; ++b)
@@ -205,9 +206,10 @@ split_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     fetch(it + ST);
   }
   if (!ok) {  // let the copies in flight land before the shared memory is given up
-    if (lane == 0)
-      for (int i = 0; i < ST; ++i) mbar_wait_limit(&full[warp][i], 0, kDrainLimitNs);
-    report_status(p.status, GW_ERR_TIMEOUT);
+    if (lane == 0) {
+      for (int i = it; i < steps && i < it + ST; ++i) mbar_wait_limit(&full[warp][i % ST], (i / ST) & 1, kDrainLimitNs);
+      report_status(p.status, GW_ERR_TIMEOUT);
+    }
   }
 #pragma unroll
   for (int d = 1; d < 4; d <<= 1) {

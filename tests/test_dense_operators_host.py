@@ -73,3 +73,30 @@ def test_entry_points_refuse_bad_arguments_before_any_launch(lib):
     assert rot(axes=5) == rot(D=512) == rot(dt=9) == -2
     assert lib.gw_packed_attn_bwd_workspace_bytes(1000, 16) == 64000
     assert lib.gw_packed_attn_bwd_workspace_bytes(0, 16) == 0
+
+
+def test_warps_of_the_packed_kernels_wait_as_one():
+    """A wait that runs out must not split a warp: outside blocks that a single lane runs, every wait goes through warp_wait, and so does
+    every look at the abort flag, or through warp_sees.  (In a split warp the next warp-wide instruction would wait without a limit.)"""
+    import os
+    import re
+
+    import geoweave_b200
+
+    csrc = os.path.join(os.path.dirname(geoweave_b200.__file__), "csrc")
+    for name in ("gw_packed_fwd.cu", "gw_packed_bwd.cu", "gw_packed_split.cu"):
+        blocks, waits = [], 0  # the lines that opened the blocks around the present one
+        for number, line in enumerate(open(os.path.join(csrc, name)), 1):
+            code = line.split("//")[0]
+            one_lane = any("lane == 0" in b for b in blocks) or "if (lane == 0)" in code
+            waits += code.count("warp_wait(")
+            if re.search(r"mbar_wait_\w+\(", code):
+                assert one_lane, f"{name}:{number}: {line.strip()}"
+            if re.search(r"abort_flag(?! = )", re.sub(r"int abort_flag;|&sh->abort_flag|warp_sees\(sh->abort_flag\)", "", code)):
+                assert one_lane, f"{name}:{number}: {line.strip()}"
+            for c in code:
+                if c == "{":
+                    blocks.append(code)
+                elif c == "}":
+                    blocks.pop()
+        assert waits > 0 and not blocks
