@@ -8,6 +8,7 @@ import threading
 from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint, c_void_p, POINTER
 
 import torch
+from torch.autograd import forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("GEOWEAVE_B200_LIB") or os.path.join(HERE, "libgeoweave_b200.so")
@@ -172,6 +173,14 @@ def require_cuda(*tensors) -> torch.device:
         elif t.device != dev:
             raise ValueError("all tensors must be on the same CUDA device")
     return dev
+
+
+def wants_autograd(*tensors) -> bool:
+    """Whether a call has to go through its autograd function: an input requires grad, or carries a forward-mode tangent, which the
+    function then refuses (NotImplementedError); a call around it would drop the tangent without a word."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def i64x3(vals):

@@ -181,7 +181,7 @@ def packed_flash_attn_func(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal: boo
     Rows without an allowed key and rows behind the last sequence give zeros (gradients too).  Non-finite values of ``k`` and
     ``v`` stay within their own sequence; within a causal sequence they may also reach rows before them.
     """
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+    if _lib.wants_autograd(q, k, v):
         return _PackedFlashAttn.apply(q, k, v, cu_seqlens_q, cu_seqlens_k, bool(causal), softmax_scale, max_seqlen_q)
     with torch.no_grad():
         return packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k, causal, softmax_scale, max_seqlen_q)[0]

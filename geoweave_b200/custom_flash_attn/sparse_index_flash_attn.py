@@ -176,15 +176,11 @@ class _SparseIndexFlashAttn(torch.autograd.Function):
         return to_bthd(dq), to_bthd(dk), to_bthd(dv), None, None, None
 
 
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
-
-
 def sparse_index_flash_attn_func(q, k, v, kv_positions, bias=None, causal=False, softmax_scale=None):
     """The reference's autograd entry (``SparseIndexFlashAttnFunc.apply``): returns ``(o, attn_sum)`` with ``attn_sum``
     fp32 ``[B,T,K]``; differentiable in q, k and v."""
     _reject(bias, causal)
-    if _wants_grad(q, k, v):
+    if _lib.wants_autograd(q, k, v):
         return _SparseIndexFlashAttn.apply(q, k, v, kv_positions, softmax_scale, "bthd")
     with torch.no_grad():
         o, attn_sum, _ = sparse_attention_forward(q, k, v, kv_positions, softmax_scale, True, False, "bthd")
@@ -193,7 +189,7 @@ def sparse_index_flash_attn_func(q, k, v, kv_positions, bias=None, causal=False,
 
 def sparse_index_flash_attn_bhtd_func(q, k, v, kv_positions, bias=None, causal=False, softmax_scale=None):
     _reject(bias, causal)
-    if _wants_grad(q, k, v):
+    if _lib.wants_autograd(q, k, v):
         return _SparseIndexFlashAttn.apply(q, k, v, kv_positions, softmax_scale, "bhtd")
     with torch.no_grad():
         o, attn_sum, _ = sparse_attention_forward(q, k, v, kv_positions, softmax_scale, True, False, "bhtd")

@@ -220,7 +220,7 @@ def sparse_topk_indexer_func(q: torch.Tensor, k: torch.Tensor, w: torch.Tensor, 
     are differentiable in q, k and w (16-bit operands); the selection itself is computed without a graph, as in the
     reference (:2071)."""
     _reject_mask(mask, view_bias_data)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or w.requires_grad):
+    if _lib.wants_autograd(q, k, w):
         if q.dtype == torch.float32:
             raise NotImplementedError("the indexer's backward kernels take bfloat16 / float16 operands")
         return _SparseTopkIndexer.apply(q, k, w, topk, softmax_scale)

@@ -133,7 +133,7 @@ def apply_rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], pos: torch.Ten
     by the positions ``pos`` int64 or int32 ``[N, axes]`` (or ``[B,N,axes]``); returns contiguous ``(q, k)``, differentiable in
     both.  Inputs may be slices of a fused projection's output.  A position outside the tables is reported by
     ``geoweave_b200.check_status()`` and counts as 0."""
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if _lib.wants_autograd(q) if k is None else _lib.wants_autograd(q, k):
         if k is None:
             return _RotaryQOnly.apply(q, pos, axes), None
         return _RotaryAxesFunc.apply(q, k, pos, axes)
