@@ -1,0 +1,167 @@
+"""The packed attention on inputs whose results are counts and sums of whole numbers: a row that is left out or taken twice at
+a border of tiles, parts, chunks or sequences shows in full, at lengths where bounds on random inputs are wide.
+
+With q = 0 (or k = 0) every score is 0, so each weight is 1 before the division, which every type holds; sums of small whole numbers are
+exact in fp32.  What is left is the division and the last rounding: (u^2 + 2^-22) of the value for o with what its rounding took off,
+u + 2^-20 for a 16-bit result whose P or dS is a power of two, twice that otherwise (P = 1 / n is rounded too).
+"""
+import math
+
+import pytest
+import torch
+
+from tests.packed_reference import HALF, TINY, borders
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+# name: query lengths, key lengths, heads, key heads, max_seqlen_q -- each way the forward divides its work
+FORMS = {
+    "two tiles a block": ([2500, 33], [2999, 1500], 16, 16, None),
+    "one tile a block": ([700, 1], [1111, 129], 8, 2, None),
+    "keys in parts": ([130], [5003], 4, 2, None),
+    "keys in parts, ragged": ([300, 17], [4100, 9], 2, 1, None),
+    "single tokens": ([1, 0, 1, 1], [3001, 64, 77, 1], 8, 2, 1),
+    "a few queries": ([3, 4], [2600, 513], 8, 2, 4),
+}
+
+
+def _zeros(n, heads, D, dtype):
+    return torch.zeros(n, heads, D, dtype=dtype, device="cuda")
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float16, 64), (torch.float16, 80), (torch.float32, 64),
+                                     (torch.float32, 128)])
+@pytest.mark.parametrize("form", list(FORMS))
+def test_every_key_counts_once(form, dtype, D, causal):
+    """o = mean of the visible values, whole numbers of up to 8, with what rounding it took off."""
+    from geoweave_b200 import check_status
+    from geoweave_b200.custom_flash_attn.packed_flash_attn import packed_attention_forward
+
+    lens_q, lens_k, H, Hk, most = FORMS[form]
+    g = torch.Generator().manual_seed(D)
+    v = torch.randint(-8, 9, (sum(lens_k), Hk, D), generator=g).to(dtype).cuda()
+    k = torch.randn(sum(lens_k), Hk, D, generator=g).to(dtype).cuda()
+    q = _zeros(sum(lens_q), H, D, dtype)
+    low = None if dtype is torch.float32 else torch.full_like(q, float("nan"))
+    o, lse = packed_attention_forward(q, k, v, borders(lens_q, q.device), borders(lens_k, q.device), causal, None, most, True, low)
+    check_status()
+    u = HALF[dtype]
+    a = c = 0
+    for lq, lk in zip(lens_q, lens_k):
+        if lq:
+            seen = torch.full((lq,), lk) if not causal else (torch.arange(lq) + lk - lq + 1).clamp(0, lk)
+            seen = seen.cuda()
+            sums = torch.cat((torch.zeros_like(v[:1]).double(), v[c:c + lk].double().cumsum(0)))[seen]
+            want = (sums / seen.clamp(min=1)[:, None, None]).repeat_interleave(H // Hk, 1)
+            got = o[a:a + lq].double() + (0 if low is None else low[a:a + lq].double())
+            err = u * u + 2.0 ** -22 if low is not None else 2.0 ** -22
+            assert ((got - want).abs() <= err * want.abs() + TINY[dtype]).all()
+            assert ((o[a:a + lq].double() - want).abs() <= (u + 2.0 ** -22) * want.abs() + TINY[dtype]).all()
+            assert ((lse[:, a:a + lq].double() - seen.double().log()).nan_to_num(0.0).abs() <= 2.0 ** -20 * (1 + seen.double().log().abs().nan_to_num(0.0, 0.0, 0.0))).all()
+            assert (lse[:, a:a + lq][:, seen == 0] == -math.inf).all()
+        a, c = a + lq, c + lk
+
+
+def _codes(n, D, dtype, heads):
+    """[n, heads, D]: row i has a one in column i % 64."""
+    x = torch.zeros(n, heads, D)
+    x[torch.arange(n), :, torch.arange(n) % 64] = 1
+    return x.to(dtype).cuda()
+
+
+def _sides(lens):
+    """[n, 1]: +1 or -1 for each row of each sequence by (row within the batch) % 64, half of them each."""
+    n = sum(lens)
+    return torch.where(torch.arange(n) % 64 < 32, 1.0, -1.0)[:, None]
+
+
+def _counts(lens, D):
+    """For each sequence: how many of its rows (numbered over the batch) have their one in each column."""
+    out, at = [], 0
+    for n in lens:
+        out.append(torch.bincount(torch.arange(at, at + n) % 64, minlength=D)[:D].double().cuda())
+        at += n
+    return out
+
+
+# lengths of keys: powers of two, so that P = 1 / n is exact; multiples of 64 otherwise (borders inside tiles of 128)
+GRADS = [([4099, 70], [4096, 64], 2, 2), ([1500], [1024], 4, 2), ([1000, 129], [2048, 512], 1, 1), ([777], [3008], 2, 1), ([2900, 65], [192, 704], 4, 2)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens_q,lens_k,H,Hk", GRADS)
+def test_every_pair_counts_once_in_the_gradients(lens_q, lens_k, H, Hk, D, dtype):
+    from geoweave_b200 import check_status
+    from geoweave_b200.custom_flash_attn import packed_flash_attn_func
+
+    T, S, group, scale, u = sum(lens_q), sum(lens_k), H // Hk, 1 / 8, HALF[dtype]
+    cu = borders(lens_q, torch.device("cuda")), borders(lens_k, torch.device("cuda"))
+    first = lambda x, heads: torch.cat((x, torch.zeros(x.shape[0], D - 1)), 1)[:, None].expand(-1, heads, -1).to(dtype).cuda()
+    v = first(_sides(lens_k), Hk)       # +-1 in column 0
+    up = first(torch.ones(T, 1), H)     # dP = +-1, its mean 0 over each sequence of 64 n keys
+    sides = _sides(lens_k)[:, 0].double().cuda()
+    for n in lens_k:
+        assert n % 64 == 0
+
+    # q = 0: dq = scale sum_j dS_j k_j counts the keys with a one in each column; dv = sum_i P d_o the queries
+    q, k, v_, g = [x.clone().requires_grad_() for x in (_zeros(T, H, D, dtype), _codes(S, D, dtype, Hk), v)] + [up]
+    dq, dk, _ = torch.autograd.grad(packed_flash_attn_func(q, k, v_, *cu, False, scale), (q, k, v_), g)
+    g = _codes(T, D, dtype, H)
+    _, _, dv = torch.autograd.grad(packed_flash_attn_func(q, k, v_, *cu, False, scale), (q, k, v_), g)
+    # k = 0: dk = scale sum_i dS_i q_i counts the queries
+    q2, k2 = _codes(T, D, dtype, H).requires_grad_(), _zeros(S, Hk, D, dtype).requires_grad_()
+    dq2, dk2, _ = torch.autograd.grad(packed_flash_attn_func(q2, k2, v_, *cu, False, scale), (q2, k2, v_), up)
+    check_status()
+    assert (dk == 0).all() and (dq2 == 0).all()
+
+    a = c = 0
+    column = torch.where(torch.arange(D) % 64 < 32, 1.0, -1.0).double().cuda()
+    for lq, lk, rows, keys in zip(lens_q, lens_k, _counts(lens_q, D), _counts(lens_k, D)):
+        err = (u if lk & (lk - 1) == 0 else 2 * u) + 2.0 ** -20
+        want = scale / lk * keys * column
+        assert ((dq[a:a + lq].double() - want).abs() <= err * want.abs() + TINY[dtype]).all(), "dq"
+        want = group / lk * rows
+        assert ((dv[c:c + lk].double() - want).abs() <= err * want.abs() + TINY[dtype]).all(), "dv"
+        want = scale / lk * group * rows * sides[c:c + lk, None, None]
+        assert ((dk2[c:c + lk].double() - want).abs() <= err * want.abs() + TINY[dtype]).all(), "dk"
+        a, c = a + lq, c + lk
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("form", list(FORMS))
+def test_row_sums_come_from_the_output_before_its_rounding(form, D, dtype):
+    """Values close to 1 and keys close to 2: dP hardly differs between the keys, so an error of D = sum d_o o, which all of them share, is not
+    lost among others.  With o as rounded, dq is off by many times these limits.
+
+    Limits (e = 2^-24, n keys, P = 1 / n): D is off by sum|d_o| ((u^2 + 2^-22)|o| + 2^-25 for fp16) + (D + 8) e sum|d_o||o|; dP by
+    (D + 8) e sum|d_o||v|; dS by 1 / n of both and (u + 2^-18) of itself; dq by scale sum |dS error||k| + n e scale sum|dS||k| + u |dq|."""
+    from geoweave_b200 import check_status
+    from geoweave_b200.custom_flash_attn import packed_flash_attn_func
+
+    lens_q, lens_k, H, Hk, most = FORMS[form]
+    g = torch.Generator().manual_seed(D + 1)
+    mk = lambda n, h, mean, size: (mean + size * torch.randn(n, h, D, generator=g)).to(dtype).cuda()
+    q = _zeros(sum(lens_q), H, D, dtype).requires_grad_()
+    k, v, up = mk(sum(lens_k), Hk, 2.0, 0.25), mk(sum(lens_k), Hk, 1.0, 1 / 64), mk(sum(lens_q), H, 0.0, 1.0)
+    o = packed_flash_attn_func(q, k, v, borders(lens_q, q.device), borders(lens_k, q.device), False, None, most)
+    (dq,) = torch.autograd.grad(o, q, up)
+    check_status()
+    u, e, scale = HALF[dtype], 2.0 ** -24, D ** -0.5
+    a = c = 0
+    for lq, lk in zip(lens_q, lens_k):
+        for h in range(H if lq else 0):
+            K, V, G = k[c:c + lk, h * Hk // H].double(), v[c:c + lk, h * Hk // H].double(), up[a:a + lq, h].double()
+            mean = V.mean(0)
+            dS = (G @ (V - mean).T) / lk
+            want = scale * dS @ K
+            size = G.abs() @ mean.abs()
+            d_err = (u * u + 2.0 ** -22) * size + TINY[dtype] * G.abs().sum(1) + (D + 8) * e * size
+            s_err = (d_err[:, None] + (D + 8) * e * (G.abs() @ V.abs().T)) / lk + (u + 2.0 ** -18) * dS.abs()
+            limit = scale * (s_err @ K.abs() + lk * e * (dS.abs() @ K.abs())) + u * want.abs() + TINY[dtype]
+            assert ((dq[a:a + lq, h].double() - want).abs() <= limit).all(), (form, h)
+        a, c = a + lq, c + lk
