@@ -91,7 +91,7 @@ extern "C" int gw_packed_attn_bwd(const void* q, const void* k, const void* v, c
                                   const int64_t* d_out_strides, float scale, int causal, void* dq, void* dk, void* dv, void* workspace,
                                   size_t workspace_bytes, int* status_dev, gw_stream_t stream) {
   PackedParams p = make_params(q, k, v, cu_q, cu_k, nseq, total_q, total_k, H, Hk, D, q_strides, k_strides, v_strides, scale, causal, status_dev);
-  if (!out || !lse || !d_out || !d_out_strides || !dq || !dk || !dv) return GW_ERR_INVALID_ARG;
+  if (!out || !lse || !d_out || !d_out_strides || !dq || !dk != !dv) return GW_ERR_INVALID_ARG;
   p.o = const_cast<void*>(out);
   p.o_low = dtype == GW_F32 ? nullptr : const_cast<void*>(out_low);
   p.lse = const_cast<float*>(lse);

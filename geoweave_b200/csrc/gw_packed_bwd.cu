@@ -728,6 +728,7 @@ int launch_bwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t 
   if (q_items > 0x7fffffff || k_items > 0x3fffffff) return GW_ERR_UNSUPPORTED;
   packed_dq_kernel<T, DP><<<static_cast<unsigned>(q_items), kThreads, smem_q, st>>>(mq, mk, mv, mg, p, format);
   GW_LAUNCH_CHECK();
+  if (p.dk == nullptr) return GW_OK;  // keys and values without a gradient
   if (W != kTile && maps(W, kTile) != GW_OK) return rc;
   // Few and long blocks -- grouped heads, whose key tiles walk every head of the group -- leave SMs idle at the end: two share a key
   // tile.  One sequence of 4099 tokens, 2 key heads of 64 under 16: 436 us against 676 for the whole training step; ragged

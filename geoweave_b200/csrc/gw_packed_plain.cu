@@ -414,6 +414,7 @@ int launch_bwd(const PackedParams& p, cudaStream_t st) {
   if (rc != GW_OK) return rc;
   plain_dq_kernel<DP><<<dim3(static_cast<unsigned>(packed_tile_bound(p.total_q, BT, p.nseq)), p.H), NT, tiles_bytes<DP>(4), st>>>(p);
   GW_LAUNCH_CHECK();
+  if (p.dk == nullptr) return GW_OK;  // keys and values without a gradient
   plain_dkv_kernel<DP><<<dim3(static_cast<unsigned>(packed_tile_bound(p.total_k, BT, p.nseq)), p.Hk), NT, tiles_bytes<DP>(4), st>>>(p);
   GW_LAUNCH_CHECK();
   return GW_OK;

@@ -117,9 +117,11 @@ def packed_attention_forward(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal=Fa
     return o, lse
 
 
-def packed_attention_backward(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, d_out, causal=False, softmax_scale=None, o_low=None):
+def packed_attention_backward(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, d_out, causal=False, softmax_scale=None, o_low=None,
+                              key_grads=True):
     """Gradients ``(dq, dk, dv)`` of the forward, contiguous and of the inputs' dtype.  The sums run in a fixed order
-    (one kernel owns query rows, another key rows; no atomics), so results are reproducible."""
+    (one kernel owns query rows, another key rows; no atomics), so results are reproducible.  ``key_grads=False``: ``(dq, None,
+    None)``, and the second kernel does not run; the first always does, for the second needs its row sums."""
     scale = _scale(softmax_scale, q.shape[-1])
     dev, T, S, H, Hk, D, cu_q, cu_k = _checked(q, k, v, cu_seqlens_q, cu_seqlens_k)
     _lib.require_cuda(q, o, lse, d_out)
@@ -128,9 +130,9 @@ def packed_attention_backward(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, d_out
     if lse.dtype != torch.float32 or o.dtype != q.dtype:
         raise TypeError("o must have q's type and lse must be float32")
     dq = torch.empty((T, H, D), device=dev, dtype=q.dtype)
-    dk, dv = [torch.empty((S, Hk, D), device=dev, dtype=q.dtype) for _ in range(2)]
+    dk, dv = [torch.empty((S, Hk, D), device=dev, dtype=q.dtype) if key_grads else None for _ in range(2)]
     if T == 0 or S == 0:
-        return dq.zero_(), dk.zero_(), dv.zero_()
+        return tuple(x if x is None else x.zero_() for x in (dq, dk, dv))
     (q, qs), (k, ks), (v, vs), (d_out, ds) = _prepared(q), _prepared(k), _prepared(v), _prepared(d_out.to(q.dtype))
     o, lse = _prepared(o.contiguous())[0], lse.contiguous()
     if o_low is not None and (o_low.shape != o.shape or o_low.dtype != o.dtype or not o_low.is_contiguous()):
@@ -142,7 +144,7 @@ def packed_attention_backward(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, d_out
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         rc = lib.gw_packed_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _lib.ptr(o_low), lse.data_ptr(), d_out.data_ptr(),
                                     _lib.dtype_code(q), cu_q.data_ptr(), cu_k.data_ptr(), nseq, T, S, H, Hk, D, qs, ks, vs, ds,
-                                    scale, int(bool(causal)), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nbytes,
+                                    scale, int(bool(causal)), dq.data_ptr(), _lib.ptr(dk), _lib.ptr(dv), ws.data_ptr(), nbytes,
                                     _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "gw_packed_attn_bwd")
     if _lib.debug_enabled():
@@ -163,7 +165,8 @@ class _PackedFlashAttn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
         q, k, v, cu_q, cu_k, o, lse, o_low = ctx.saved_tensors
-        dq, dk, dv = packed_attention_backward(q, k, v, cu_q, cu_k, o, lse, d_out, ctx.causal, ctx.softmax_scale, o_low)
+        dq, dk, dv = packed_attention_backward(q, k, v, cu_q, cu_k, o, lse, d_out, ctx.causal, ctx.softmax_scale, o_low,
+                                               any(ctx.needs_input_grad[1:3]))
         return dq, dk, dv, None, None, None, None, None
 
 

@@ -125,7 +125,11 @@ class _RotaryAxesFunc(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         pos, _, _ = ctx.saved_tensors
-        return (*_rotate(dq, dk, pos, ctx.axes, True), None, None)
+        if all(ctx.needs_input_grad[:2]):
+            return (*_rotate(dq, dk, pos, ctx.axes, True), None, None)
+        if ctx.needs_input_grad[0]:
+            return _rotate(dq, None, pos, ctx.axes, True)[0], None, None, None
+        return None, _rotate(dk, None, pos, ctx.axes, True)[0], None, None
 
 
 def apply_rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], pos: torch.Tensor, axes: RotaryAxes):

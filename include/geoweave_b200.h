@@ -325,7 +325,7 @@ int gw_packed_attn_fwd(const void* q, const void* k, const void* v, int dtype, c
                        void* workspace, size_t workspace_bytes, int* status_dev, gw_stream_t stream);
 
 /* Its backward pass.  out, out_low (nullable) and lse are the forward's results, d_out [total_q, H, D] the gradient (strides as q's); dq, dk, dv
- * are contiguous and like q, k, v:
+ * are contiguous and like q, k, v (dk and dv may both be null: keys and values without a gradient, whose kernel is then not run):
  *   D = rowsum(d_out * (out + out_low)),  dS = P * (d_out v^T - D) * scale,  dq = dS k,  dk = sum over the key head's query heads dS^T q,
  *   dv = the same sum of P^T d_out.
  * P is made again from q, k and lse.  No atomics: the results do not depend on timing.  workspace holds D:

@@ -100,3 +100,12 @@ def test_warps_of_the_packed_kernels_wait_as_one():
                 elif c == "}":
                     blocks.pop()
         assert waits > 0 and not blocks
+
+
+def test_one_of_the_key_sides_gradients_alone_is_refused(lib):
+    from geoweave_b200 import _lib
+
+    p, two = 4096, _lib.i64x2([64, 64])
+    bwd = lambda dk, dv: lib.gw_packed_attn_bwd(p, p, p, p, None, p, p, _lib.GW_F16, p, p, 1, 8, 8, 1, 1, 64, two, two, two, two, 1.0, 0, p, dk, dv,
+                                                p, 1 << 20, None, None)
+    assert bwd(None, p) == bwd(p, None) == -1
