@@ -8,7 +8,7 @@ namespace {
 int check_packed(const PackedParams& p, int dtype, int* dev, DeviceFacts* facts) {
   if (!p.q || !p.k || !p.v || !p.cu_q || !p.cu_k || p.nseq < 0 || p.total_q < 0 || p.total_k < 0) return GW_ERR_INVALID_ARG;
   if (p.H <= 0 || p.Hk <= 0 || p.H % p.Hk != 0 || p.D <= 0) return GW_ERR_INVALID_ARG;
-  if (!(p.scale > 0.f) || p.scale > 3.0e38f) return GW_ERR_INVALID_ARG;
+  if (!(p.scale > 0.f) || !(p.scale * kLog2e <= 3.4028234e38f)) return GW_ERR_INVALID_ARG;  // the kernels multiply with scale log2 e
   if (dtype != GW_F32 && dtype != GW_BF16 && dtype != GW_F16) return GW_ERR_UNSUPPORTED;
   if (p.D > 128 || p.D % 8 != 0 || p.H > 65535 || p.total_q > 0x7fffff00 || p.total_k > 0x7fffff00 || p.nseq > 0xffffff)
     return GW_ERR_UNSUPPORTED;

@@ -24,8 +24,8 @@ def _scale(softmax_scale, D):
     if softmax_scale is None:
         return 1.0 / math.sqrt(D)
     scale = float(softmax_scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
+    if not 2.0 ** -126 <= scale <= 2.0 ** 127:  # as fp32, and times log2 e
+        raise ValueError(f"softmax_scale must be positive and finite in fp32, at least 2**-126 and at most 2**127, got {softmax_scale}")
     return scale
 
 

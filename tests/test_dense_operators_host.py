@@ -109,3 +109,18 @@ def test_one_of_the_key_sides_gradients_alone_is_refused(lib):
     bwd = lambda dk, dv: lib.gw_packed_attn_bwd(p, p, p, p, None, p, p, _lib.GW_F16, p, p, 1, 8, 8, 1, 1, 64, two, two, two, two, 1.0, 0, p, dk, dv,
                                                 p, 1 << 20, None, None)
     assert bwd(None, p) == bwd(p, None) == -1
+
+
+def test_scales_that_fp32_cannot_hold_are_refused(lib):
+    """Times log2 e the largest fp32 numbers are infinite, and infinity times a score of zero is not a number."""
+    from geoweave_b200 import _lib
+    from geoweave_b200.custom_flash_attn.packed_flash_attn import _scale
+
+    p, two = 4096, _lib.i64x2([64, 64])
+    fwd = lambda scale: lib.gw_packed_attn_fwd(p, p, p, _lib.GW_BF16, p, p, 1, 8, 8, 1, 1, 64, two, two, two, scale, 0, 0, p, None, None, None, 0,
+                                               None, None)
+    assert fwd(2.9e38) == fwd(2.4e38) == fwd(float("inf")) == -1
+    for scale in (1e-50, 2.4e38, 1e300, float("inf"), float("nan"), 0.0, -1.0):
+        with pytest.raises(ValueError):
+            _scale(scale, 64)
+    assert _scale(2.0 ** 127, 64) == 2.0 ** 127 and _scale(None, 64) == 0.125
