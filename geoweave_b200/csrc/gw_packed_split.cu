@@ -401,7 +401,7 @@ int64_t split_slots(const PackedParams& p, int chunk) { return p.total_k / chunk
 }  // namespace
 
 bool packed_split_fits(const PackedParams& p, int64_t max_q) {
-  return max_q > 0 && max_q * (p.H / p.Hk) <= kRows && p.Hk <= 65535;
+  return max_q > 0 && max_q <= kRows / (p.H / p.Hk) && p.Hk <= 65535;  // no product: the bound may be any 64-bit number
 }
 
 size_t packed_split_bytes(const PackedParams& p, int64_t max_q, int sms) {

@@ -165,3 +165,30 @@ def test_row_sums_come_from_the_output_before_its_rounding(form, D, dtype):
             limit = scale * (s_err @ K.abs() + lk * e * (dS.abs() @ K.abs())) + u * want.abs() + TINY[dtype]
             assert ((dq[a:a + lq, h].double() - want).abs() <= limit).all(), (form, h)
         a, c = a + lq, c + lk
+
+
+def test_a_bound_on_the_queries_may_be_any_number():
+    """Through C, where nothing clips it to the number of queries: a bound beyond 2^31, or whose product with the heads of a group passes 64
+    bits, says no more than none at all."""
+    from geoweave_b200 import _lib, check_status
+    from tests.gpu_util import dev
+
+    lib = _lib.load()
+    T, S, H, Hk, D = 40, 700, 8, 2, 64
+    g = torch.Generator().manual_seed(0)
+    q, k, v = [torch.randn(n, h, D, generator=g).bfloat16().to(dev()) for n, h in ((T, H), (S, Hk), (S, Hk))]
+    cu_q, cu_k = borders([T], dev()), borders([S], dev())
+    outs = []
+    for most in (0, T, 1 << 31, (1 << 32) + 1, 1 << 40, 1 << 62, (1 << 62) + 1, (1 << 63) - 1):
+        n = lib.gw_packed_attn_fwd_workspace_bytes(_lib.GW_BF16, 1, T, S, H, Hk, D, most)
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=dev())
+        outs.append(torch.empty_like(q))
+        strides = [_lib.i64x2((h * D, D)) for h in (H, Hk, Hk)]
+        rc = lib.gw_packed_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.GW_BF16, cu_q.data_ptr(), cu_k.data_ptr(), 1, T, S, H, Hk, D,
+                                    *strides, 0.125, 0, most, outs[-1].data_ptr(), None, None, ws.data_ptr(), n, _lib.status_word(dev()).data_ptr(),
+                                    _lib.stream_ptr(dev()))
+        _lib.check(rc, "gw_packed_attn_fwd")
+        assert n == lib.gw_packed_attn_fwd_workspace_bytes(_lib.GW_BF16, 1, T, S, H, Hk, D, 0)
+    check_status()
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
