@@ -15,6 +15,9 @@ int check_packed(const PackedParams& p, int dtype, int* dev, DeviceFacts* facts)
   const int64_t es = static_cast<int64_t>(dtype_size(dtype));
   for (const void* t : {p.q, p.k, p.v, static_cast<const void*>(p.o), static_cast<const void*>(p.o_low)})
     if (!aligned16(t)) return GW_ERR_INVALID_ARG;
+  for (const void* t : {static_cast<const void*>(p.cu_q), static_cast<const void*>(p.cu_k), static_cast<const void*>(p.lse),
+                        static_cast<const void*>(p.delta), static_cast<const void*>(p.status)})
+    if (reinterpret_cast<uintptr_t>(t) % 4 != 0) return GW_ERR_INVALID_ARG;
   for (const int64_t s : {p.qs[0], p.qs[1], p.ks[0], p.ks[1], p.vs[0], p.vs[1]})
     if (s <= 0 || s * es % 16 != 0) return GW_ERR_INVALID_ARG;
   const int rc = device_facts(dev, facts);
@@ -96,6 +99,7 @@ extern "C" int gw_packed_attn_bwd(const void* q, const void* k, const void* v, c
   p.o_low = dtype == GW_F32 ? nullptr : const_cast<void*>(out_low);
   p.lse = const_cast<float*>(lse);
   p.d_o = d_out;
+  p.delta = static_cast<float*>(workspace);
   p.dq = dq; p.dk = dk; p.dv = dv;
   p.dos[0] = d_out_strides[0];
   p.dos[1] = d_out_strides[1];
@@ -108,7 +112,6 @@ extern "C" int gw_packed_attn_bwd(const void* q, const void* k, const void* v, c
   for (const int64_t s : {p.dos[0], p.dos[1]})
     if (s <= 0 || s * static_cast<int64_t>(dtype_size(dtype)) % 16 != 0) return GW_ERR_INVALID_ARG;
   if (total_q > 0 && (!workspace || workspace_bytes < gw_packed_attn_bwd_workspace_bytes(total_q, H))) return GW_ERR_WORKSPACE;
-  p.delta = static_cast<float*>(workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return dtype == GW_F32 ? packed_plain_bwd(p, st) : packed_mma_bwd(p, dtype, dev, facts.sms, st);
 }

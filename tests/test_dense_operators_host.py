@@ -124,3 +124,16 @@ def test_scales_that_fp32_cannot_hold_are_refused(lib):
         with pytest.raises(ValueError):
             _scale(scale, 64)
     assert _scale(2.0 ** 127, 64) == 2.0 ** 127 and _scale(None, 64) == 0.125
+
+
+def test_pointers_between_the_words_that_they_point_to_are_refused(lib):
+    from geoweave_b200 import _lib
+
+    p, odd, two = 4096, 4098, _lib.i64x2([64, 64])
+    fwd = lambda cu_q=p, cu_k=p, lse=p, status=p: lib.gw_packed_attn_fwd(p, p, p, _lib.GW_BF16, cu_q, cu_k, 1, 8, 8, 1, 1, 64, two, two, two, 1.0, 0,
+                                                                         0, p, None, lse, None, 0, status, None)
+    bwd = lambda cu_q=p, cu_k=p, lse=p, status=p, ws=p: lib.gw_packed_attn_bwd(p, p, p, p, None, lse, p, _lib.GW_F16, cu_q, cu_k, 1, 8, 8, 1, 1, 64, two,
+                                                                               two, two, two, 1.0, 0, p, p, p, ws, 1 << 20, status, None)
+    for call, names in ((fwd, ("cu_q", "cu_k", "lse", "status")), (bwd, ("cu_q", "cu_k", "lse", "status", "ws"))):
+        for name in names:
+            assert call(**{name: odd}) == -1, name
