@@ -135,7 +135,7 @@ def packed_attention_backward(q, k, v, cu_seqlens_q, cu_seqlens_k, o, lse, d_out
         return tuple(x if x is None else x.zero_() for x in (dq, dk, dv))
     (q, qs), (k, ks), (v, vs), (d_out, ds) = _prepared(q), _prepared(k), _prepared(v), _prepared(d_out.to(q.dtype))
     o, lse = _prepared(o.contiguous())[0], lse.contiguous()
-    if o_low is not None and (o_low.shape != o.shape or o_low.dtype != o.dtype or not o_low.is_contiguous()):
+    if o_low is not None and (o_low.shape != o.shape or o_low.dtype != o.dtype or o_low.device != dev or not o_low.is_contiguous()):
         raise ValueError("o_low must be the forward's")
     nseq = cu_q.numel() - 1
     lib = _lib.load()

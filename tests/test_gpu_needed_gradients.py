@@ -67,3 +67,17 @@ def test_rotary(dtype, monkeypatch):
         for a, b, n in zip(every, _some(call, inputs, needed, up), needed):
             assert b is None if not n else torch.equal(a, b)
         assert turned[1] == backward
+
+
+def test_what_the_output_lost_must_be_on_the_same_device():
+    from geoweave_b200.custom_flash_attn.packed_flash_attn import packed_attention_backward, packed_attention_forward
+
+    x = torch.randn(20, 2, 64, dtype=torch.bfloat16, device="cuda")
+    cu, low = borders([20], x.device), torch.empty_like(x)
+    o, lse = packed_attention_forward(x, x, x, cu, return_lse=True, o_low=low)
+    packed_attention_backward(x, x, x, cu, None, o, lse, x, o_low=low)
+    for bad in (low.cpu(), low.float(), low[:10], low.transpose(0, 1)):
+        with pytest.raises(ValueError):
+            packed_attention_backward(x, x, x, cu, None, o, lse, x, o_low=bad)
+        with pytest.raises(ValueError):
+            packed_attention_forward(x, x, x, cu, o_low=bad)
