@@ -2,7 +2,7 @@
 //
 // Sequences lie back to back along the token axis; cu_q / cu_k (int32 [nseq + 1], on the device) hold their borders.  The
 // host never reads them: a grid is launched for the largest number of tiles that the totals allow,
-// floor(total / tile) + nseq, plus one, and each block finds its sequence by a warp-wide prefix sum over the lengths.
+// floor(total / tile) + nseq, plus one, and each block finds its sequence by a warp-wide search over the borders.
 // Blocks behind the last tile (one at least) share the rows behind the last sequence, which get zeros.
 #pragma once
 
@@ -55,46 +55,51 @@ __device__ __forceinline__ void packed_check(const PackedParams& p) {
   if (__any_sync(0xffffffffu, bad) && (threadIdx.x & 31) == 0) report_status(p.status, GW_ERR_INVALID_ARG);
 }
 
-// Warp-wide: tile `slot` of the list of all sequences' tiles (tile_rows rows each, along the q or the k side).  True
-// when there is such a tile.  Otherwise *tiles is the number of tiles and *end the row behind the last sequence.  All lanes get
-// the same answers.
+// The first slot of sequence b's tiles (b = nseq: the first slot behind all of them).  Sequence b has slots for one tile more than fit in front
+// of it: floor(border / R) + b rises by at least ceil(length / R) from b to b + 1, so every tile has a slot of its own, some slots stay
+// empty, and a slot's sequence is found by a search over the borders instead of a sum over all lengths.
+__device__ __forceinline__ int64_t packed_slot(const PackedParams& p, bool key_side, int tile_rows, int b) {
+  return packed_border(key_side ? p.cu_k : p.cu_q, b, key_side ? p.total_k : p.total_q) / tile_rows + static_cast<int64_t>(b);
+}
+
+// Warp-wide: the tile in `slot` of all sequences' tiles (tile_rows rows each, along the q or the k side).  True when there is one.
+// Otherwise *tiles is the first slot behind the last sequence (`slot` may lie in front of it, and be an empty one) and *end
+// the row there.  All lanes get the same answers.  32 borders are looked at in a step, so the steps are the logarithm of the number of
+// sequences to the base of 32: two for a thousand.
 __device__ __forceinline__ bool packed_find(const PackedParams& p, bool key_side, int tile_rows, int64_t slot, PackedSeq* out,
                                             int64_t* tiles, int64_t* end) {
   const int lane = threadIdx.x & 31;
-  int64_t base = 0;
-  for (int b0 = 0; b0 < p.nseq; b0 += 32) {
-    const int b = b0 + lane;
-    int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
-    if (b < p.nseq) {
-      q0 = packed_border(p.cu_q, b, p.total_q);
-      q1 = packed_border(p.cu_q, b + 1, p.total_q);
-      k0 = packed_border(p.cu_k, b, p.total_k);
-      k1 = packed_border(p.cu_k, b + 1, p.total_k);
-      q1 = max(q0, q1);
-      k1 = max(k0, k1);
-    }
-    const int n = static_cast<int>((static_cast<int64_t>(key_side ? k1 - k0 : q1 - q0) + tile_rows - 1) / tile_rows);
-    int64_t incl = n;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += up;
-    }
-    const int64_t total = __shfl_sync(0xffffffffu, incl, 31);
-    if (slot < base + total) {
-      const int src = __ffs(__ballot_sync(0xffffffffu, slot < base + incl)) - 1;
-      out->q0 = __shfl_sync(0xffffffffu, q0, src);
-      out->lq = __shfl_sync(0xffffffffu, q1, src) - out->q0;
-      out->k0 = __shfl_sync(0xffffffffu, k0, src);
-      out->lk = __shfl_sync(0xffffffffu, k1, src) - out->k0;
-      out->tile = static_cast<int>(slot - base - __shfl_sync(0xffffffffu, incl - n, src));
-      return true;
-    }
-    base += total;
-  }
-  *tiles = base;
+  *tiles = p.nseq > 0 ? packed_slot(p, key_side, tile_rows, p.nseq) : 0;
   *end = p.nseq > 0 ? packed_border(key_side ? p.cu_k : p.cu_q, p.nseq, key_side ? p.total_k : p.total_q) : 0;
-  return false;
+  if (slot >= *tiles) return false;
+  int lo = 0, hi = p.nseq;  // the sequence is one of these
+  while (hi - lo > 32) {
+    const int step = (hi - lo + 31) / 32, b = lo + lane * step;
+    const unsigned here = __ballot_sync(0xffffffffu, lane == 0 || (b < hi && packed_slot(p, key_side, tile_rows, b) <= slot));
+    lo += (31 - __clz(here)) * step;
+    hi = min(hi, lo + step);
+  }
+  const int b = lo + lane;
+  int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+  if (b < hi) {
+    q0 = packed_border(p.cu_q, b, p.total_q);
+    q1 = packed_border(p.cu_q, b + 1, p.total_q);
+    k0 = packed_border(p.cu_k, b, p.total_k);
+    k1 = packed_border(p.cu_k, b + 1, p.total_k);
+    q1 = max(q0, q1);
+    k1 = max(k0, k1);
+  }
+  const int64_t at = slot - ((key_side ? k0 : q0) / tile_rows + static_cast<int64_t>(b));
+  const unsigned here = __ballot_sync(0xffffffffu, b < hi && at >= 0);
+  if (here == 0) return false;
+  const int src = 31 - __clz(here);
+  out->q0 = __shfl_sync(0xffffffffu, q0, src);
+  out->lq = __shfl_sync(0xffffffffu, q1, src) - out->q0;
+  out->k0 = __shfl_sync(0xffffffffu, k0, src);
+  out->lk = __shfl_sync(0xffffffffu, k1, src) - out->k0;
+  const int64_t tile = __shfl_sync(0xffffffffu, at, src);
+  out->tile = static_cast<int>(tile);
+  return tile < (static_cast<int64_t>(key_side ? out->lk : out->lq) + tile_rows - 1) / tile_rows;
 }
 
 // Tiles of a sequence whose work is at least x (in tiles of the other side); the work of a tile is the number of keys (key side:
@@ -145,7 +150,12 @@ __device__ __forceinline__ bool packed_find_sorted(const PackedParams& p, bool k
     for (int i = 0; i < SETS; ++i) n += packed_at_least(p, key_side, R, lq[i], lk[i], x);
     return static_cast<int64_t>(__reduce_add_sync(0xffffffffu, static_cast<unsigned>(n)));
   };
-  if (rank >= count(0)) return packed_find(p, key_side, R, rank, out, tiles, end);
+  const int64_t all = count(0);
+  if (rank >= all) {
+    *tiles = all;
+    *end = p.nseq > 0 ? packed_border(key_side ? p.cu_k : p.cu_q, p.nseq, key_side ? p.total_k : p.total_q) : 0;
+    return false;
+  }
   int lo = 0, hi = top;  // the largest x with more than `rank` tiles of that much work
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -181,10 +191,12 @@ __device__ __forceinline__ bool packed_find_sorted(const PackedParams& p, bool k
   return false;  // not reached: the counts above say that the tile exists
 }
 
-// The rows of one head behind the last sequence, shared by the blocks `part` of `parts`, each with its first `threads` threads.
+// The rows of one head behind the last sequence, shared by the blocks `part` of `parts`, each with its first `threads` threads.  Nothing
+// for the blocks of empty slots, whose part is negative.
 template <typename T>
 __device__ __forceinline__ void packed_zero_rows(void* out, float* lse, int64_t from, int64_t to, int heads, int head, int D, int64_t part,
                                                  int64_t parts, int threads) {
+  if (part < 0) return;
   T* dst = static_cast<T*>(out);
   const int64_t n = (to - from) * D;
   for (int64_t i = part * threads + threadIdx.x; i < n; i += parts * threads)

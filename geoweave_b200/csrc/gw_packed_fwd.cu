@@ -148,14 +148,20 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     for (int64_t at = blockIdx.x; ok; at += gridDim.x, ++i) {
       FwdItem w{};
       const int parts = TILES == 1 ? fp.count : 1;
+      PackedSeq seq{};
+      int64_t rank, tiles = 0;
+      bool found = false;
+      for (;; at += gridDim.x) {  // past the empty slots
+        rank = at / parts / p.H;
+        if (rank >= slots) break;
+        found = packed_find_sorted(p, false, TILES * kTile, rank, &seq, &tiles, &w.end);
+        if (found || rank >= tiles) break;
+      }
       w.part = static_cast<int>(at % parts);
       w.head = static_cast<int>(at / parts % p.H);
-      const int64_t rank = at / parts / p.H;
-      PackedSeq seq{};
-      int64_t tiles = 0;
       if (rank >= slots) {
         w.kind = kItemEnd;
-      } else if (packed_find_sorted(p, false, TILES * kTile, rank, &seq, &tiles, &w.end)) {
+      } else if (found) {
         w.kind = kItemRows;
         w.q0 = seq.q0;
         w.lq = seq.lq;

@@ -206,7 +206,7 @@ __device__ __forceinline__ float prob(float s, float c2, float lse) {
 }
 
 template <int DP>
-__global__ void __launch_bounds__(NT) plain_dq_kernel(const PackedParams p) {
+__global__ void __launch_bounds__(NT, DP == 64 ? 2 : 1) plain_dq_kernel(const PackedParams p) {
   extern __shared__ float smem[];
   float *qt = smem, *dt = qt + BT * (DP + 4), *kt = dt + BT * (DP + 4), *vt = kt + BT * (DP + 4), *w = vt + BT * (DP + 4);
   const int head = blockIdx.y, kv = head / (p.H / p.Hk), ty = threadIdx.x >> 4, tx = threadIdx.x & 15;

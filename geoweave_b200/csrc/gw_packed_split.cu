@@ -265,9 +265,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_join_kernel(const SplitPa
     wait_for_predecessor();  // every block: the kernel must not end before the chunks do
     if (r > 0) return;
     if (kv == 0 && warp == 0) packed_check(p);
-    PackedSeq s;
-    int64_t tiles, end;
-    packed_find(p, false, 1, static_cast<int64_t>(0x7fffffffffffffff), &s, &tiles, &end);
+    const int64_t end = p.nseq > 0 ? packed_border(p.cu_q, p.nseq, p.total_q) : 0;
     for (int h = kv * group; h < (kv + 1) * group; ++h) packed_zero_rows<T>(p.o, p.lse, end, p.total_q, p.H, h, p.D, 0, 1, blockDim.x);
     return;
   }
@@ -282,13 +280,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_join_kernel(const SplitPa
     wait_for_predecessor();
     return;
   }
-  int64_t before = 0;  // chunks in front of this sequence
-  for (int i = lane; i < b; i += 32) {
-    const int c0 = packed_border(p.cu_k, i, p.total_k), c1 = packed_border(p.cu_k, i + 1, p.total_k);
-    before += (static_cast<int64_t>(max(0, c1 - c0)) + sp.chunk - 1) / sp.chunk;
-  }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
+  const int64_t before = packed_slot(p, true, sp.chunk, b);  // the sequence's first chunk
   wait_for_predecessor();
   const int64_t left = sp.slots - before;
   const int chunks = static_cast<int>(min((static_cast<int64_t>(lk) + sp.chunk - 1) / sp.chunk, left < 0 ? 0 : left));
