@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(BwdShape<DP>::kThreads, BwdShape<DP>::kBlocks)
 packed_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                  const __grid_constant__ CUtensorMap tmG, const PackedParams p, const int ab_format) {
   using Shape = BwdShape<DP>;
-  constexpr int SK = Shape::kStagesK, SV = Shape::kStagesV;  // key tiles by which K runs ahead of V
+  constexpr int SK = Shape::kStagesK, SV = Shape::kStagesV;  // depths of the rings of K and V
   constexpr int TB = Shape::kOwnBytes, W = Shape::kWalk, WB = Shape::kWalkBytes;
   constexpr uint32_t kS = 0, kDp = W, kDs = 2 * W, kDq = Shape::kColumns - DP;
   extern __shared__ unsigned char smem_raw[];
@@ -731,11 +731,13 @@ int launch_bwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t 
   if (p.dk == nullptr) return GW_OK;  // keys and values without a gradient
   if (W != kTile && maps(W, kTile) != GW_OK) return rc;
   // Few and long blocks -- grouped heads, whose key tiles walk every head of the group -- leave SMs idle at the end: two share a key
-  // tile.  One sequence of 4099 tokens, 2 key heads of 64 under 16: 436 us against 676 for the whole training step; ragged
-  // prompts, 4 key heads of 128: 556 against 594.  Not for more than two and a half rounds of blocks (8328 tokens, 16 heads: 1590
-  // against 1563) nor for less than 24 pairs of tiles a block (views of 1041 tokens, 16 heads: 190 against 167).
+  // tile.  Training steps, alone -> shared.  One causal sequence of 4099 tokens, 2 key heads of 64 under 16: 687 -> 447 us; of 128:
+  // 670 -> 466; ragged prompts, 4 key heads of 128 (1.74 rounds of blocks): 563 -> 518.  Not where a round or two more are
+  // needed (8 views of 1041 tokens, 4 key heads of 128, 1.78 rounds: 446 -> 475; 8200 causal tokens, 1.76: 1187 -> 1189), nor for
+  // few pairs of tiles (200 queries, 2 heads a group, 8 pairs: 99 -> 110; 2 views of 1041 tokens, 2 heads a group of 128, 16 pairs:
+  // 95 -> 85), nor for heads of their own (4099 tokens, 16 heads of 64: 451 -> 480, of 128: 623 -> 679).
   const int64_t items = (p.total_k + kTile - 1) / kTile * p.Hk, at_once = static_cast<int64_t>(sms) * BwdShape<DP>::kBlocks;
-  const bool share = 2 * items < 5 * at_once && p.total_q * (p.H / p.Hk) >= 24 * static_cast<int64_t>(W) * p.nseq;
+  const bool share = p.H > p.Hk && 4 * items < 7 * at_once && p.total_q * (p.H / p.Hk) >= 16 * static_cast<int64_t>(W) * p.nseq;
   if (!share) {
     packed_dkv_kernel<T, DP, 1><<<static_cast<unsigned>(k_items), kThreads, smem, st>>>(mq, mk, mv, mg, p, format);
     GW_LAUNCH_CHECK();
