@@ -69,9 +69,6 @@ __device__ __forceinline__ int64_t packed_slot(const PackedParams& p, bool key_s
 __device__ __forceinline__ bool packed_find(const PackedParams& p, bool key_side, int tile_rows, int64_t slot, PackedSeq* out,
                                             int64_t* tiles, int64_t* end) {
   const int lane = threadIdx.x & 31;
-  *tiles = p.nseq > 0 ? packed_slot(p, key_side, tile_rows, p.nseq) : 0;
-  *end = p.nseq > 0 ? packed_border(key_side ? p.cu_k : p.cu_q, p.nseq, key_side ? p.total_k : p.total_q) : 0;
-  if (slot >= *tiles) return false;
   int lo = 0, hi = p.nseq;  // the sequence is one of these
   while (hi - lo > 32) {
     const int step = (hi - lo + 31) / 32, b = lo + lane * step;
@@ -91,15 +88,19 @@ __device__ __forceinline__ bool packed_find(const PackedParams& p, bool key_side
   }
   const int64_t at = slot - ((key_side ? k0 : q0) / tile_rows + static_cast<int64_t>(b));
   const unsigned here = __ballot_sync(0xffffffffu, b < hi && at >= 0);
-  if (here == 0) return false;
-  const int src = 31 - __clz(here);
-  out->q0 = __shfl_sync(0xffffffffu, q0, src);
-  out->lq = __shfl_sync(0xffffffffu, q1, src) - out->q0;
-  out->k0 = __shfl_sync(0xffffffffu, k0, src);
-  out->lk = __shfl_sync(0xffffffffu, k1, src) - out->k0;
-  const int64_t tile = __shfl_sync(0xffffffffu, at, src);
-  out->tile = static_cast<int>(tile);
-  return tile < (static_cast<int64_t>(key_side ? out->lk : out->lq) + tile_rows - 1) / tile_rows;
+  if (here != 0) {
+    const int src = 31 - __clz(here);
+    out->q0 = __shfl_sync(0xffffffffu, q0, src);
+    out->lq = __shfl_sync(0xffffffffu, q1, src) - out->q0;
+    out->k0 = __shfl_sync(0xffffffffu, k0, src);
+    out->lk = __shfl_sync(0xffffffffu, k1, src) - out->k0;
+    const int64_t tile = __shfl_sync(0xffffffffu, at, src);
+    out->tile = static_cast<int>(tile);
+    if (tile < (static_cast<int64_t>(key_side ? out->lk : out->lq) + tile_rows - 1) / tile_rows) return true;
+  }
+  *tiles = p.nseq > 0 ? packed_slot(p, key_side, tile_rows, p.nseq) : 0;
+  *end = p.nseq > 0 ? packed_border(key_side ? p.cu_k : p.cu_q, p.nseq, key_side ? p.total_k : p.total_q) : 0;
+  return false;
 }
 
 // Tiles of a sequence whose work is at least x (in tiles of the other side); the work of a tile is the number of keys (key side:
