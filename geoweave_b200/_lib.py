@@ -178,8 +178,10 @@ def require_cuda(*tensors) -> torch.device:
 def wants_autograd(*tensors) -> bool:
     """Whether a call has to go through its autograd function: an input requires grad, or carries a forward-mode tangent, which the
     function then refuses (NotImplementedError); a call around it would drop the tangent without a word."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        return True
+    if torch.is_grad_enabled():
+        for t in tensors:  # a generator would cost as much as the rest of the call's checks
+            if t.requires_grad:
+                return True
     return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
