@@ -12,6 +12,9 @@
 // make P and dS in registers (a thread owns a row of its 64 columns) and put them back into tensor memory as 16-bit A operands of
 // the accumulating products, whose B operand is the tile that is in shared memory already, read along its rows.  The key-side
 // kernel works on the transposes (rows are keys), so neither P nor dS is ever transposed.
+//
+// P and dS are rounded to the inputs' type, the only one that may stand beside the tile of the other operand, once each: with bf16 dq and dk
+// are off by 0.0024 of their norm, of which the last rounding alone makes 0.0017.  All else (S, dP, D, lse, the sums) is fp32.
 #include <type_traits>
 
 #include "gw_packed_mma.cuh"

@@ -305,6 +305,8 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           if (!v_here) {
             ok = ok && warp_wait(&sh->v_full[st], ((ring + j) / ST) & 1, &sh->abort_flag);
             if (DP != 64 && j + 1 < mine) ok = ok && warp_wait(&sh->k_full[st_next], ((ring + j + 1) / ST) & 1, &sh->abort_flag);
+            // With an issuer for each tile both clear these rows, one perhaps while the other's product reads them: zeros over the zeros
+            // that it wrote itself and waited for.
             if (ok && (j + 1) * kTile > lk) zero_rows_from<DP>(v_smem + st * TB, lk - j * kTile);
             v_here = true;
           }
@@ -442,6 +444,9 @@ packed_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         const float base = m == -INFINITY ? 0.f : -m * c;
         const uint64_t c2 = pack_f2(c, c), base2 = pack_f2(base, base);
         uint64_t sum[2] = {0, 0};
+        // P as an operand of the second product has the inputs' type, the only one that may stand beside V: off by half a step at most, and
+        // o by 0.0010 (37 keys) to 0.0016 of its norm (4000) in bf16, beside the 0.0017 of its own rounding; fp16 an eighth.  P as two
+        // operands would keep more and double that product.  l is summed from P before its rounding.
         uint32_t pk[64];
         auto exponentials = [&](int from, int to) {
 #pragma unroll
@@ -612,12 +617,12 @@ int launch_fwd(const PackedParams& p, int dtype, int dev, int sms, int parts, vo
 }
 
 // Rows for fewer blocks of two tiles than there are SMs: one tile a block, twice the blocks (one view of 1041 tokens, 16 heads: 20.5 us
-// against 26.6; 1041 rows against 33 312 keys: 274 against 379).  With three views the two are equal, with 32 two tiles
-// win, 269 us against 340, since both share every key tile.
+// against 26.6; 1041 rows against 33 312 keys: 274 against 383).  With three views the two are close, 43 and 45, with 32 two tiles
+// win, 290 us against 357, since both share every key tile.  (Each alone, with cold caches.)
 bool few_rows(const PackedParams& p, int sms) { return (p.total_q + 2 * kTile - 1) / (2 * kTile) * p.H < sms; }
 
 // Fewer row tiles than half the SMs, and keys enough for at least six key tiles a part: the keys are divided too (300 rows, 8 heads
-// against 8328 keys: 30 us against 78; 1041 rows, 4 heads against 33 312: 88 against 274).  With nine key tiles in two parts
+// against 8328 keys: 29 us against 76; 1041 rows, 4 heads against 33 312: 87 against 274).  With nine key tiles in two parts
 // the second kernel costs what they bring (23.6 against 20.5).
 int key_parts(const PackedParams& p, int sms) {
   int64_t tiles = (p.total_q + kTile - 1) / kTile;

@@ -173,7 +173,7 @@ split_mma_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     m1 = t1;
     l0 *= f0;
     l1 *= f1;
-    uint32_t pa[NT][2];
+    uint32_t pa[NT][2];  // P in the inputs' type, as the product with V needs it; l is summed before that rounding
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const float a = exp2_fast(sc[t][0] - b0), b = exp2_fast(sc[t][1] - b0), d = exp2_fast(sc[t][2] - b1), e = exp2_fast(sc[t][3] - b1);
@@ -380,8 +380,8 @@ int launch_split(const SplitParams& sp, int max_q, int dtype, int dev, cudaStrea
 }
 
 // Chunks of a size that gives every SM about four blocks, two at a time: with eight the fixed cost of a block shows (24 caches of 129 to
-// 33 312 keys, 4 key heads: 52 us against 48; one cache of 33 312 keys, 16 key heads: 50 against 44), with two the uneven ends of ragged
-// caches do (16 key heads: 130 against 125).  No shorter than two steps of a block's warps.
+// 33 312 keys, 4 key heads: 49 us against 45; one cache of 33 312 keys, 16 key heads: 47 against 41), with two the uneven ends of ragged
+// caches do (16 key heads: 131 against 121).  No shorter than two steps of a block's warps.
 int chunk_keys(int64_t total_k, int Hk, int sms) {
   const int64_t want = total_k * Hk / (4 * static_cast<int64_t>(sms));
   const int64_t c = (want + 127) / 128 * 128;

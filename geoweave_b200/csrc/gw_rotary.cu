@@ -11,10 +11,11 @@
 // Bound by memory: q and k are read once and written once.  A thread owns one piece of the columns (V pairs, or V copied
 // columns) of one token and walks the heads, so cosines and sines are loaded once for all heads; V is the widest piece of at
 // most 16 bytes that the widths, strides and pointers allow.  Blocks stay and take tokens gridDim apart: 33 312 tokens of 16 + 16
-// heads of 64 in bf16, sliced from a projection's output, 58 us = 4.7 TB/s (64 us with a block for every four tokens; a copy of as
-// many contiguous bytes takes 45 us); fp32 5.4 TB/s.  Looked at and dropped: whole 16-byte pieces a lane with the partners
-// found through shared memory (104 us: the registers for two angles a column halve the occupancy), loads ahead of the position (96 us,
-// the same), other block sizes.  Without the position and angle loads it takes 56 us, so they are not the bound.
+// heads of 64 in bf16, sliced from a projection's output, 58 us a pass among others = 4.7 TB/s (64 with a block for every four tokens; a
+// copy of as many contiguous bytes takes 45 us), 61 us alone with cold caches; fp32 5.4 TB/s.  Looked at and dropped: whole
+// 16-byte pieces a lane with the partners found through shared memory (104 us: the registers for two angles a column halve
+// the occupancy), loads ahead of the position (96 us, the same), other block sizes.  Without the position and angle loads it
+// takes 56 us, so they are not the bound.
 #include "gw_common.cuh"
 
 namespace gw {
@@ -22,9 +23,9 @@ namespace {
 
 constexpr int kAxes = 4;
 constexpr int kThreads = 256;
-// Blocks an SM, and so registers a thread: with whole 16-byte pieces the compiler needs more (fp32, 33 312 tokens: 94 us with four
-// against 103 with six; bf16 heads of 128: 41 against 47), with 8-byte ones more threads are better (bf16, 12-column halves: 61
-// with six against 72 with four).
+// Blocks an SM, and so registers a thread (33 312 tokens, alone with cold caches): with whole 16-byte pieces the compiler needs more
+// (fp32: 93 us with four against 102 with six; bf16, two axes: 53 against 60), with 8-byte ones more threads are better (bf16,
+// three axes, 12-column halves: 61 with six against 69 with four).
 template <typename T, int V>
 constexpr int kBlocksPerSm = sizeof(T) * V >= 16 ? 4 : 6;
 

@@ -178,8 +178,14 @@ def packed_flash_attn_func(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal: boo
     ``Hk``: query head ``h`` reads key head ``h // (H // Hk)``).  ``cu_seqlens_q``, ``cu_seqlens_k`` int32 ``[sequences + 1]``
     on the same device: sequence ``b`` holds rows ``cu[b]`` to ``cu[b + 1]``; ``cu_seqlens_k=None`` means the queries' own
     tokens.  ``causal``: the last query of a sequence sees all its keys, the one before it one key less, and so on.
-    ``max_seqlen_q``: an upper bound on the queries of one sequence, if the caller knows one; with few queries (single new
-    tokens) the work is then divided along the keys.  A bound that is too small sets the status word and leaves rows unwritten.
+    ``max_seqlen_q``: an upper bound on the queries of one sequence, if the caller knows one.  Up to 16 query rows a key head
+    (queries times heads of a group) the work is then divided along the keys; without the bound such a batch takes the kernel for prompts, where each
+    query head reads all keys for a tile of rows that is almost empty: give it for single new tokens, where it decides a factor.
+    A bound that is too small sets the status word and leaves rows unwritten.
+
+    Under autograd a 16-bit call keeps, beside its output, a second tensor of that size until the backward pass: what rounding the output took
+    off, for exact row sums.  Without gradients (``packed_flash_attn_inference_func``) there is none.  Derivatives are first-order and
+    backward only: forward-mode tangents and second derivatives are refused.
 
     Rows without an allowed key and rows behind the last sequence give zeros (gradients too).  Non-finite values of ``k`` and
     ``v`` stay within their own sequence; within a causal sequence they may also reach rows before them.

@@ -310,12 +310,12 @@ int gw_project_fused(const void* x, const void* weight, const void* bias, int dt
  * cu_k[b] .. cu_k[b+1] of k and v (int32 [nseq + 1] on the device, starting at 0, not decreasing, within the totals; anything
  * else sets the status word, and no access leaves the tensors).  causal: query i of lq sees the keys 0 .. i + lk - lq of lk.
  * out [total_q, H, D] contiguous; lse fp32 [H, total_q], nullable; out_low like out, nullable: what rounding out to 16 bits took
- * off, for the backward pass (unused with GW_F32).  A row without an allowed key gets out = 0 and
+ * off, for exact row sums in the backward pass (unused with GW_F32).  A row without an allowed key gets out = 0 and
  * lse = -inf, as do the rows behind the last sequence.  Non-finite values of k and v stay within their own sequence.
  * max_q: no sequence has more query rows (0: unknown).  It may only choose the kernel: a longer sequence sets the status
  * word and its rows further on are not written.
  * Requirements: D <= 128 and a multiple of 8, H a multiple of Hk, H <= 65535; 16-byte aligned pointers and strides;
- *               scale > 0.  workspace: gw_packed_attn_fwd_workspace_bytes(same arguments) bytes (null where that is 0).
+ *               scale > 0 and scale log2 e finite in fp32.  workspace: gw_packed_attn_fwd_workspace_bytes(same arguments) bytes (null where that is 0).
  * No reference counterpart: there the dense blocks call the framework's own dense attention.
  * ---------------------------------------------------------------------------------------------- */
 size_t gw_packed_attn_fwd_workspace_bytes(int dtype, int nseq, int64_t total_q, int64_t total_k, int H, int Hk, int D, int64_t max_q);
