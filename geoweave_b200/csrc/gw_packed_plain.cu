@@ -66,10 +66,18 @@ __device__ __forceinline__ void dot_tile(float (&acc)[R][4], const float* a, con
     }
 }
 
-// acc[i][c] += sum_k w[ty*R+i][k] * m[k][column c of this thread]; columns tx*4 + 64*(c/4) + c%4, two to a packed value
+// acc[i][c] += sum_k w[ty*R+i][k] * m[k][column c of this thread]; columns tx*4 + 64*(c/4) + c%4, two to a packed value.  The tile's
+// 64 products are summed by themselves first: a sum of n products in one go is off by about 2^-24 sqrt(n / 6) of its size, this one by
+// sqrt(64 / 6) and sqrt(n / 384) (gradients of a key head under eight over 1348 causal tokens: 1.7e-6 -> 5e-7 of their norm).  A single
+// row unrolls all steps: 24 single tokens of 16 heads over 4 against 129 to 33 312 keys 242 us, 255 with four steps at a time.
 template <int DP, int R>
 __device__ __forceinline__ void accumulate(uint64_t (&acc)[R][DP / 32], const float* w, const float* m, int ty, int tx) {
-#pragma unroll 4
+  uint64_t part[R][DP / 32];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) part[i][c] = 0;
+#pragma unroll (R == 1 ? BT / 4 : 4)
   for (int k = 0; k < BT; k += 4) {
     float4 wv[R];
 #pragma unroll
@@ -82,11 +90,15 @@ __device__ __forceinline__ void accumulate(uint64_t (&acc)[R][DP / 32], const fl
 #pragma unroll
         for (int i = 0; i < R; ++i) {
           const float x = kk == 0 ? wv[i].x : kk == 1 ? wv[i].y : kk == 2 ? wv[i].z : wv[i].w;
-          acc[i][c] = fma_f2(pack_f2(x, x), mv.x, acc[i][c]);
-          acc[i][c + 1] = fma_f2(pack_f2(x, x), mv.y, acc[i][c + 1]);
+          part[i][c] = fma_f2(pack_f2(x, x), mv.x, part[i][c]);
+          part[i][c + 1] = fma_f2(pack_f2(x, x), mv.y, part[i][c + 1]);
         }
       }
   }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) acc[i][c] = add_f2(acc[i][c], part[i][c]);
 }
 
 template <int DP>

@@ -10,7 +10,7 @@ import math
 import pytest
 import torch
 
-from tests.packed_reference import HALF, TINY, borders
+from tests.packed_reference import HALF, TINY, borders, packed_reference
 
 pytestmark = pytest.mark.gpu
 
@@ -192,3 +192,41 @@ def test_a_bound_on_the_queries_may_be_any_number():
     check_status()
     for o in outs[1:]:
         assert torch.equal(o, outs[0])
+
+
+@pytest.mark.parametrize("lens_q,lens_k,H,Hk,D,causal", [
+    ([1348, 33], [1348, 33], 16, 2, 64, True), ([447] * 4, [447] * 4, 16, 2, 32, True), ([2, 2], [6982, 2327], 8, 1, 80, False), ([900], [900], 8, 1, 128, True),
+    ([1, 1], [40000, 9000], 4, 4, 64, False),
+])
+def test_fp32_sums_over_thousands_of_rows_stay_exact(lens_q, lens_k, H, Hk, D, causal):
+    """The error's norm against 64 bits, in half steps u = 2^-24 of the result's, as a root of these squares, times 1.6, since weights of different
+    sizes make a sum's steps uneven:
+      * a sum of n products of either sign in one go: n / 6, for its k-th partial sum is sqrt(k / n) of the whole and rounded once, by
+        u / sqrt(3) of itself on average (16 to 82 u here); in two levels, 64 products and then n / 64 sums: 64 / 6 + n / 384;
+      * a score, a sum of D products and 1.5 in size, moves its P by 1.5 sqrt(D / 6) u; dP, for dq and dk, is off by sqrt(D / 6) u of itself;
+      * the gradients' P = 2^(S log2 e - lse log2 e): with X = log2 e (ln n + 1.2) for the size of lse and h u the half step of numbers of
+        that size (h = 8 from 8 to 16), lse, its product with log2 e and the difference are rounded once each, which moves P by
+        h, h ln 2 and h ln 2 over sqrt(3) at most: 0.65 h^2;
+      * exp and the last rounding: 2 u.
+    (First written as 14 u for every case, then without dP's and the exponents' own roundings: errors of 14.1, 12.8 and 12.6 u, of dq, dq and dk,
+    showed that terms were missing, not digits.)"""
+    from geoweave_b200 import check_status
+    from geoweave_b200.custom_flash_attn import packed_flash_attn_func
+
+    g = torch.Generator().manual_seed(H + D)
+    mk = lambda n, h, size=1.0: (torch.randn(n, h, D, generator=g) * size).cuda()
+    q, k, v, up = mk(sum(lens_q), H, 1.5), mk(sum(lens_k), Hk), mk(sum(lens_k), Hk), mk(sum(lens_q), H)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    most = 1 if max(lens_q) == 1 else None
+    o = packed_flash_attn_func(*leaves, borders(lens_q, q.device), borders(lens_k, q.device), causal, None, most)
+    got = (o, *torch.autograd.grad(o, leaves, up))
+    check_status()
+    ref = packed_reference(q.detach(), k.detach(), v.detach(), lens_q, lens_k, causal, D ** -0.5, up)
+    for name, x in zip(("o", "dq", "dk", "dv"), got):
+        value = ref[name][0]
+        off = (x.double() - value).norm() / value.norm()
+        n = max(lens_k) if name in ("o", "dq") else max(lens_q) * (H // Hk)
+        h = 2.0 ** math.floor(math.log2((math.log(max(lens_k)) + 1.2) / math.log(2)))
+        squares = 64 / 6 + n / 384 + 1.5 ** 2 * D / 6 + 4 + (D / 6 if name in ("dq", "dk") else 0) + (0 if name == "o" else 0.65 * h * h)
+        limit = 1.6 * math.sqrt(squares)
+        assert off <= limit * 2.0 ** -24, f"{name}: {off * 2 ** 24:.1f} half steps, at most {limit:.1f}"
