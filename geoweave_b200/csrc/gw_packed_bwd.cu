@@ -734,11 +734,11 @@ int launch_bwd(const PackedParams& p, int dtype, int dev, int sms, cudaStream_t 
   if (p.dk == nullptr) return GW_OK;  // keys and values without a gradient
   if (W != kTile && maps(W, kTile) != GW_OK) return rc;
   // Few and long blocks -- grouped heads, whose key tiles walk every head of the group -- leave SMs idle at the end: two share a key
-  // tile.  Training steps, alone -> shared.  One causal sequence of 4099 tokens, 2 key heads of 64 under 16: 687 -> 447 us; of 128:
-  // 670 -> 466; ragged prompts, 4 key heads of 128 (1.74 rounds of blocks): 563 -> 518.  Not where a round or two more are
-  // needed (8 views of 1041 tokens, 4 key heads of 128, 1.78 rounds: 446 -> 475; 8200 causal tokens, 1.76: 1187 -> 1189), nor for
-  // few pairs of tiles (200 queries, 2 heads a group, 8 pairs: 99 -> 110; 2 views of 1041 tokens, 2 heads a group of 128, 16 pairs:
-  // 95 -> 85), nor for heads of their own (4099 tokens, 16 heads of 64: 451 -> 480, of 128: 623 -> 679).
+  // tile.  Training steps, alone -> shared.  One causal sequence of 4099 tokens, 2 key heads of 64 under 16: 687 -> 447 us, of 128
+  // 670 -> 466; ragged prompts, 4 key heads of 128 (1.74 rounds of blocks) 563 -> 518.  Not beyond: 8200 causal tokens (1.76 rounds)
+  // 1187 -> 1189, 8 views of 1041 tokens, 4 key heads of 128 (1.78) 446 -> 475.  With 16 pairs of tiles and more for a block: 2 views of 1041
+  // tokens, 4 key heads of 128 under 8 (16 pairs) 95 -> 85, 200 queries of 16 heads over 8 (8 pairs) 99 -> 110.  Not for heads of their
+  // own: 4099 tokens, 16 heads of 64 451 -> 480, of 128 623 -> 679.
   const int64_t items = (p.total_k + kTile - 1) / kTile * p.Hk, at_once = static_cast<int64_t>(sms) * BwdShape<DP>::kBlocks;
   const bool share = p.H > p.Hk && 4 * items < 7 * at_once && p.total_q * (p.H / p.Hk) >= 16 * static_cast<int64_t>(W) * p.nseq;
   if (!share) {

@@ -78,6 +78,24 @@ def test_short_and_long_sequences_among_a_thousand(dtype, causal):
     assert_within("lse", lse, ref["lse"])
 
 
+@pytest.mark.parametrize("n", [66, 70, 74])
+def test_divided_keys_of_many_sequences(n):
+    """One head and just over 64 sequences of long keys: slots that stay empty, and each row's keys in two parts."""
+    from geoweave_b200 import check_status
+    from geoweave_b200.custom_flash_attn import packed_flash_attn_inference_func
+
+    g = torch.Generator().manual_seed(n)
+    lens_q, lens_k = [3 + i % 5 if i % 11 else 0 for i in range(n)], [2100 + 17 * i if i % 13 else 0 for i in range(n)]
+    mk = lambda rows: torch.randn(rows, 1, 64, generator=g).bfloat16().cuda()
+    q, k, v = mk(sum(lens_q)), mk(sum(lens_k)), mk(sum(lens_k))
+    for causal in (False, True):
+        ref = packed_reference(q, k, v, lens_q, lens_k, causal, 0.125)
+        o, lse = packed_flash_attn_inference_func(q, k, v, borders(lens_q, q.device), borders(lens_k, q.device), causal, return_lse=True)
+        check_status()
+        assert_within("o", o, ref["o"])
+        assert_within("lse", lse, ref["lse"])
+
+
 def test_finding_a_tile_does_not_cost_a_look_at_every_sequence():
     """300 000 sequences: with work for each tile that grows with their number this took minutes; it is some tens of milliseconds."""
     from geoweave_b200.custom_flash_attn import packed_flash_attn_func, packed_flash_attn_inference_func
