@@ -54,10 +54,11 @@ def rotary_axes(widths: Sequence[int], max_position: int, device, frequency: Uni
         raise ValueError("frequency must be one positive number, or one for each axis")
     if int(max_position) < 1:
         raise ValueError(f"max_position must be at least 1, got {max_position}")
-    position = torch.arange(int(max_position), device=device, dtype=torch.float64)
-    angles = torch.cat([position[:, None] * f ** (-torch.arange(0, w, 2, device=device, dtype=torch.float64) / w)
-                        for w, f in zip(widths, bases)], 1)
-    return RotaryAxes(widths, angles.cos().float().contiguous(), angles.sin().float().contiguous())
+    with torch.inference_mode(False):  # kept across calls: tables made during inference serve training too
+        position = torch.arange(int(max_position), device=device, dtype=torch.float64)
+        angles = torch.cat([position[:, None] * f ** (-torch.arange(0, w, 2, device=device, dtype=torch.float64) / w)
+                            for w, f in zip(widths, bases)], 1)
+        return RotaryAxes(widths, angles.cos().float().contiguous(), angles.sin().float().contiguous())
 
 
 def _strides(x):

@@ -137,3 +137,12 @@ def test_pointers_between_the_words_that_they_point_to_are_refused(lib):
     for call, names in ((fwd, ("cu_q", "cu_k", "lse", "status")), (bwd, ("cu_q", "cu_k", "lse", "status", "ws"))):
         for name in names:
             assert call(**{name: odd}) == -1, name
+
+
+def test_tables_made_during_inference_serve_training():
+    from geoweave_b200.rotary import rotary_axes
+
+    with torch.inference_mode():
+        axes = rotary_axes((16, 24, 24), 50, "cpu")
+    assert not axes.cos.is_inference() and not axes.sin.is_inference()  # an inference tensor cannot be kept for a backward pass
+    (torch.ones(50, 32, requires_grad=True) * axes.cos).sum().backward()
